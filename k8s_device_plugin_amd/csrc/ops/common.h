@@ -1,0 +1,171 @@
+/* Shared pieces of the head operators (gfx950 only): element types, vector
+ * loads, wave reductions, activations and the C interface's structures.
+ *
+ * Sums, statistics and accumulators are held in fp32; values are rounded to
+ * the tensors' type once, when they are stored.
+ */
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+typedef __bf16 bf16;
+typedef _Float16 fp16;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+enum DType { DT_F32 = 0, DT_BF16 = 1, DT_FP16 = 2 };
+enum Act { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
+
+/* What the entry points return beside HIP's own codes (which are >= 0). */
+enum { OPS_BAD_ARG = -1 };
+
+template <typename T>
+struct Vec { /* 16 bytes of T */
+  static constexpr int N = 16 / sizeof(T);
+  typedef T type __attribute__((ext_vector_type(N)));
+};
+
+template <typename T>
+__device__ inline float to_f(T v) { return (float)v; }
+template <typename T>
+__device__ inline T from_f(float v) { return (T)v; }
+
+/* n <= Vec<T>::N values at p, in one access where all N are there.  Global
+ * accesses of 16 bytes need no alignment beyond the element's, so rows of an
+ * odd width or start take the same path. */
+template <typename T>
+struct Loose {
+  typedef T type __attribute__((ext_vector_type(Vec<T>::N), aligned(sizeof(T))));
+};
+
+template <typename T>
+__device__ inline void load_vec(const T *p, int n, float *out) {
+  constexpr int V = Vec<T>::N;
+  if (n >= V) {
+    typename Loose<T>::type v = *(const typename Loose<T>::type *)p;
+#pragma unroll
+    for (int i = 0; i < V; i++) out[i] = to_f<T>(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++) out[i] = i < n ? to_f<T>(p[i]) : 0.f;
+  }
+}
+
+template <typename T>
+__device__ inline void store_vec(T *p, int n, const float *in) {
+  constexpr int V = Vec<T>::N;
+  if (n >= V) {
+    typename Loose<T>::type v;
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = from_f<T>(in[i]);
+    *(typename Loose<T>::type *)p = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++)
+      if (i < n) p[i] = from_f<T>(in[i]);
+  }
+}
+
+__device__ inline float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+/* y = act(z); the slope is dy/dz.  gelu is z Phi(z) with the error function. */
+__device__ inline float activate(float z, int act) {
+  if (act == ACT_RELU) return z > 0.f || z != z ? z : 0.f;
+  if (act == ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  if (act == ACT_SILU) return z / (1.f + __expf(-z));
+  return z;
+}
+
+__device__ inline float slope(float z, int act) {
+  if (act == ACT_RELU) return z > 0.f ? 1.f : 0.f;
+  if (act == ACT_GELU) {
+    float cdf = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+    return cdf + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+  }
+  if (act == ACT_SILU) {
+    float s = 1.f / (1.f + __expf(-z));
+    return s * (1.f + z * (1.f - s));
+  }
+  return 1.f;
+}
+
+/* y[m,n] = act(sum_k a[m,k] b[n,k] + bias[n]) + res[m,n].
+ * a_kc: a's element (m,k) is at a[m*lda + k]; otherwise at a[k*lda + m].
+ * Likewise b.  Extents are the bytes that may be read from a and b on. */
+struct GemmArgs {
+  const void *a, *b;
+  int64_t lda, ldb, a_extent, b_extent;
+  int64_t m, n, k;
+  const void *bias, *res;
+  int64_t ldr;
+  void *y;
+  int64_t ldy;
+  void *z; /* the value before the activation, where backward needs it */
+  int64_t ldz;
+  float *work; /* splits x m x n partial sums */
+  int32_t dtype, a_kc, b_kc, act;
+  int32_t plan, splits;
+};
+
+/* dz = dy act'(z) into rows of lddz elements with zeros behind n, and, in
+ * part [parts, n], sums of dz's columns over runs of rows. */
+struct SlopeArgs {
+  const void *dy, *z;
+  void *dz, *dbias;
+  float *part;
+  int64_t lddy, ldz, lddz, m, n;
+  int32_t dtype, act, parts;
+};
+
+/* Layer norm of each (row, group): x [rows, groups*d].  mean and rstd hold
+ * rows*groups values, part 2 x parts x groups*d partial sums of the weight's
+ * and bias's gradients. */
+struct NormArgs {
+  const void *x, *weight, *bias, *dy;
+  void *y, *dx, *dweight, *dbias;
+  float *mean, *rstd, *part;
+  int64_t ldx, ldy, lddy, lddx, rows, groups, d;
+  int32_t dtype, wtype;
+  int32_t parts;
+  float eps;
+};
+
+/* Distillation from a teacher's top logits.  rows_loss and lse hold one value a
+ * row, slot_p and slot_i `top` values a row, part 2 x chunks a row; count is
+ * the number of rows with a target. */
+struct DistillArgs {
+  const void *x, *index, *teacher;
+  void *dx;
+  const float *grad; /* of the loss: one value, or one a row */
+  float *rows_loss, *lse, *slot_p, *loss, *count;
+  int32_t *slot_i;
+  float *part;
+  int64_t ldx, lddx, ldi, ldt, rows, v;
+  int32_t dtype, ttype, index_bytes, top;
+  int32_t chunks, reduction; /* 0 none, 1 sum, 2 mean */
+  float temperature;
+};
+
+/* Column sums of part [parts, width] in a fixed order: 16 runs of rows a
+ * column, joined through LDS.  1024 threads for 64 columns. */
+template <typename W>
+__device__ inline void join_columns(const float *part, int64_t parts, int64_t width, W *out) {
+  __shared__ float lds[16][64];
+  int64_t col = (int64_t)blockIdx.x * 64 + threadIdx.x % 64;
+  int run = threadIdx.x / 64;
+  float s = 0.f;
+  if (col < width)
+    for (int64_t r = run; r < parts; r += 16) s += part[r * width + col];
+  lds[run][threadIdx.x % 64] = s;
+  __syncthreads();
+  if (run || col >= width) return;
+  for (int r = 1; r < 16; r++) s += lds[r][threadIdx.x];
+  if (out) out[col] = from_f<W>(s);
+}
+
+#define OPS_LAUNCHED() ((int)hipGetLastError())

@@ -1,0 +1,477 @@
+/* Matrix product with bias, activation and residual in its epilogue.
+ *
+ *   y = act(a b^T + bias) + res,   a [m,k], b [n,k], y [m,n]
+ *
+ * Either operand may lie with k contiguous or with k strided, so one kernel
+ * serves x W^T and both gradients (dz W and dz^T x) without a transposed copy.
+ */
+#include "common.h"
+
+#include <algorithm>
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+namespace {
+
+constexpr uint32_t OUT_OF_RANGE = 0x80000000u; /* past any num_records below */
+constexpr int STAGE_BYTES = 128;               /* of k per row and stage */
+
+/* A fragment is what one lane gives one 64-byte step of k: 16 bytes.  Lane l
+ * holds row l%16 and, of the step's k, the (l/16)-th quarter. */
+template <typename T>
+struct Frag {
+  typename Vec<T>::type v;
+};
+
+__device__ inline f32x4 mma(const Frag<bf16> &a, const Frag<bf16> &b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
+}
+__device__ inline f32x4 mma(const Frag<fp16> &a, const Frag<fp16> &b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v, b.v, c, 0, 0, 0);
+}
+/* Step j takes element j of every lane: both operands number k alike, so the
+ * order in which k is summed is free. */
+__device__ inline f32x4 mma(const Frag<float> &a, const Frag<float> &b, f32x4 c) {
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
+  return c;
+}
+
+/* One operand's tile of R rows (of m or n) by 128 bytes of k in LDS, filled
+ * by loads that go to LDS directly: lane l of a wave writes base + 16 l, so
+ * the order of 16-byte chunks is chosen by which chunk a lane asks for.
+ *
+ * k contiguous: rows of 8 chunks, chunk c of row r at c ^ ((r >> 1) & 7): the
+ * 16 rows that a fragment reads at once fall on all 64 banks.
+ * k strided: rows are k; a 16-bit fragment is read with the transposing read
+ * (4 rows of k by 16 columns), so 32-byte pieces of rows that are read
+ * together are spread by xor; fp32 reads 64-byte pieces of 4 rows. */
+template <typename T, bool KC, int R, int THREADS>
+struct Tile {
+  static constexpr int E = Vec<T>::N;
+  static constexpr int LOADS = R * STAGE_BYTES / (THREADS * 16);
+  static constexpr int ROW_CHUNKS = R / E; /* k strided */
+  static constexpr int BYTES = R * STAGE_BYTES;
+  static_assert(LOADS * THREADS * 16 == BYTES, "whole loads");
+  static_assert(KC || ROW_CHUNKS >= 8, "room for the xor");
+  uint32_t off[LOADS];
+  int kpos[LOADS]; /* first k of the chunk within the stage */
+
+  static __device__ int spread(int k) {
+    if (sizeof(T) == 4) return ((k >> 2) & 3) << 2;
+    int s = ((k & 3) | (((k >> 3) & 1) << 2)) << 1;
+    return ROW_CHUNKS >= 16 ? s : s & 7;
+  }
+
+  __device__ void init(int64_t ld, int64_t rows_left, int tid) {
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+      int q = i * THREADS + tid;
+      if (KC) {
+        int r = q >> 3, c = (q & 7) ^ ((r >> 1) & 7);
+        kpos[i] = c * E;
+        off[i] = r < rows_left ? (uint32_t)(r * ld * sizeof(T)) + c * 16 : OUT_OF_RANGE;
+      } else {
+        int k = q / ROW_CHUNKS, c = (q % ROW_CHUNKS) ^ spread(k);
+        kpos[i] = k;
+        off[i] = c * E < rows_left ? (uint32_t)(k * ld * sizeof(T)) + c * 16 : OUT_OF_RANGE;
+      }
+    }
+  }
+
+  /* Chunks past the end of k come as zeros. */
+  __device__ void load(const char *base, int64_t extent, int64_t k_left, char *lds, int wave) {
+    int records = (int)min(max(extent, (int64_t)0), (int64_t)0x7ffffff0);
+    __amdgpu_buffer_rsrc_t rsrc =
+        __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, records, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+      uint32_t o = kpos[i] < k_left ? off[i] : OUT_OF_RANGE;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc, (lds_void *)(lds + (i * THREADS + wave * 64) * 16), 16, o, 0, 0, 0);
+    }
+  }
+
+  /* The fragment of rows row0 .. row0+15 at step `step` (0 or 1). */
+  static __device__ Frag<T> frag(const char *lds, int row0, int step, int lane) {
+    int i = lane & 15, g = lane >> 4;
+    Frag<T> f;
+    if constexpr (KC) {
+      int c = (step * 4 + g) ^ ((i >> 1) & 7);
+      f.v = *(const typename Vec<T>::type *)(lds + (row0 + i) * STAGE_BYTES + c * 16);
+    } else if constexpr (sizeof(T) == 4) {
+      int c = ((row0 + i) >> 2) ^ (g << 2);
+      const char *p = lds + (step * 16 + 4 * g) * (R * 4) + c * 16 + (i & 3) * 4;
+#pragma unroll
+      for (int j = 0; j < 4; j++) f.v[j] = *(const float *)(p + j * (R * 4));
+    } else {
+      int k = step * 32 + 8 * g + (i >> 2);
+      int c = ((row0 >> 3) + ((i & 3) >> 1)) ^ spread(k);
+      const char *p = lds + k * (R * 2) + c * 16 + (i & 1) * 8;
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      union {
+        s16x4 s[2];
+        typename Vec<T>::type v;
+      } u;
+      u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p);
+      u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 4 * (R * 2)));
+      f.v = u.v;
+    }
+    return f;
+  }
+};
+
+/* Four neighbouring columns of one row: bias, activation, residual, store.
+ * Accesses of four need no alignment beyond the element's. */
+template <typename T>
+struct Epilogue {
+  const T *bias, *res;
+  T *y, *z;
+  int64_t ldr, ldy, ldz, n;
+  int act;
+
+  __device__ Epilogue(const GemmArgs &p)
+      : bias((const T *)p.bias), res((const T *)p.res), y((T *)p.y), z((T *)p.z),
+        ldr(p.ldr), ldy(p.ldy), ldz(p.ldz), n(p.n), act(p.act) {}
+
+  __device__ void operator()(int64_t m, int64_t col, f32x4 v) const {
+    typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    if (col + 4 <= n) {
+      if (bias) {
+        four b = *(const four *)(bias + col);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] += to_f<T>(b[i]);
+      }
+      four o;
+      if (z) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = from_f<T>(v[i]);
+        *(four *)(z + m * ldz + col) = o;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] = activate(v[i], act);
+      if (res) {
+        four r = *(const four *)(res + m * ldr + col);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] += to_f<T>(r[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[i] = from_f<T>(v[i]);
+      *(four *)(y + m * ldy + col) = o;
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      int64_t c = col + i;
+      if (c >= n) return;
+      float u = v[i];
+      if (bias) u += to_f<T>(bias[c]);
+      if (z) z[m * ldz + c] = from_f<T>(u);
+      u = activate(u, act);
+      if (res) u += to_f<T>(res[m * ldr + c]);
+      y[m * ldy + c] = from_f<T>(u);
+    }
+  }
+};
+
+/* Workgroups are dealt to the 8 XCDs in turn; give each XCD a run of tiles
+ * that share rows of a and b in its own L2, in bands of 8 tiles of m. */
+__device__ inline void tile_of(int block, int blocks, int tiles_m, int tiles_n, int *tm, int *tn) {
+  int q = blocks / 8, r = blocks % 8, xcd = block % 8;
+  int t = xcd * q + min(xcd, r) + block / 8;
+  constexpr int BAND = 8;
+  int band = t / (BAND * tiles_n), first = band * BAND;
+  int height = min(BAND, tiles_m - first);
+  int in = t - first * tiles_n;
+  *tm = first + in % height;
+  *tn = in / height;
+}
+
+/* A TM x TN tile of y per workgroup of WR x WC waves, two stages of LDS: the
+ * loads of a stage run while the one before is multiplied, and one barrier a
+ * stage both publishes the new one and frees the old one. */
+template <typename T, bool AKC, bool BKC, int TM, int TN, int WR, int WC>
+__global__ __launch_bounds__(WR *WC * 64) void gemm_tile(GemmArgs p) {
+  constexpr int THREADS = WR * WC * 64;
+  constexpr int BK = STAGE_BYTES / sizeof(T);
+  constexpr int FM = TM / WR / 16, FN = TN / WC / 16;
+  using TA = Tile<T, AKC, TM, THREADS>;
+  using TB = Tile<T, BKC, TN, THREADS>;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * (TA::BYTES + TB::BYTES)];
+
+  int tid = threadIdx.x, lane = tid & 63;
+  int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int tiles_m = (int)((p.m + TM - 1) / TM), tiles_n = (int)((p.n + TN - 1) / TN);
+  int tm, tn;
+  tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, &tm, &tn);
+  int64_t m0 = (int64_t)tm * TM, n0 = (int64_t)tn * TN;
+  int64_t stages_all = (p.k + BK - 1) / BK;
+  int64_t s0 = stages_all * blockIdx.y / p.splits, s1 = stages_all * (blockIdx.y + 1) / p.splits;
+
+  TA ta;
+  TB tb;
+  ta.init(p.lda, p.m - m0, tid);
+  tb.init(p.ldb, p.n - n0, tid);
+  auto fetch = [&](int64_t s) {
+    int64_t k = s * BK;
+    int64_t oa = (AKC ? m0 * p.lda + k : k * p.lda + m0) * (int64_t)sizeof(T);
+    int64_t ob = (BKC ? n0 * p.ldb + k : k * p.ldb + n0) * (int64_t)sizeof(T);
+    char *at = lds + (s & 1) * (TA::BYTES + TB::BYTES);
+    ta.load((const char *)p.a + oa, p.a_extent - oa, p.k - k, at, wave);
+    tb.load((const char *)p.b + ob, p.b_extent - ob, p.k - k, at + TA::BYTES, wave);
+  };
+
+  f32x4 acc[FM][FN] = {};
+  int wm = wave / WC * (TM / WR), wn = wave % WC * (TN / WC);
+  if (s0 < s1) fetch(s0);
+  for (int64_t s = s0; s < s1; s++) {
+    __builtin_amdgcn_s_waitcnt(0x0f70); /* vmcnt(0) */
+    __syncthreads();
+    if (s + 1 < s1) fetch(s + 1);
+    const char *la = lds + (s & 1) * (TA::BYTES + TB::BYTES), *lb = la + TA::BYTES;
+#pragma unroll
+    for (int step = 0; step < 2; step++) {
+      Frag<T> fa[FM], fb[FN];
+#pragma unroll
+      for (int j = 0; j < FN; j++) fb[j] = TB::frag(lb, wn + j * 16, step, lane);
+#pragma unroll
+      for (int i = 0; i < FM; i++) fa[i] = TA::frag(la, wm + i * 16, step, lane);
+#pragma unroll
+      for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
+    }
+  }
+
+  /* b is the first operand of the product, so a lane holds 4 neighbouring
+   * columns of row lane%16.  Each wave turns its part through its own piece
+   * of LDS, so that rows are stored whole and the epilogue's code is there
+   * once; 16-byte pieces are spread by xor over the banks. */
+  constexpr int WM = TM / WR, WN = TN / WC, PIECES = WN / 4;
+  constexpr int PIECE_LDS = (int)sizeof(lds) / (WR * WC);
+  constexpr int ROWS = PIECE_LDS / (WN * 4) < WM ? PIECE_LDS / (WN * 4) : WM;
+  static_assert(ROWS % 16 == 0 && WM % ROWS == 0, "whole fragments a pass");
+  __syncthreads();
+  float *mine = (float *)(lds + wave * PIECE_LDS);
+  Epilogue<T> store(p);
+  float *part = p.work + (int64_t)blockIdx.y * p.m * p.n;
+#pragma unroll
+  for (int pass = 0; pass < WM / ROWS; pass++) {
+#pragma unroll
+    for (int i = 0; i < ROWS / 16; i++)
+#pragma unroll
+      for (int j = 0; j < FN; j++) {
+        int r = i * 16 + (lane & 15), c = (j * 4 + (lane >> 4)) ^ (r & (PIECES - 1));
+        *(f32x4 *)(mine + r * WN + c * 4) = acc[pass * (ROWS / 16) + i][j];
+      }
+#pragma unroll 1
+    for (int q = lane; q < ROWS * PIECES; q += 64) {
+      int r = q / PIECES, c = q % PIECES;
+      f32x4 v = *(const f32x4 *)(mine + r * WN + (c ^ (r & (PIECES - 1))) * 4);
+      int64_t m = m0 + wm + pass * ROWS + r, n = n0 + wn + c * 4;
+      if (m >= p.m || n >= p.n) continue;
+      if (p.splits == 1) {
+        store(m, n, v);
+      } else if (p.n % 4 == 0) {
+        *(f32x4 *)(part + m * p.n + n) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (n + e < p.n) part[m * p.n + n + e] = v[e];
+      }
+    }
+  }
+}
+
+/* Adds the splits' partial sums in their order and finishes the rows. */
+template <typename T>
+__global__ __launch_bounds__(256) void gemm_join(GemmArgs p) {
+  int64_t fours = (p.n + 3) / 4;
+  int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= p.m * fours) return;
+  int64_t m = at / fours, n = at % fours * 4;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  const float *q = p.work + m * p.n + n;
+  if (n + 4 <= p.n && p.n % 4 == 0) {
+    for (int s = 0; s < p.splits; s++) v += *(const f32x4 *)(q + (int64_t)s * p.m * p.n);
+  } else {
+    for (int s = 0; s < p.splits; s++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (n + e < p.n) v[e] += q[(int64_t)s * p.m * p.n + e];
+  }
+  Epilogue<T> store(p);
+  store(m, n, v);
+}
+
+template <typename T, bool AKC, bool BKC>
+void launch_tile(const GemmArgs &p, hipStream_t stream) {
+  auto blocks = [&](int tm, int tn) {
+    return dim3((unsigned)(((p.m + tm - 1) / tm) * ((p.n + tn - 1) / tn)), (unsigned)p.splits);
+  };
+  if (p.plan == 0)
+    gemm_tile<T, AKC, BKC, 256, 256, 2, 4><<<blocks(256, 256), 512, 0, stream>>>(p);
+  else if (p.plan == 1)
+    gemm_tile<T, AKC, BKC, 128, 128, 2, 2><<<blocks(128, 128), 256, 0, stream>>>(p);
+  else
+    gemm_tile<T, AKC, BKC, 64, 64, 2, 2><<<blocks(64, 64), 256, 0, stream>>>(p);
+}
+
+template <typename T>
+int run(const GemmArgs &p, hipStream_t stream) {
+  if (p.a_kc && p.b_kc) launch_tile<T, true, true>(p, stream);
+  else if (p.a_kc) launch_tile<T, true, false>(p, stream);
+  else if (p.b_kc) launch_tile<T, false, true>(p, stream);
+  else launch_tile<T, false, false>(p, stream);
+  if (p.splits > 1) {
+    int64_t items = p.m * ((p.n + 3) / 4);
+    gemm_join<T><<<(unsigned)((items + 255) / 256), 256, 0, stream>>>(p);
+  }
+  return OPS_LAUNCHED();
+}
+
+/* [rows, cols] of any strides to rows of `ld` elements, zeros behind. */
+template <typename T>
+__global__ __launch_bounds__(256) void repack(const T *src, int64_t rs, int64_t cs, int64_t rows,
+                                              int64_t cols, T *dst, int64_t ld) {
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
+    for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < ld; c += (int64_t)gridDim.x * 256)
+      dst[r * ld + c] = c < cols ? src[r * rs + c * cs] : (T)0;
+}
+
+/* A workgroup's four waves share 64 vectors of columns; wave w takes rows w,
+ * w+4, ... of the workgroup's run of rows. */
+template <typename T>
+__global__ __launch_bounds__(256) void slope_rows(SlopeArgs p) {
+  constexpr int V = Vec<T>::N;
+  __shared__ float lds[3][64][V + 1];
+  int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  int64_t col = ((int64_t)blockIdx.x * 64 + lane) * V;
+  int n = (int)max((int64_t)0, min((int64_t)V, p.n - col));
+  int64_t from = p.m * blockIdx.y / p.parts, to = p.m * (blockIdx.y + 1) / p.parts;
+  const T *dy = (const T *)p.dy, *z = (const T *)p.z;
+  T *dz = (T *)p.dz;
+  float sum[V] = {};
+  for (int64_t r = from + wave; r < to; r += 4) {
+    float g[V], u[V];
+    load_vec<T>(dy + r * p.lddy + col, n, g);
+    if (p.act != ACT_NONE) {
+      load_vec<T>(z + r * p.ldz + col, n, u);
+#pragma unroll
+      for (int e = 0; e < V; e++) g[e] *= slope(u[e], p.act);
+    }
+#pragma unroll
+    for (int e = 0; e < V; e++) sum[e] += g[e];
+    if (dz && col < p.lddz) store_vec<T>(dz + r * p.lddz + col, (int)min((int64_t)V, p.lddz - col), g);
+  }
+  if (!p.part) return;
+  if (wave)
+#pragma unroll
+    for (int e = 0; e < V; e++) lds[wave - 1][lane][e] = sum[e];
+  __syncthreads();
+  if (wave || n <= 0) return;
+#pragma unroll
+  for (int e = 0; e < V; e++)
+    for (int w = 0; w < 3; w++) sum[e] += lds[w][lane][e];
+  float *part = p.part + blockIdx.y * p.n + col;
+#pragma unroll
+  for (int e = 0; e < V; e++)
+    if (e < n) part[e] = sum[e];
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void slope_join(SlopeArgs p) {
+  join_columns<T>(p.part, p.parts, p.n, (T *)p.dbias);
+}
+
+template <typename T>
+int run_slope(const SlopeArgs &p, hipStream_t s) {
+  int64_t vecs = (std::max(p.n, p.dz ? p.lddz : p.n) + Vec<T>::N - 1) / Vec<T>::N;
+  slope_rows<T><<<dim3((unsigned)((vecs + 63) / 64), (unsigned)p.parts), 256, 0, s>>>(p);
+  if (p.part) slope_join<T><<<(unsigned)((p.n + 63) / 64), 1024, 0, s>>>(p);
+  return OPS_LAUNCHED();
+}
+
+}  // namespace
+
+extern "C" {
+
+/* Into how many runs of rows the columns' sums are cut: about four
+ * workgroups a CU, and at least 8 rows each. */
+int32_t vgpu_ops_slope_parts(int64_t m, int64_t n, int32_t dtype) {
+  int64_t per = 64 * (dtype == DT_F32 ? 4 : 8), blocks = (n + per - 1) / per;
+  return (int32_t)std::max<int64_t>(1, std::min<int64_t>((m + 7) / 8, 1024 / blocks));
+}
+
+int vgpu_ops_slope(const SlopeArgs *args, void *stream) {
+  const SlopeArgs &p = *args;
+  if (p.m <= 0 || p.n <= 0 || p.parts < 1 || p.parts > 65535 || (p.dz && p.lddz < p.n) ||
+      (p.act != ACT_NONE && !p.z) || (p.dbias && !p.part))
+    return OPS_BAD_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  if (p.dtype == DT_F32) return run_slope<float>(p, s);
+  if (p.dtype == DT_BF16) return run_slope<bf16>(p, s);
+  if (p.dtype == DT_FP16) return run_slope<fp16>(p, s);
+  return OPS_BAD_ARG;
+}
+
+/* Which tile, and over how many parts k is split, from the sizes alone.
+ * A split adds a pass over fp32 partial sums, so it is taken only while there
+ * are fewer tiles than CUs and each part keeps 4 stages. */
+void vgpu_ops_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t *plan,
+                        int32_t *splits) {
+  const int side[3] = {256, 128, 64};
+  int64_t stages = (k * (dtype == DT_F32 ? 4 : 2) + STAGE_BYTES - 1) / STAGE_BYTES;
+  int64_t tiles = 0;
+  for (*plan = 0; *plan < 3; ++*plan) {
+    int s = side[*plan];
+    tiles = ((m + s - 1) / s) * ((n + s - 1) / s);
+    if (tiles >= 256) break;
+  }
+  *splits = 1;
+  if (*plan == 3) {
+    *plan = tiles >= 128 ? 2 : (m > 64 && n > 64 ? 1 : 2);
+    int s = side[*plan];
+    tiles = ((m + s - 1) / s) * ((n + s - 1) / s);
+    *splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, stages / 4, 64}));
+  }
+}
+
+int vgpu_ops_gemm(const GemmArgs *args, void *stream) {
+  const GemmArgs &p = *args;
+  if (p.m <= 0 || p.n <= 0 || p.k < 0 || p.splits < 1 || p.plan < 0 || p.plan > 2 ||
+      (p.splits > 1 && !p.work))
+    return OPS_BAD_ARG;
+  int size = p.dtype == DT_F32 ? 4 : 2;
+  /* 16-byte loads at 32-bit offsets inside a tile; a k that is contiguous is
+   * read in whole chunks */
+  if ((uintptr_t)p.a % 16 || (uintptr_t)p.b % 16 || p.lda * size % 16 || p.ldb * size % 16 ||
+      ((p.a_kc || p.b_kc) && p.k * size % 16) || p.lda < 0 || p.ldb < 0 ||
+      p.lda * size >= (1 << 23) || p.ldb * size >= (1 << 23))
+    return OPS_BAD_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  if (p.dtype == DT_F32) return run<float>(p, s);
+  if (p.dtype == DT_BF16) return run<bf16>(p, s);
+  if (p.dtype == DT_FP16) return run<fp16>(p, s);
+  return OPS_BAD_ARG;
+}
+
+int vgpu_ops_repack(const void *src, int64_t rs, int64_t cs, int64_t rows, int64_t cols, void *dst,
+                    int64_t ld, int32_t dtype, void *stream) {
+  if (rows <= 0 || cols < 0 || ld < cols || ld <= 0) return OPS_BAD_ARG;
+  dim3 grid((unsigned)std::min<int64_t>((ld + 255) / 256, 1024),
+            (unsigned)std::min<int64_t>(rows, 16384));
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == DT_F32)
+    repack<float><<<grid, 256, 0, s>>>((const float *)src, rs, cs, rows, cols, (float *)dst, ld);
+  else if (dtype == DT_BF16 || dtype == DT_FP16) /* bits only */
+    repack<uint16_t><<<grid, 256, 0, s>>>((const uint16_t *)src, rs, cs, rows, cols,
+                                          (uint16_t *)dst, ld);
+  else
+    return OPS_BAD_ARG;
+  return OPS_LAUNCHED();
+}
+
+}  // extern "C"

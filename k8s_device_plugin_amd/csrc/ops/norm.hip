@@ -1,0 +1,254 @@
+/* Layer norm over groups of d neighbouring values, forward and backward.
+ *
+ *   y = h w + b,  h = (x - mean) rstd        (per row and group)
+ *   dx = rstd (a - mean(a) - h mean(a h)),   a = dy w
+ *   dw = sum over rows of dy h,  db = sum over rows of dy
+ *
+ * Bound by memory: a row is read once and stays in registers between its
+ * statistics and its result; the variance is taken around the mean, in fp32.
+ */
+#include "common.h"
+
+#include <algorithm>
+
+namespace {
+
+/* The sum over the TH threads of a row; every one of them gets it.  Waves
+ * join through LDS, in their order; TH = 64 is one wave. */
+template <int TH, int COUNT>
+__device__ inline void row_sum(float (&v)[COUNT], float *lds) {
+#pragma unroll
+  for (int c = 0; c < COUNT; c++) v[c] = wave_sum(v[c]);
+  if constexpr (TH > 64) {
+    constexpr int WAVES = TH / 64;
+    __syncthreads(); /* the last use of lds is over */
+    if (threadIdx.x % 64 == 0)
+#pragma unroll
+      for (int c = 0; c < COUNT; c++) lds[c * WAVES + threadIdx.x / 64] = v[c];
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < COUNT; c++) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < WAVES; w++) s += lds[c * WAVES + w];
+      v[c] = s;
+    }
+  }
+}
+
+/* Rows of up to 64 lanes' worth take a wave each, four waves a workgroup. */
+template <int TH>
+constexpr int rows_at_once() { return TH == 64 ? 4 : 1; }
+template <int TH>
+constexpr int block_of() { return TH == 64 ? 256 : TH; }
+
+template <typename T, typename W, int TH, int VECS>
+__global__ __launch_bounds__(block_of<TH>()) void norm_forward(NormArgs p) {
+  constexpr int V = Vec<T>::N;
+  __shared__ float lds[TH / 64];
+  int lane = threadIdx.x % TH;
+  int64_t row = (int64_t)blockIdx.x * rows_at_once<TH>() + threadIdx.x / TH;
+  if (row >= p.rows) return; /* a whole wave, and only where TH is 64 */
+  int64_t group = blockIdx.y, d = p.d;
+  const T *x = (const T *)p.x + row * p.ldx + group * d;
+  float v[VECS][V];
+  float s[1] = {0.f};
+#pragma unroll
+  for (int i = 0; i < VECS; i++) {
+    int64_t at = (int64_t)(i * TH + lane) * V;
+    int n = (int)min((int64_t)V, d - at);
+    load_vec<T>(x + at, n, v[i]);
+#pragma unroll
+    for (int e = 0; e < V; e++) s[0] += v[i][e];
+  }
+  row_sum<TH>(s, lds);
+  float mean = s[0] / d;
+  s[0] = 0.f;
+#pragma unroll
+  for (int i = 0; i < VECS; i++) {
+    int64_t at = (int64_t)(i * TH + lane) * V;
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      v[i][e] = at + e < d ? v[i][e] - mean : 0.f;
+      s[0] += v[i][e] * v[i][e];
+    }
+  }
+  row_sum<TH>(s, lds);
+  float rstd = 1.f / sqrtf(s[0] / d + p.eps);
+  if (lane == 0 && p.mean) {
+    p.mean[row * p.groups + group] = mean;
+    p.rstd[row * p.groups + group] = rstd;
+  }
+  const W *w = (const W *)p.weight + group * d, *b = (const W *)p.bias + group * d;
+  T *y = (T *)p.y + row * p.ldy + group * d;
+#pragma unroll
+  for (int i = 0; i < VECS; i++) {
+    int64_t at = (int64_t)(i * TH + lane) * V;
+    int n = (int)min((int64_t)V, d - at);
+    if (n <= 0) continue;
+    float o[V];
+#pragma unroll
+    for (int e = 0; e < V; e++) o[e] = v[i][e] * rstd;
+    if (p.weight) {
+      float t[V];
+      constexpr int VW = Vec<W>::N;
+#pragma unroll
+      for (int h = 0; h < V; h += VW) load_vec<W>(w + at + h, n - h, t + h);
+#pragma unroll
+      for (int e = 0; e < V; e++) o[e] *= t[e];
+    }
+    if (p.bias) {
+      float t[V];
+      constexpr int VW = Vec<W>::N;
+#pragma unroll
+      for (int h = 0; h < V; h += VW) load_vec<W>(b + at + h, n - h, t + h);
+#pragma unroll
+      for (int e = 0; e < V; e++) o[e] += t[e];
+    }
+    store_vec<T>(y + at, n, o);
+  }
+}
+
+/* Each row (or wave) of the grid takes every parts-th row, keeps its columns'
+ * sums of dy h and dy in registers and writes them once, so x and dy are read
+ * a single time for all three gradients. */
+template <typename T, typename W, int TH, int VECS>
+__global__ __launch_bounds__(block_of<TH>()) void norm_backward(NormArgs p) {
+  constexpr int V = Vec<T>::N;
+  __shared__ float lds[2 * (TH / 64)];
+  int lane = threadIdx.x % TH;
+  int64_t part = (int64_t)blockIdx.x * rows_at_once<TH>() + threadIdx.x / TH;
+  int64_t group = blockIdx.y, d = p.d;
+  const W *w = (const W *)p.weight + group * d;
+  float dw[VECS][V] = {}, db[VECS][V] = {};
+  for (int64_t row = part; row < p.rows; row += p.parts) {
+    const T *x = (const T *)p.x + row * p.ldx + group * d;
+    const T *dy = (const T *)p.dy + row * p.lddy + group * d;
+    float mean = p.mean[row * p.groups + group], rstd = p.rstd[row * p.groups + group];
+    float h[VECS][V], a[VECS][V];
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < VECS; i++) {
+      int64_t at = (int64_t)(i * TH + lane) * V;
+      int n = (int)min((int64_t)V, d - at);
+      load_vec<T>(x + at, n, h[i]);
+      load_vec<T>(dy + at, n, a[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < VECS; i++) {
+      int64_t at = (int64_t)(i * TH + lane) * V;
+      int n = (int)min((int64_t)V, d - at);
+      float t[V];
+      if (p.weight) {
+        constexpr int VW = Vec<W>::N;
+#pragma unroll
+        for (int c = 0; c < V; c += VW) load_vec<W>(w + at + c, n - c, t + c);
+      }
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        h[i][e] = e < n ? (h[i][e] - mean) * rstd : 0.f;
+        dw[i][e] += a[i][e] * h[i][e];
+        db[i][e] += a[i][e];
+        if (p.weight) a[i][e] *= t[e];
+        s[0] += a[i][e];
+        s[1] += a[i][e] * h[i][e];
+      }
+    }
+    if (!p.dx) continue; /* the same for all threads */
+    row_sum<TH>(s, lds);
+    float ma = s[0] / d, mah = s[1] / d;
+    T *dx = (T *)p.dx + row * p.lddx + group * d;
+#pragma unroll
+    for (int i = 0; i < VECS; i++) {
+      int64_t at = (int64_t)(i * TH + lane) * V;
+      int n = (int)min((int64_t)V, d - at);
+      float o[V];
+#pragma unroll
+      for (int e = 0; e < V; e++) o[e] = rstd * (a[i][e] - ma - h[i][e] * mah);
+      store_vec<T>(dx + at, n, o);
+    }
+  }
+  if (!p.part) return;
+  float *pw = p.part + part * p.groups * d + group * d, *pb = pw + (int64_t)p.parts * p.groups * d;
+#pragma unroll
+  for (int i = 0; i < VECS; i++) {
+    int64_t at = (int64_t)(i * TH + lane) * V;
+    int n = (int)min((int64_t)V, d - at);
+#pragma unroll
+    for (int c = 0; c < V; c += 4) {
+      store_vec<float>(pw + at + c, n - c, dw[i] + c);
+      store_vec<float>(pb + at + c, n - c, db[i] + c);
+    }
+  }
+}
+
+/* blockIdx.y: 0 the weight, 1 the bias. */
+template <typename W>
+__global__ __launch_bounds__(1024) void norm_join(NormArgs p) {
+  int64_t width = p.groups * p.d;
+  join_columns<W>(p.part + blockIdx.y * p.parts * width, p.parts, width,
+                  (W *)(blockIdx.y ? p.dbias : p.dweight));
+}
+
+template <typename T, typename W, int TH, int VALUES>
+void launch(const NormArgs &p, hipStream_t s) {
+  constexpr int VECS = VALUES / Vec<T>::N;
+  constexpr int R = rows_at_once<TH>();
+  if (p.dy)
+    norm_backward<T, W, TH, VECS>
+        <<<dim3(p.parts / R, (unsigned)p.groups), block_of<TH>(), 0, s>>>(p);
+  else
+    norm_forward<T, W, TH, VECS>
+        <<<dim3((unsigned)((p.rows + R - 1) / R), (unsigned)p.groups), block_of<TH>(), 0, s>>>(p);
+}
+
+/* The fewest threads whose registers hold the row, 32 values each at most. */
+template <typename T, typename W>
+void dispatch(const NormArgs &p, hipStream_t s) {
+  if (p.d <= 64 * 8) launch<T, W, 64, 8>(p, s);
+  else if (p.d <= 64 * 16) launch<T, W, 64, 16>(p, s);
+  else if (p.d <= 64 * 32) launch<T, W, 64, 32>(p, s);
+  else if (p.d <= 256 * 16) launch<T, W, 256, 16>(p, s);
+  else if (p.d <= 256 * 32) launch<T, W, 256, 32>(p, s);
+  else if (p.d <= 512 * 32) launch<T, W, 512, 32>(p, s);
+  else launch<T, W, 1024, 32>(p, s);
+  if (p.dy && p.part) {
+    int64_t width = p.groups * p.d;
+    norm_join<W><<<dim3((unsigned)((width + 63) / 64), 2), 1024, 0, s>>>(p);
+  }
+}
+
+template <typename T>
+int run(const NormArgs &p, hipStream_t s) {
+  if (p.wtype == DT_F32) dispatch<T, float>(p, s);
+  else if (p.wtype == p.dtype) dispatch<T, T>(p, s);
+  else return OPS_BAD_ARG;
+  return OPS_LAUNCHED();
+}
+
+}  // namespace
+
+extern "C" {
+
+/* How many partial sums of the weight's gradient: enough rows in flight for
+ * 256 CUs, no more than there are rows, whole workgroups. */
+int32_t vgpu_ops_norm_parts(int64_t rows, int64_t groups, int64_t d) {
+  int64_t at_once = d <= 2048 ? 4 : 1;
+  int64_t most = (d <= 2048 ? 2048 : 512) / std::min<int64_t>(groups, 32);
+  int64_t parts = std::max<int64_t>(1, std::min(rows, most));
+  return (int32_t)((parts + at_once - 1) / at_once * at_once);
+}
+
+int vgpu_ops_norm(const NormArgs *args, void *stream) {
+  const NormArgs &p = *args;
+  if (p.rows <= 0 || p.rows >= (int64_t)1 << 31 || p.groups <= 0 || p.groups > 65535 || p.d <= 0 ||
+      p.d > 1024 * 32 || (p.dy ? p.parts != vgpu_ops_norm_parts(p.rows, p.groups, p.d) : !p.y))
+    return OPS_BAD_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  if (p.dtype == DT_F32) return run<float>(p, s);
+  if (p.dtype == DT_BF16) return run<bf16>(p, s);
+  if (p.dtype == DT_FP16) return run<fp16>(p, s);
+  return OPS_BAD_ARG;
+}
+
+}  // extern "C"

@@ -1,0 +1,127 @@
+"""Loads libvgpu_ops.so (csrc/ops/*.hip) and holds its argument structures.
+
+The library is built in-tree by ``make native``.  On a GPU there is no other
+path: a missing library is an error, never a silent fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+from ctypes import POINTER, c_float, c_int32, c_int64, c_void_p
+from functools import lru_cache
+from pathlib import Path
+
+import torch
+
+PACKAGE = Path(__file__).resolve().parent.parent
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_PLAIN_TENSORS = (torch.Tensor, torch.nn.Parameter)
+
+
+def _struct(name, **groups):
+    fields = [(f, kind) for kind, names in groups.values() for f in names.split()]
+    return type(name, (ctypes.Structure,), {"_fields_": fields})
+
+
+GemmArgs = _struct(
+    "GemmArgs", a=(c_void_p, "a b"), b=(c_int64, "lda ldb a_extent b_extent m n k"),
+    c=(c_void_p, "bias res"), d=(c_int64, "ldr"), e=(c_void_p, "y"), f=(c_int64, "ldy"),
+    g=(c_void_p, "z"), h=(c_int64, "ldz"), i=(c_void_p, "work"),
+    j=(c_int32, "dtype a_kc b_kc act plan splits"))
+SlopeArgs = _struct(
+    "SlopeArgs", a=(c_void_p, "dy z dz dbias part"), b=(c_int64, "lddy ldz lddz m n"),
+    c=(c_int32, "dtype act parts"))
+NormArgs = _struct(
+    "NormArgs", a=(c_void_p, "x weight bias dy y dx dweight dbias mean rstd part"),
+    b=(c_int64, "ldx ldy lddy lddx rows groups d"), c=(c_int32, "dtype wtype parts"),
+    d=(c_float, "eps"))
+DistillArgs = _struct(
+    "DistillArgs",
+    a=(c_void_p, "x index teacher dx grad rows_loss lse slot_p loss count slot_i part"),
+    b=(c_int64, "ldx lddx ldi ldt rows v"),
+    c=(c_int32, "dtype ttype index_bytes top chunks reduction"), d=(c_float, "temperature"))
+
+
+@lru_cache(maxsize=None)
+def library() -> ctypes.CDLL:
+    # torch has loaded its HIP runtime by now; the library binds to that one
+    # by its soname, so streams and memory are shared
+    for path in (PACKAGE / "csrc" / "libvgpu_ops.so", PACKAGE.parent / "lib" / "libvgpu_ops.so"):
+        if path.exists():
+            break
+    else:
+        raise RuntimeError(
+            "libvgpu_ops.so is not built: run `make native` (hipcc, gfx950)")
+    lib = ctypes.CDLL(str(path))
+    for name, struct in (("gemm", GemmArgs), ("slope", SlopeArgs), ("norm", NormArgs),
+                         ("distill", DistillArgs)):
+        getattr(lib, "vgpu_ops_" + name).argtypes = [POINTER(struct), c_void_p]
+    lib.vgpu_ops_repack.argtypes = [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                    c_int64, c_int32, c_void_p]
+    lib.vgpu_ops_gemm_plan.argtypes = [c_int64, c_int64, c_int64, c_int32,
+                                       POINTER(c_int32), POINTER(c_int32)]
+    lib.vgpu_ops_gemm_plan.restype = None
+    lib.vgpu_ops_slope_parts.argtypes = [c_int64, c_int64, c_int32]
+    lib.vgpu_ops_norm_parts.argtypes = [c_int64, c_int64, c_int64]
+    lib.vgpu_ops_distill_chunks.argtypes = [c_int64, c_int64, c_int32]
+    return lib
+
+
+@lru_cache(maxsize=None)
+def _check_arch(device: int) -> None:
+    arch = torch.cuda.get_device_properties(device).gcnArchName
+    if not arch.startswith("gfx950"):
+        raise RuntimeError(f"the head operators are built for gfx950, not {arch}")
+
+
+def on_gpu(*tensors) -> bool:
+    """Whether the kernels run: ordinary tensors on a GPU, and nothing that
+    traces or transforms the call.  Otherwise the plain formula runs."""
+    for t in tensors:
+        if t is not None and (type(t) not in _PLAIN_TENSORS or not t.is_cuda):
+            return False
+    return not (torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None
+                or torch._C._are_functorch_transforms_active())
+
+
+def launch(name: str, args, device: torch.device) -> None:
+    """Runs an entry point on the device's current stream."""
+    index = device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return launch(name, args, device)
+    _check_arch(index)
+    rc = getattr(library(), "vgpu_ops_" + name)(
+        ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        raise RuntimeError(f"vgpu_ops_{name}: " + ("refused the arguments" if rc < 0
+                                                   else f"HIP error {rc}"))
+
+
+def needs_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
+    """[..., width] as a matrix whose rows are contiguous."""
+    m = t if t.dim() == 2 else t.reshape(-1, width)
+    return m if width == 1 or m.stride(1) == 1 else m.contiguous()
+
+
+def ptr(t) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def same_device(**tensors) -> None:
+    devices = {name: t.device for name, t in tensors.items() if t is not None}
+    if len(set(devices.values())) > 1:
+        raise ValueError("tensors on different devices: "
+                         + ", ".join(f"{n} on {d}" for n, d in devices.items()))
+
+
+def gradients_of(plain, inputs, needed, grad):
+    """The gradients with a graph of their own, for a second derivative: the
+    plain formula is run again and differentiated."""
+    with torch.enable_grad():
+        wanted = [t for t, need in zip(inputs, needed) if need]
+        found = iter(torch.autograd.grad(plain(*inputs), wanted, grad, create_graph=True))
+        return [next(found) if need else None for need in needed]

@@ -1,0 +1,121 @@
+"""Layer norm over groups of neighbouring values.
+
+    y = (x - mean) / sqrt(var + eps) * weight + bias
+
+The kernels are csrc/ops/norm.hip; statistics and the weight's gradient are
+summed in fp32.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn.functional as F
+
+from . import _native
+from ._native import DTYPES, NormArgs, launch, ptr, rows_of
+
+WIDEST = 32768  # values of a group: what one workgroup's registers hold
+
+
+def layer_norm(x, weight=None, bias=None, *, groups=1, eps=1e-5):
+    """Normalises each of ``groups`` equal parts of x's last axis, then scales
+    and shifts by weight and bias [x.shape[-1]]; differentiable.
+
+    ``groups=1`` is layer norm; more is group norm of rows that have no extent
+    beside their channels.  x: float32, bfloat16 or float16 on a GPU, any
+    strides, groups of at most 32768 values; weight and bias: x's type or
+    float32, both the same.  Under autocast x is normalised in float32, as by
+    torch's own.  On the CPU, and while a call is traced or transformed, the
+    formula is run by torch.  Runs on the current stream of x's device; can be
+    captured into a graph.  Results do not depend on the run.
+    """
+    if x.dim() < 1 or groups < 1 or x.shape[-1] == 0 or x.shape[-1] % groups:
+        raise ValueError(f"x {tuple(x.shape)} does not split into {groups} groups")
+    width = x.shape[-1]
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and t.shape != (width,):
+            raise ValueError(f"{name} {tuple(t.shape)}, wanted ({width},)")
+    if torch.is_autocast_enabled(x.device.type) and x.dtype != torch.float64:
+        x, weight, bias = (t if t is None else t.float() for t in (x, weight, bias))
+    kinds = {t.dtype for t in (weight, bias) if t is not None}
+    if len(kinds) > 1 or not kinds <= {x.dtype, torch.float32}:
+        raise TypeError(f"weight and bias are {kinds}: wanted both {x.dtype} or both float32")
+    _native.same_device(x=x, weight=weight, bias=bias)
+    if not _native.on_gpu(x, weight, bias):
+        return _plain(x, weight, bias, groups, eps)
+    if x.dtype not in DTYPES:
+        raise TypeError(f"layer_norm on a GPU takes float32, bfloat16 or float16, not {x.dtype}")
+    if width // groups > WIDEST or groups > 65535:
+        raise ValueError(f"layer_norm: groups of at most {WIDEST} values, at most 65535 groups")
+    if x.numel() == 0:
+        return _plain(x, weight, bias, groups, eps)
+    if _native.needs_grad(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, groups, eps)
+    return _forward(x, weight, bias, groups, eps, False)[0]
+
+
+def _plain(x, weight, bias, groups, eps):
+    kind = x.dtype if x.dtype == torch.float64 else torch.float32
+    y = F.layer_norm(x.to(kind).unflatten(-1, (groups, -1)), (x.shape[-1] // groups,), eps=eps)
+    y = y.flatten(-2)
+    if weight is not None:
+        y = y * weight
+    if bias is not None:
+        y = y + bias
+    return y.to(x.dtype)
+
+
+def _vector(t):
+    return t if t is None or t.numel() == 1 or t.stride(0) == 1 else t.contiguous()
+
+
+def _forward(x, weight, bias, groups, eps, keep):
+    width = x.shape[-1]
+    x2 = rows_of(x, width)
+    rows = x2.shape[0]
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = (torch.empty((2, rows * groups), dtype=torch.float32, device=x.device)
+             if keep else None)
+    weight, bias = _vector(weight), _vector(bias)
+    kind = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
+    at = ptr(stats)
+    launch("norm", NormArgs(
+        x2.data_ptr(), ptr(weight), ptr(bias), None, y.data_ptr(), None, None, None,
+        at, at and at + 4 * rows * groups, None, x2.stride(0), width, 0, 0, rows, groups,
+        width // groups, DTYPES[x.dtype], DTYPES[kind], 0, eps), x.device)
+    return y, stats
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps):
+        y, stats = _forward(x, weight, bias, groups, eps, True)
+        ctx.groups, ctx.eps = groups, eps
+        ctx.save_for_backward(x, weight, bias, stats)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        groups = ctx.groups
+        if torch.is_grad_enabled():
+            return (*_native.gradients_of(
+                lambda x, w, b: _plain(x, w, b, groups, ctx.eps), (x, weight, bias),
+                (need_x, need_w, need_b), dy), None, None)
+        width = x.shape[-1]
+        x2, dy2 = rows_of(x, width), rows_of(dy, width)
+        rows, d = x2.shape[0], width // groups
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        dw = torch.empty(width, dtype=weight.dtype, device=x.device) if need_w else None
+        db = torch.empty(width, dtype=bias.dtype, device=x.device) if need_b else None
+        parts = _native.library().vgpu_ops_norm_parts(rows, groups, d)
+        part = (torch.empty(2 * parts * width, dtype=torch.float32, device=x.device)
+                if need_w or need_b else None)
+        kind = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
+        weight = _vector(weight)
+        launch("norm", NormArgs(
+            x2.data_ptr(), ptr(weight), None, dy2.data_ptr(), None, ptr(dx), ptr(dw), ptr(db),
+            stats.data_ptr(), stats.data_ptr() + 4 * rows * groups, ptr(part), x2.stride(0), 0,
+            dy2.stride(0), width, rows, groups, d, DTYPES[x.dtype], DTYPES[kind], parts, ctx.eps),
+            x.device)
+        return dx, dw, db, None, None
