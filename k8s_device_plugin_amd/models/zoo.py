@@ -13,6 +13,10 @@ data and random-init weights (no network for datasets/checkpoints):
 
 ResNet-V2 = pre-activation bottlenecks (BN-ReLU-conv), matching the
 "resnet_v2" family the suite names.
+
+The models' heads (projection, the norm of DeepLab's pooled branch, the
+training loss) run through ``ops.linear``, ``ops.layer_norm`` and
+``ops.distill_loss``: gfx950 kernels on a GPU, torch's formula on the CPU.
 """
 from __future__ import annotations
 
@@ -22,6 +26,28 @@ from typing import Callable, Dict, List, Tuple
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from .. import ops
+from ..ops.matmul import formula
+
+
+class HeadLinear(nn.Linear):
+    """nn.Linear with its activation in the product's epilogue (ops.linear).
+    Parameters and state are nn.Linear's."""
+
+    def __init__(self, in_features, out_features, bias=True, activation="none"):
+        super().__init__(in_features, out_features, bias)
+        self.activation = activation
+
+    def forward(self, x):
+        # scripts, and 64 bits on a GPU, take torch's own
+        if torch.jit.is_scripting():
+            y = F.linear(x, self.weight, self.bias)
+            return F.relu(y) if self.activation == "relu" else y
+        else:
+            if x.dtype == torch.float64:
+                return formula(x, self.weight, self.bias, None, self.activation)
+            return ops.linear(x, self.weight, self.bias, activation=self.activation)
 
 
 # ---------------------------------------------------------------------------
@@ -67,7 +93,7 @@ class ResNetV2(nn.Module):
                 in_ch = w * PreActBottleneck.expansion
         self.blocks = nn.Sequential(*blocks)
         self.bn_final = nn.BatchNorm2d(in_ch)
-        self.fc = nn.Linear(in_ch, num_classes)
+        self.fc = HeadLinear(in_ch, num_classes)
 
     def forward(self, x):
         x = self.pool(self.stem(x))
@@ -104,9 +130,10 @@ class VGG16(nn.Module):
                 in_ch = v
         self.features = nn.Sequential(*layers)
         self.classifier = nn.Sequential(
-            nn.Linear(512 * 7 * 7, 4096), nn.ReLU(inplace=True), nn.Dropout(0.5),
-            nn.Linear(4096, 4096), nn.ReLU(inplace=True), nn.Dropout(0.5),
-            nn.Linear(4096, num_classes),
+            # Identity where the relu stood: layers keep their numbers
+            HeadLinear(512 * 7 * 7, 4096, activation="relu"), nn.Identity(), nn.Dropout(0.5),
+            HeadLinear(4096, 4096, activation="relu"), nn.Identity(), nn.Dropout(0.5),
+            HeadLinear(4096, num_classes),
         )
 
     def forward(self, x):
@@ -140,10 +167,23 @@ class ASPP(nn.Module):
             nn.Conv2d(out_ch * 5, out_ch, 1, bias=False),
             nn.BatchNorm2d(out_ch), nn.ReLU(inplace=True))
 
+    def pooled(self, x):
+        """self.gp(x).  On a 1x1 map the convolution is a matrix product and
+        the group norm a layer norm of each group's channels."""
+        if torch.jit.is_scripting():
+            return self.gp(x)
+        else:
+            if x.dtype == torch.float64:
+                return self.gp(x)
+            pool, conv, norm, act = self.gp
+            p = ops.linear(pool(x).flatten(1), conv.weight.flatten(1))
+            p = ops.layer_norm(p, norm.weight, norm.bias, groups=norm.num_groups, eps=norm.eps)
+            return act(p)[:, :, None, None]
+
     def forward(self, x):
         size = x.shape[-2:]
         feats = [b(x) for b in self.branches]
-        gp = F.interpolate(self.gp(x), size=size, mode="bilinear",
+        gp = F.interpolate(self.pooled(x), size=size, mode="bilinear",
                            align_corners=False)
         return self.project(torch.cat(feats + [gp], dim=1))
 
@@ -183,7 +223,7 @@ class LSTMNet(nn.Module):
         super().__init__()
         self.lstm = nn.LSTM(input_size, hidden, num_layers=layers,
                             batch_first=True)
-        self.fc = nn.Linear(hidden, num_classes)
+        self.fc = HeadLinear(hidden, num_classes)
 
     def forward(self, x):
         out, _ = self.lstm(x)
@@ -241,6 +281,30 @@ def build(case: BenchCase, device, dtype=torch.float32) -> nn.Module:
     return model
 
 
+def distilled_batch(case: BenchCase, teacher: nn.Module, batch, top: int):
+    """The batch with a teacher's top classes and their logits as its target."""
+    if case.seg:
+        raise ValueError(f"{case.name}: maps of classes are not distilled")
+    x, _ = batch
+    with torch.no_grad():
+        logits = teacher(x)
+    if logits.shape[-1] != case.num_classes:
+        raise ValueError(f"{case.name} has {case.num_classes} classes, "
+                         f"the teacher {logits.shape[-1]}")
+    values, index = logits.topk(top, dim=-1)
+    return x, (index, values)
+
+
+def loss_of(case: BenchCase, out, y):
+    """Cross entropy with labels, or the distance to a teacher's top logits."""
+    if case.seg:
+        return F.cross_entropy(out.float(), y)
+    index, teacher = y if isinstance(y, tuple) else (y.unsqueeze(1), None)
+    if out.dtype == torch.float64:
+        out = out.float()
+    return ops.distill_loss(out, index, teacher)
+
+
 def step(case: BenchCase, model: nn.Module, batch, optimizer=None) -> None:
     """One benchmark step: forward (inference) or fwd+loss+bwd+opt (training)."""
     x, y = batch
@@ -249,7 +313,7 @@ def step(case: BenchCase, model: nn.Module, batch, optimizer=None) -> None:
             model(x)
     else:
         out = model(x)
-        loss = F.cross_entropy(out.float(), y)
+        loss = loss_of(case, out, y)
         loss.backward()
         if optimizer is not None:
             optimizer.step()
@@ -272,16 +336,23 @@ def main(argv=None):
                    help="timed steps per case; 0 = run forever")
     p.add_argument("--warmup", type=int, default=5)
     p.add_argument("--device", default="cuda:0")
+    p.add_argument("--teacher", choices=list(CASES),
+                   help="train against the top logits of this case's model")
+    p.add_argument("--top-k", type=int, default=8,
+                   help="how many of the teacher's logits a sample keeps")
     args = p.parse_args(argv)
 
     names = list(CASES) if args.cases == "all" else [
         c.strip() for c in args.cases.split(",") if c.strip()]
     dev = torch.device(args.device)
     results = {}
+    teacher = build(CASES[args.teacher], dev).eval() if args.teacher else None
     for name in names:
         case = CASES[name]
         model = build(case, dev)
         batch = synthetic_batch(case, dev)
+        if teacher is not None and case.phase == "training":
+            batch = distilled_batch(case, teacher, batch, args.top_k)
         opt = (torch.optim.SGD(model.parameters(), lr=0.01, momentum=0.9)
                if case.phase == "training" else None)
         for _ in range(args.warmup):
