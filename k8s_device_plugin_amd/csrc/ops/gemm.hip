@@ -16,6 +16,8 @@ namespace {
 
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u; /* past any num_records below */
 constexpr int STAGE_BYTES = 128;               /* of k per row and stage */
+/* 0, 1, 2: tiles of 256, 128, 64 */
+constexpr int PLAN_ROWS = 3, PLAN_OUTER = 4;
 
 /* A fragment is what one lane gives one 64-byte step of k: 16 bytes.  Lane l
  * holds row l%16 and, of the step's k, the (l/16)-th quarter. */
@@ -306,6 +308,176 @@ __global__ __launch_bounds__(256) void gemm_join(GemmArgs p) {
   store(m, n, v);
 }
 
+/* Few rows (m <= 64): b is read once, at the memory's rate, straight into the
+ * matrix cores' registers.  A workgroup takes a strip of n; its eight waves
+ * share k between them, a step of 64 bytes of a's k at a time, and join in
+ * LDS.  FM is the number of 16-row pieces of a.
+ *
+ * k contiguous in b: the strip is 16 rows of b, a step 16 rows by 64 bytes.
+ * k strided: the strip is 16 lanes by 16 bytes of n, a step 4 V rows of k;
+ * lane i holds V neighbouring columns, of which the j-th go to the j-th
+ * product, so 16-bit values are only turned inside a lane. */
+template <typename T, bool BKC, int FM>
+__global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
+  constexpr int V = Vec<T>::N, WAVES = 8;
+  constexpr int FN = BKC ? 1 : V;          /* products a step */
+  constexpr int STRIP = 16 * FN;           /* columns of y */
+  constexpr int C = BKC ? (FM == 4 ? 4 : 8) : 1; /* steps a wave takes at once */
+  constexpr int LOADS = BKC ? 1 : V;       /* of b a step */
+  typedef typename Vec<T>::type vec;
+  __shared__ f32x4 lds[WAVES][16][STRIP / 4];
+
+  int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int64_t n0 = (int64_t)blockIdx.x * STRIP;
+  int64_t all = (p.k + 4 * V - 1) / (4 * V);
+  int64_t s0 = all * blockIdx.y / p.splits, s1 = all * (blockIdx.y + 1) / p.splits;
+  const char *a = (const char *)p.a;
+  const char *b = (const char *)p.b + n0 * (BKC ? p.ldb : 1) * (int64_t)sizeof(T);
+  int64_t b_left = p.b_extent - (b - (const char *)p.b);
+  int a_records = (int)min(p.a_extent, (int64_t)0x7ffffff0);
+  __amdgpu_buffer_rsrc_t ra =
+      __builtin_amdgcn_make_buffer_rsrc((void *)a, 0, a_records, 0x00020000);
+
+  uint32_t a_off[FM], b_off[LOADS];
+#pragma unroll
+  for (int f = 0; f < FM; f++)
+    a_off[f] = f * 16 + i < p.m ? (uint32_t)((f * 16 + i) * p.lda * sizeof(T)) + g * 16
+                                : OUT_OF_RANGE;
+#pragma unroll
+  for (int t = 0; t < LOADS; t++) {
+    if (BKC) b_off[t] = n0 + i < p.n ? (uint32_t)(i * p.ldb * sizeof(T)) + g * 16 : OUT_OF_RANGE;
+    else b_off[t] = n0 + i * V < p.n ? (uint32_t)((g * V + t) * p.ldb * sizeof(T)) + i * 16
+                                     : OUT_OF_RANGE;
+  }
+
+  struct Step {
+    u32x4 a[FM], b[LOADS];
+  };
+  auto fetch = [&](Step &q, int64_t s) {
+    bool in = s < s1 && (s * 4 + g) * V < p.k; /* k ends on a whole chunk of a */
+    uint32_t at = (uint32_t)(s * 64);
+#pragma unroll
+    for (int f = 0; f < FM; f++)
+      q.a[f] = __builtin_amdgcn_raw_buffer_load_b128(ra, in ? a_off[f] + at : OUT_OF_RANGE, 0, 0);
+    int64_t skip = BKC ? 0 : s * 4 * V * p.ldb * (int64_t)sizeof(T);
+    int records = (int)min(max(b_left - skip, (int64_t)0), (int64_t)0x7ffffff0);
+    __amdgpu_buffer_rsrc_t rb =
+        __builtin_amdgcn_make_buffer_rsrc((void *)(b + skip), 0, records, 0x00020000);
+#pragma unroll
+    for (int t = 0; t < LOADS; t++)
+      q.b[t] = __builtin_amdgcn_raw_buffer_load_b128(
+          rb, (BKC ? in : s < s1) ? b_off[t] + (BKC ? at : 0) : OUT_OF_RANGE, 0, 0);
+  };
+
+  f32x4 acc[FM][FN] = {};
+  auto multiply = [&](const Step &q) {
+    Frag<T> fb[FN];
+    if constexpr (BKC) {
+      fb[0].v = __builtin_bit_cast(vec, q.b[0]);
+    } else {
+      vec r[V];
+#pragma unroll
+      for (int t = 0; t < V; t++) r[t] = __builtin_bit_cast(vec, q.b[t]);
+#pragma unroll
+      for (int j = 0; j < V; j++)
+#pragma unroll
+        for (int t = 0; t < V; t++) fb[j].v[t] = r[t][j];
+    }
+#pragma unroll
+    for (int f = 0; f < FM; f++) {
+      Frag<T> fa;
+      fa.v = __builtin_bit_cast(vec, q.a[f]);
+#pragma unroll
+      for (int j = 0; j < FN; j++) acc[f][j] = mma(fb[j], fa, acc[f][j]);
+    }
+  };
+  for (int64_t s = s0 + wave * C; s < s1; s += WAVES * C) {
+    Step q[C];
+#pragma unroll
+    for (int c = 0; c < C; c++) fetch(q[c], s + c);
+#pragma unroll
+    for (int c = 0; c < C; c++) multiply(q[c]);
+  }
+
+  Epilogue<T> store(p);
+  float *part = p.work + (int64_t)blockIdx.y * p.m * p.n;
+#pragma unroll
+  for (int f = 0; f < FM; f++) {
+    if (f) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < FN; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        /* column (4 g + e) FN + j of the strip, row i */
+        int c = (4 * g + e) * FN + j;
+        ((float *)lds[wave][i])[c] = acc[f][j][e];
+      }
+    __syncthreads();
+    for (int q = threadIdx.x; q < 16 * (STRIP / 4); q += 512) {
+      int r = q / (STRIP / 4), c = q % (STRIP / 4);
+      int64_t m = f * 16 + r, n = n0 + c * 4;
+      if (m >= p.m || n >= p.n) continue;
+      f32x4 v = lds[0][r][c];
+#pragma unroll
+      for (int w = 1; w < WAVES; w++) v += lds[w][r][c];
+      if (p.splits == 1) {
+        store(m, n, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (n + e < p.n) part[m * p.n + n + e] = v[e];
+      }
+    }
+  }
+}
+
+/* A short sum (k <= 32) with k strided on both sides, as a weight's gradient
+ * from few rows is: bound by writing y.  A wave holds 8 rows by 64 vectors of
+ * columns; a's values are the same for the whole wave. */
+constexpr int OUTER_K = 32, OUTER_ROWS = 8;
+
+template <typename T>
+__global__ __launch_bounds__(256) void gemm_outer(GemmArgs p) {
+  constexpr int V = Vec<T>::N;
+  __shared__ float lds[OUTER_K][4 * OUTER_ROWS];
+  int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int64_t m0 = (int64_t)blockIdx.y * (4 * OUTER_ROWS);
+  const T *a = (const T *)p.a, *b = (const T *)p.b;
+  for (int q = threadIdx.x; q < p.k * 4 * OUTER_ROWS; q += 256) {
+    int k = q / (4 * OUTER_ROWS), r = q % (4 * OUTER_ROWS);
+    lds[k][r] = m0 + r < p.m ? to_f<T>(a[k * p.lda + m0 + r]) : 0.f;
+  }
+  __syncthreads();
+  int64_t n = ((int64_t)blockIdx.x * 64 + lane) * V;
+  int count = (int)max((int64_t)0, min((int64_t)V, p.n - n));
+  float acc[OUTER_ROWS][V] = {};
+  for (int k = 0; k < p.k; k++) {
+    float v[V];
+    load_vec<T>(b + k * p.ldb + n, count, v);
+#pragma unroll
+    for (int r = 0; r < OUTER_ROWS; r++) {
+      float w = lds[k][wave * OUTER_ROWS + r];
+#pragma unroll
+      for (int e = 0; e < V; e++) acc[r][e] += w * v[e];
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < OUTER_ROWS; r++) {
+    int64_t m = m0 + wave * OUTER_ROWS + r;
+    if (m < p.m) store_vec<T>((T *)p.y + m * p.ldy + n, count, acc[r]);
+  }
+}
+
+template <typename T, bool BKC>
+void launch_rows(const GemmArgs &p, hipStream_t stream) {
+  constexpr int STRIP = BKC ? 16 : 16 * Vec<T>::N;
+  dim3 grid((unsigned)((p.n + STRIP - 1) / STRIP), (unsigned)p.splits);
+  if (p.m <= 16) gemm_rows<T, BKC, 1><<<grid, 512, 0, stream>>>(p);
+  else if (p.m <= 32) gemm_rows<T, BKC, 2><<<grid, 512, 0, stream>>>(p);
+  else gemm_rows<T, BKC, 4><<<grid, 512, 0, stream>>>(p);
+}
+
 template <typename T, bool AKC, bool BKC>
 void launch_tile(const GemmArgs &p, hipStream_t stream) {
   auto blocks = [&](int tm, int tn) {
@@ -321,7 +493,15 @@ void launch_tile(const GemmArgs &p, hipStream_t stream) {
 
 template <typename T>
 int run(const GemmArgs &p, hipStream_t stream) {
-  if (p.a_kc && p.b_kc) launch_tile<T, true, true>(p, stream);
+  if (p.plan == PLAN_OUTER) {
+    dim3 grid((unsigned)((p.n + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N)),
+              (unsigned)((p.m + 4 * OUTER_ROWS - 1) / (4 * OUTER_ROWS)));
+    gemm_outer<T><<<grid, 256, 0, stream>>>(p);
+    return OPS_LAUNCHED();
+  }
+  if (p.plan == PLAN_ROWS && p.b_kc) launch_rows<T, true>(p, stream);
+  else if (p.plan == PLAN_ROWS) launch_rows<T, false>(p, stream);
+  else if (p.a_kc && p.b_kc) launch_tile<T, true, true>(p, stream);
   else if (p.a_kc) launch_tile<T, true, false>(p, stream);
   else if (p.b_kc) launch_tile<T, false, true>(p, stream);
   else launch_tile<T, false, false>(p, stream);
@@ -417,20 +597,33 @@ int vgpu_ops_slope(const SlopeArgs *args, void *stream) {
   return OPS_BAD_ARG;
 }
 
-/* Which tile, and over how many parts k is split, from the sizes alone.
- * A split adds a pass over fp32 partial sums, so it is taken only while there
- * are fewer tiles than CUs and each part keeps 4 stages. */
-void vgpu_ops_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t *plan,
-                        int32_t *splits) {
+/* Which kernel, and over how many parts k is split, from the sizes and the
+ * operands' layouts alone.  A split adds a pass over fp32 partial sums, so it
+ * is taken only while there are fewer workgroups than fill the 256 CUs, and
+ * each part keeps enough steps. */
+void vgpu_ops_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t a_kc, int32_t b_kc,
+                        int32_t bare, int32_t *plan, int32_t *splits) {
   const int side[3] = {256, 128, 64};
-  int64_t stages = (k * (dtype == DT_F32 ? 4 : 2) + STAGE_BYTES - 1) / STAGE_BYTES;
+  int64_t size = dtype == DT_F32 ? 4 : 2;
+  int64_t stages = (k * size + STAGE_BYTES - 1) / STAGE_BYTES;
+  *splits = 1;
+  if (k <= OUTER_K && !a_kc && !b_kc && bare && m <= 65535 * 4 * OUTER_ROWS) {
+    *plan = PLAN_OUTER;
+    return;
+  }
+  if (m <= 64 && a_kc) {
+    *plan = PLAN_ROWS;
+    int64_t strip = b_kc ? 16 : 256 / size, strips = (n + strip - 1) / strip;
+    int64_t steps = stages * 2;
+    *splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({512 / strips, steps / 64, 64}));
+    return;
+  }
   int64_t tiles = 0;
   for (*plan = 0; *plan < 3; ++*plan) {
     int s = side[*plan];
     tiles = ((m + s - 1) / s) * ((n + s - 1) / s);
     if (tiles >= 256) break;
   }
-  *splits = 1;
   if (*plan == 3) {
     *plan = tiles >= 128 ? 2 : (m > 64 && n > 64 ? 1 : 2);
     int s = side[*plan];
@@ -441,8 +634,12 @@ void vgpu_ops_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t 
 
 int vgpu_ops_gemm(const GemmArgs *args, void *stream) {
   const GemmArgs &p = *args;
-  if (p.m <= 0 || p.n <= 0 || p.k < 0 || p.splits < 1 || p.plan < 0 || p.plan > 2 ||
-      (p.splits > 1 && !p.work))
+  if (p.m <= 0 || p.n <= 0 || p.k < 0 || p.splits < 1 || p.plan < 0 ||
+      p.plan > PLAN_OUTER || (p.splits > 1 && !p.work))
+    return OPS_BAD_ARG;
+  if (p.plan == PLAN_ROWS && (p.m > 64 || !p.a_kc)) return OPS_BAD_ARG;
+  if (p.plan == PLAN_OUTER && (p.k > OUTER_K || p.a_kc || p.b_kc || p.bias || p.res || p.z ||
+                               p.act || p.splits > 1 || p.m > 65535 * 4 * OUTER_ROWS))
     return OPS_BAD_ARG;
   int size = p.dtype == DT_F32 ? 4 : 2;
   /* 16-byte loads at 32-bit offsets inside a tile; a k that is contiguous is

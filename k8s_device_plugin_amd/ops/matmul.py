@@ -69,17 +69,19 @@ def formula(x, weight, bias, residual, activation):
 
 
 @lru_cache(maxsize=4096)
-def _plan(m, n, k, dtype):
+def _plan(m, n, k, dtype, a_kc, b_kc, bare):
     plan, splits = ctypes.c_int32(), ctypes.c_int32()
-    _native.library().vgpu_ops_gemm_plan(m, n, k, dtype, ctypes.byref(plan), ctypes.byref(splits))
+    _native.library().vgpu_ops_gemm_plan(m, n, k, dtype, a_kc, b_kc, bare, ctypes.byref(plan),
+                                         ctypes.byref(splits))
     return plan.value, splits.value
 
 
-def _operand(t, zeros_behind=False):
+def _operand(t, any_axis=True):
     """A matrix [rows, k] as the kernel reads it: (tensor, ld, k contiguous,
     bytes that may be read, k).  Loads are 16 bytes wide, so rows that do not
     start on 16 bytes, or that end inside 16, are laid out anew with zeros
-    behind; so is a matrix that is contiguous along neither axis."""
+    behind; so is a matrix that is contiguous along neither axis, or not along
+    k where any_axis is false."""
     rows, k = t.shape
     s0, s1 = t.stride()
     size = t.element_size()
@@ -88,7 +90,7 @@ def _operand(t, zeros_behind=False):
             s0 = k
         if s1 == 1 and k * size % 16 == 0 and s0 * size % 16 == 0 and s0 * size < 1 << 23:
             return t, s0, 1, ((rows - 1) * s0 + k) * size, k
-        if s0 == 1 and s1 >= rows and s1 * size % 16 == 0 and s1 * size < 1 << 23:
+        if any_axis and s0 == 1 and s1 >= rows and s1 * size % 16 == 0 and s1 * size < 1 << 23:
             # the last row's last load is whole: its 16 bytes are one line's
             return t, s1, 0, -(-((k - 1) * s1 + rows) * size // 16) * 16, k
     wide = -(-k * size // 16) * 16 // size
@@ -108,12 +110,15 @@ def _gemm(a, b, out, bias=None, residual=None, act=0, z=None):
     """out [m, n] = act(a [m, k] b [n, k]^T + bias) + residual."""
     m, n = out.shape
     dtype = DTYPES[out.dtype]
-    a, lda, a_kc, a_extent, ka = _operand(a)
+    # few rows are read with k contiguous, but for the short sums of a
+    # weight's gradient
+    a, lda, a_kc, a_extent, ka = _operand(a, m > 64 or a.shape[1] <= 32)
     b, ldb, b_kc, b_extent, kb = _operand(b)
     # a k that one side pads with zeros ends beyond the other's extent, which
     # reads as zeros there too
     k = max(ka, kb)
-    plan, splits = _plan(m, n, k, dtype)
+    bare = bias is None and residual is None and z is None and not act
+    plan, splits = _plan(m, n, k, dtype, a_kc, b_kc, bare)
     work = (torch.empty(splits * m * n, dtype=torch.float32, device=out.device)
             if splits > 1 else None)
     launch("gemm", GemmArgs(
