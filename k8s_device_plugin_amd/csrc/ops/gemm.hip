@@ -8,6 +8,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 typedef __attribute__((address_space(3))) void lds_void;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -15,15 +16,18 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 namespace {
 
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u; /* past any num_records below */
-constexpr int STAGE_BYTES = 128;               /* of k per row and stage */
-/* 0, 1, 2: tiles of 256, 128, 64 */
-constexpr int PLAN_ROWS = 3, PLAN_OUTER = 4;
+constexpr int STEP_BYTES = 64; /* of k per row: what one fragment covers */
+constexpr int STEPS = 2;       /* a stage: whole lines of 128 bytes */
+/* 0 to 3: tiles of 256 x 256, 128 x 128, 64 x 128, 32 x 128 */
+constexpr int PLAN_ROWS = 4, PLAN_OUTER = 5;
 
 /* A fragment is what one lane gives one 64-byte step of k: 16 bytes.  Lane l
  * holds row l%16 and, of the step's k, the (l/16)-th quarter. */
 template <typename T>
 struct Frag {
   typename Vec<T>::type v;
+  /* instructions that read one from LDS */
+  static constexpr int reads(bool kc) { return kc ? 1 : sizeof(T) == 4 ? 4 : 2; }
 };
 
 __device__ inline f32x4 mma(const Frag<bf16> &a, const Frag<bf16> &b, f32x4 c) {
@@ -41,68 +45,95 @@ __device__ inline f32x4 mma(const Frag<float> &a, const Frag<float> &b, f32x4 c)
   return c;
 }
 
-/* One operand's tile of R rows (of m or n) by 128 bytes of k in LDS, filled
+/* A window on memory of which nothing past `extent` bytes is read: a buffer's
+ * descriptor (base, no stride, size in bytes, raw 32-bit data). */
+__device__ inline u32x4 window(const void *base, int64_t extent) {
+  uintptr_t at = (uintptr_t)base;
+  return u32x4{(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu,
+               (uint32_t)min(max(extent, (int64_t)0), (int64_t)0x7ffffff0), 0x00020000u};
+}
+
+__device__ inline u32x4 load16(u32x4 from, uint32_t offset) {
+  __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(
+      (void *)(((uintptr_t)from[1] << 32) | from[0]), 0, (int)from[2], (int)from[3]);
+  return __builtin_amdgcn_raw_buffer_load_b128(rsrc, offset, 0, 0);
+}
+
+/* 16 bytes a lane straight to LDS, at `to` + 16 lane.  Written out because the
+ * compiler, which cannot tell this buffer from the ones being read, would wait
+ * for it before the next read of LDS; land_and_meet() does the waiting. */
+__device__ inline void load16_to_lds(u32x4 from, uint32_t offset, char *to) {
+  uint32_t at = (uint32_t)(uintptr_t)(lds_void *)to;
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+      :
+      : "s"(at), "v"(offset), "s"(from)
+      : "memory", "m0");
+}
+
+/* One operand's tile of R rows (of m or n) by STEPS steps of k in LDS, filled
  * by loads that go to LDS directly: lane l of a wave writes base + 16 l, so
  * the order of 16-byte chunks is chosen by which chunk a lane asks for.
  *
- * k contiguous: rows of 8 chunks, chunk c of row r at c ^ ((r >> 1) & 7): the
- * 16 rows that a fragment reads at once fall on all 64 banks.
+ * k contiguous: the chunks of a row are spread by xor with higher bits of the
+ * row, so that the 16 rows that a fragment reads at once fall on all 64 banks.
  * k strided: rows are k; a 16-bit fragment is read with the transposing read
  * (4 rows of k by 16 columns), so 32-byte pieces of rows that are read
- * together are spread by xor; fp32 reads 64-byte pieces of 4 rows. */
+ * together are spread by xor; fp32 reads 64-byte pieces of 4 rows.
+ * Counted on 8192^3: no bank conflicts in any layout. */
 template <typename T, bool KC, int R, int THREADS>
 struct Tile {
   static constexpr int E = Vec<T>::N;
-  static constexpr int LOADS = R * STAGE_BYTES / (THREADS * 16);
-  static constexpr int ROW_CHUNKS = R / E; /* k strided */
-  static constexpr int BYTES = R * STAGE_BYTES;
+  static constexpr int STAGE = STEPS * STEP_BYTES;
+  static constexpr int BYTES = R * STAGE;
+  static constexpr int LOADS = BYTES / (THREADS * 16);
+  static constexpr int ROW_CHUNKS = KC ? STAGE / 16 : R / E;
   static_assert(LOADS * THREADS * 16 == BYTES, "whole loads");
-  static_assert(KC || ROW_CHUNKS >= 8, "room for the xor");
-  uint32_t off[LOADS];
-  int kpos[LOADS]; /* first k of the chunk within the stage */
+  static_assert((ROW_CHUNKS & (ROW_CHUNKS - 1)) == 0, "the xor stays in the row");
+  /* A thread's chunks lie ROWS rows apart.  The xor repeats every 16 rows, so
+   * but for WAYS of them their offsets differ by whole rows alone. */
+  static constexpr int ROWS = THREADS / ROW_CHUNKS;
+  static constexpr int WAYS = ROWS >= 16 ? 1 : 16 / ROWS;
+  static_assert(LOADS % WAYS == 0 || LOADS < WAYS, "rows alike");
+  uint32_t off[WAYS], stride; /* bytes */
+  int kpos;                   /* first k of the thread's first chunk */
 
-  static __device__ int spread(int k) {
-    if (sizeof(T) == 4) return ((k >> 2) & 3) << 2;
-    int s = ((k & 3) | (((k >> 3) & 1) << 2)) << 1;
-    return ROW_CHUNKS >= 16 ? s : s & 7;
+  static __device__ int spread(int row) {
+    int x;
+    if (KC) x = row >> 1;
+    else if (sizeof(T) == 4) x = ((row >> 2) & 3) << 2;
+    else x = ((row & 3) | (((row >> 3) & 1) << 2)) << 1;
+    return x & (ROW_CHUNKS - 1);
   }
 
-  __device__ void init(int64_t ld, int64_t rows_left, int tid) {
+  __device__ void init(int64_t ld, int tid) {
+    int r = tid / ROW_CHUNKS;
+    stride = (uint32_t)(ld * sizeof(T));
+    kpos = KC ? ((tid % ROW_CHUNKS) ^ spread(r)) * E : r;
 #pragma unroll
-    for (int i = 0; i < LOADS; i++) {
-      int q = i * THREADS + tid;
-      if (KC) {
-        int r = q >> 3, c = (q & 7) ^ ((r >> 1) & 7);
-        kpos[i] = c * E;
-        off[i] = r < rows_left ? (uint32_t)(r * ld * sizeof(T)) + c * 16 : OUT_OF_RANGE;
-      } else {
-        int k = q / ROW_CHUNKS, c = (q % ROW_CHUNKS) ^ spread(k);
-        kpos[i] = k;
-        off[i] = c * E < rows_left ? (uint32_t)(k * ld * sizeof(T)) + c * 16 : OUT_OF_RANGE;
-      }
-    }
+    for (int w = 0; w < WAYS; w++)
+      off[w] = (r + w * ROWS) * stride + ((tid % ROW_CHUNKS) ^ spread(r + w * ROWS)) * 16;
   }
 
-  /* Chunks past the end of k come as zeros. */
-  __device__ void load(const char *base, int64_t extent, int64_t k_left, char *lds, int wave) {
-    int records = (int)min(max(extent, (int64_t)0), (int64_t)0x7ffffff0);
-    __amdgpu_buffer_rsrc_t rsrc =
-        __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, records, 0x00020000);
-#pragma unroll
-    for (int i = 0; i < LOADS; i++) {
-      uint32_t o = kpos[i] < k_left ? off[i] : OUT_OF_RANGE;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rsrc, (lds_void *)(lds + (i * THREADS + wave * 64) * 16), 16, o, 0, 0, 0);
-    }
+  /* One of a stage's loads.  Chunks past the end of k come as zeros, and so
+   * does what lies past the operand's end.  Rows past m or n only feed results
+   * that are not stored. */
+  __device__ void load(int i, u32x4 from, int k_left, char *lds, int wave) const {
+    uint32_t skip = i / WAYS * WAYS * ROWS * stride;
+    /* added anew every time: kept, the sums would cost a register a load */
+    asm volatile("" : "+s"(skip));
+    bool in = kpos < (KC ? k_left : k_left - i * ROWS);
+    uint32_t o = (in ? off[i % WAYS] : OUT_OF_RANGE) + skip;
+    load16_to_lds(from, o, lds + (i * THREADS + wave * 64) * 16);
   }
 
-  /* The fragment of rows row0 .. row0+15 at step `step` (0 or 1). */
+  /* The fragment of rows row0 .. row0+15 at one of the stage's steps. */
   static __device__ Frag<T> frag(const char *lds, int row0, int step, int lane) {
     int i = lane & 15, g = lane >> 4;
     Frag<T> f;
     if constexpr (KC) {
-      int c = (step * 4 + g) ^ ((i >> 1) & 7);
-      f.v = *(const typename Vec<T>::type *)(lds + (row0 + i) * STAGE_BYTES + c * 16);
+      int c = (step * 4 + g) ^ spread(i); /* row0 is a multiple of 16 */
+      f.v = *(const typename Vec<T>::type *)(lds + (row0 + i) * STAGE + c * 16);
     } else if constexpr (sizeof(T) == 4) {
       int c = ((row0 + i) >> 2) ^ (g << 2);
       const char *p = lds + (step * 16 + 4 * g) * (R * 4) + c * 16 + (i & 3) * 4;
@@ -125,55 +156,79 @@ struct Tile {
   }
 };
 
-/* Four neighbouring columns of one row: bias, activation, residual, store.
- * Accesses of four need no alignment beyond the element's. */
+/* Finishes COUNT rows of the same four neighbouring columns, `step` rows
+ * apart: bias, activation, residual, store, or the partial sums of a split.
+ * All that is read is asked for before any of it is used.  Accesses of four
+ * need no alignment beyond the element's. */
 template <typename T>
 struct Epilogue {
-  const T *bias, *res;
-  T *y, *z;
-  int64_t ldr, ldy, ldz, n;
-  int act;
+  typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  const GemmArgs &p;
+  float *part; /* of this split, or null */
 
-  __device__ Epilogue(const GemmArgs &p)
-      : bias((const T *)p.bias), res((const T *)p.res), y((T *)p.y), z((T *)p.z),
-        ldr(p.ldr), ldy(p.ldy), ldz(p.ldz), n(p.n), act(p.act) {}
+  __device__ Epilogue(const GemmArgs &args, int split = 0)
+      : p(args), part(args.splits > 1 ? args.work + (int64_t)split * args.m * args.n : nullptr) {}
 
-  __device__ void operator()(int64_t m, int64_t col, f32x4 v) const {
-    typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    if (col + 4 <= n) {
-      if (bias) {
-        four b = *(const four *)(bias + col);
+  template <int COUNT>
+  __device__ void operator()(int64_t m, int step, int64_t col, f32x4 (&v)[COUNT]) const {
+    int width = (int)min((int64_t)4, p.n - col);
+    if (width <= 0) return;
+    if (part) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] += to_f<T>(b[i]);
-      }
-      four o;
-      if (z) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = from_f<T>(v[i]);
-        *(four *)(z + m * ldz + col) = o;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; i++) v[i] = activate(v[i], act);
-      if (res) {
-        four r = *(const four *)(res + m * ldr + col);
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] += to_f<T>(r[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; i++) o[i] = from_f<T>(v[i]);
-      *(four *)(y + m * ldy + col) = o;
+      for (int q = 0; q < COUNT; q++)
+        if (m + q * step < p.m) put(part + (m + q * step) * p.n + col, width, v[q]);
       return;
     }
+    f32x4 res[COUNT];
+    if (p.res)
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      int64_t c = col + i;
-      if (c >= n) return;
-      float u = v[i];
-      if (bias) u += to_f<T>(bias[c]);
-      if (z) z[m * ldz + c] = from_f<T>(u);
-      u = activate(u, act);
-      if (res) u += to_f<T>(res[m * ldr + c]);
-      y[m * ldy + c] = from_f<T>(u);
+      for (int q = 0; q < COUNT; q++)
+        if (m + q * step < p.m)
+          res[q] = get((const T *)p.res + (m + q * step) * p.ldr + col, width);
+    if (p.bias) {
+      f32x4 b = get((const T *)p.bias + col, width);
+#pragma unroll
+      for (int q = 0; q < COUNT; q++) v[q] += b;
+    }
+    if (p.z)
+#pragma unroll
+      for (int q = 0; q < COUNT; q++)
+        if (m + q * step < p.m) put((T *)p.z + (m + q * step) * p.ldz + col, width, v[q]);
+    if (p.act != ACT_NONE)
+#pragma unroll
+      for (int q = 0; q < COUNT; q++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[q][e] = activate<T>(v[q][e], p.act);
+    if (p.res)
+#pragma unroll
+      for (int q = 0; q < COUNT; q++) v[q] += res[q];
+#pragma unroll
+    for (int q = 0; q < COUNT; q++)
+      if (m + q * step < p.m) put((T *)p.y + (m + q * step) * p.ldy + col, width, v[q]);
+  }
+
+  static __device__ f32x4 get(const T *at, int width) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (width == 4) {
+      four t = *(const four *)at;
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = to_f<T>(t[e]);
+    } else {
+      for (int e = 0; e < width; e++) v[e] = to_f<T>(at[e]);
+    }
+    return v;
+  }
+
+  template <typename D>
+  static __device__ void put(D *at, int width, f32x4 v) {
+    typedef D quad __attribute__((ext_vector_type(4), aligned(sizeof(D))));
+    if (width == 4) {
+      quad t;
+#pragma unroll
+      for (int e = 0; e < 4; e++) t[e] = from_f<D>(v[e]);
+      *(quad *)at = t;
+    } else {
+      for (int e = 0; e < width; e++) at[e] = from_f<D>(v[e]);
     }
   }
 };
@@ -191,17 +246,29 @@ __device__ inline void tile_of(int block, int blocks, int tiles_m, int tiles_n, 
   *tn = in / height;
 }
 
-/* A TM x TN tile of y per workgroup of WR x WC waves, two stages of LDS: the
- * loads of a stage run while the one before is multiplied, and one barrier a
- * stage both publishes the new one and frees the old one. */
-template <typename T, bool AKC, bool BKC, int TM, int TN, int WR, int WC>
+/* Waits until at most N of the wave's loads to LDS are in flight and its LDS
+ * reads are done, then for the other waves.  The compiler moves no memory
+ * access across it. */
+template <int N>
+__device__ inline void land_and_meet() {
+  static_assert(N < 64, "vmcnt has six bits");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+/* A TM x TN tile of y per workgroup of WR x WC waves, and BUFFERS stages of
+ * STEPS steps of k in LDS.  The fragments of a step are read while the step
+ * before is multiplied, so the matrix cores wait for neither; one barrier a
+ * stage says both that the next stage has landed and that this one has been
+ * read, and its buffer is filled again at once. */
+template <typename T, bool AKC, bool BKC, int TM, int TN, int WR, int WC, int BUFFERS>
 __global__ __launch_bounds__(WR *WC * 64) void gemm_tile(GemmArgs p) {
   constexpr int THREADS = WR * WC * 64;
-  constexpr int BK = STAGE_BYTES / sizeof(T);
+  constexpr int BK = STEPS * STEP_BYTES / sizeof(T);
   constexpr int FM = TM / WR / 16, FN = TN / WC / 16;
   using TA = Tile<T, AKC, TM, THREADS>;
   using TB = Tile<T, BKC, TN, THREADS>;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * (TA::BYTES + TB::BYTES)];
+  constexpr int LOADS = TA::LOADS + TB::LOADS, BYTES = TA::BYTES + TB::BYTES;
+  __shared__ __attribute__((aligned(1024))) char lds[BUFFERS * BYTES];
 
   int tid = threadIdx.x, lane = tid & 63;
   int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -209,43 +276,94 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_tile(GemmArgs p) {
   int tm, tn;
   tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, &tm, &tn);
   int64_t m0 = (int64_t)tm * TM, n0 = (int64_t)tn * TN;
-  int64_t stages_all = (p.k + BK - 1) / BK;
-  int64_t s0 = stages_all * blockIdx.y / p.splits, s1 = stages_all * (blockIdx.y + 1) / p.splits;
+  int stages_all = (int)((p.k + BK - 1) / BK);
+  int s0 = (int)((int64_t)stages_all * blockIdx.y / p.splits);
+  int s1 = (int)((int64_t)stages_all * (blockIdx.y + 1) / p.splits);
 
   TA ta;
   TB tb;
-  ta.init(p.lda, p.m - m0, tid);
-  tb.init(p.ldb, p.n - n0, tid);
-  auto fetch = [&](int64_t s) {
-    int64_t k = s * BK;
+  ta.init(p.lda, tid);
+  tb.init(p.ldb, tid);
+  /* past this part's last stage the loads bring zeros, so that their number
+   * stays the same */
+  struct Source {
+    u32x4 a, b;
+    int left;
+  };
+  auto source = [&](int s) {
+    int64_t k = (int64_t)s * BK;
     int64_t oa = (AKC ? m0 * p.lda + k : k * p.lda + m0) * (int64_t)sizeof(T);
     int64_t ob = (BKC ? n0 * p.ldb + k : k * p.ldb + n0) * (int64_t)sizeof(T);
-    char *at = lds + (s & 1) * (TA::BYTES + TB::BYTES);
-    ta.load((const char *)p.a + oa, p.a_extent - oa, p.k - k, at, wave);
-    tb.load((const char *)p.b + ob, p.b_extent - ob, p.k - k, at + TA::BYTES, wave);
+    return Source{window((const char *)p.a + oa, p.a_extent - oa),
+                  window((const char *)p.b + ob, p.b_extent - ob),
+                  s < s1 ? (int)min(p.k - k, (int64_t)BK) : 0};
+  };
+  auto load = [&](int i, const Source &q, char *at) {
+    if (i < TA::LOADS) ta.load(i, q.a, q.left, at, wave);
+    else tb.load(i - TA::LOADS, q.b, q.left, at + TA::BYTES, wave);
   };
 
   f32x4 acc[FM][FN] = {};
   int wm = wave / WC * (TM / WR), wn = wave % WC * (TN / WC);
-  if (s0 < s1) fetch(s0);
-  for (int64_t s = s0; s < s1; s++) {
-    __builtin_amdgcn_s_waitcnt(0x0f70); /* vmcnt(0) */
-    __syncthreads();
-    if (s + 1 < s1) fetch(s + 1);
-    const char *la = lds + (s & 1) * (TA::BYTES + TB::BYTES), *lb = la + TA::BYTES;
+  struct Step {
+    Frag<T> a[FM], b[FN];
+  } even, odd;
+  auto read = [&](int f, Step &h, const char *at, int step) {
+    if (f < FN) h.b[f] = TB::frag(at + TA::BYTES, wn + f * 16, step, lane);
+    else h.a[f - FN] = TA::frag(at, wm + (f - FN) * 16, step, lane);
+  };
+  auto multiply = [&](const Step &h) {
 #pragma unroll
-    for (int step = 0; step < 2; step++) {
-      Frag<T> fa[FM], fb[FN];
+    for (int i = 0; i < FM; i++)
 #pragma unroll
-      for (int j = 0; j < FN; j++) fb[j] = TB::frag(lb, wn + j * 16, step, lane);
+      for (int j = 0; j < FN; j++) acc[i][j] = mma(h.b[j], h.a[i], acc[i][j]);
+  };
+  /* Deals a step's reads, and the loads that stand between them, out between
+   * its products: in a row they would hold up the matrix cores of all waves. */
+  constexpr int FRAGS = FM + FN;
+  constexpr int PRODUCTS = FM * FN * (sizeof(T) == 4 ? 4 : 1);
+  constexpr int EACH = PRODUCTS / FRAGS > 0 ? PRODUCTS / FRAGS : 1;
+  auto deal = [] {
 #pragma unroll
-      for (int i = 0; i < FM; i++) fa[i] = TA::frag(la, wm + i * 16, step, lane);
-#pragma unroll
-      for (int i = 0; i < FM; i++)
-#pragma unroll
-        for (int j = 0; j < FN; j++) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
+    for (int f = 0; f < FRAGS; f++) {
+      if (f < FN) __builtin_amdgcn_sched_group_barrier(0x100, Frag<T>::reads(BKC), 0);
+      else __builtin_amdgcn_sched_group_barrier(0x100, Frag<T>::reads(AKC), 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
     }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  int buffer = 0;
+  /* the stage whose first step is in `now`; leaves the next one's there */
+  auto stage = [&](int s, Step &now, Step &then) {
+    char *at = lds + buffer * BYTES;
+    buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
+    char *ahead = lds + buffer * BYTES;
+    Source q = source(s + BUFFERS);
+#pragma unroll
+    for (int f = 0; f < FRAGS; f++) read(f, then, at, 1);
+    multiply(now);
+    deal();
+    land_and_meet<(BUFFERS - 2) * LOADS>();
+#pragma unroll
+    for (int f = 0; f < (FRAGS > LOADS ? FRAGS : LOADS); f++) {
+      if (f < FRAGS) read(f, now, ahead, 0);
+      if (f < LOADS) load(f, q, at);
+    }
+    multiply(then);
+    deal();
+  };
+
+#pragma unroll
+  for (int i = 0; i < BUFFERS; i++) {
+    Source q = source(s0 + i);
+#pragma unroll
+    for (int f = 0; f < LOADS; f++) load(f, q, lds + i * BYTES);
   }
+  land_and_meet<(BUFFERS - 1) * LOADS>();
+#pragma unroll
+  for (int f = 0; f < FRAGS; f++) read(f, even, lds, 0);
+  for (int s = s0; s < s1; s++) stage(s, even, odd);
+  land_and_meet<0>();
 
   /* b is the first operand of the product, so a lane holds 4 neighbouring
    * columns of row lane%16.  Each wave turns its part through its own piece
@@ -253,12 +371,14 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_tile(GemmArgs p) {
    * once; 16-byte pieces are spread by xor over the banks. */
   constexpr int WM = TM / WR, WN = TN / WC, PIECES = WN / 4;
   constexpr int PIECE_LDS = (int)sizeof(lds) / (WR * WC);
-  constexpr int ROWS = PIECE_LDS / (WN * 4) < WM ? PIECE_LDS / (WN * 4) : WM;
-  static_assert(ROWS % 16 == 0 && WM % ROWS == 0, "whole fragments a pass");
-  __syncthreads();
+  constexpr int FIT = PIECE_LDS / (WN * 4);
+  constexpr int ROWS = FIT >= WM ? WM : FIT >= WM / 2 ? WM / 2 : WM / 4;
+  static_assert(ROWS % 16 == 0 && ROWS <= FIT, "whole fragments a pass");
+  static_assert(64 % PIECES == 0, "a lane keeps its columns");
+  constexpr int DOWN = 64 / PIECES, U = ROWS / DOWN < 4 ? ROWS / DOWN : 4;
   float *mine = (float *)(lds + wave * PIECE_LDS);
-  Epilogue<T> store(p);
-  float *part = p.work + (int64_t)blockIdx.y * p.m * p.n;
+  Epilogue<T> finish(p, blockIdx.y);
+  int row = lane / PIECES, piece = lane % PIECES;
 #pragma unroll
   for (int pass = 0; pass < WM / ROWS; pass++) {
 #pragma unroll
@@ -269,20 +389,13 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_tile(GemmArgs p) {
         *(f32x4 *)(mine + r * WN + c * 4) = acc[pass * (ROWS / 16) + i][j];
       }
 #pragma unroll 1
-    for (int q = lane; q < ROWS * PIECES; q += 64) {
-      int r = q / PIECES, c = q % PIECES;
-      f32x4 v = *(const f32x4 *)(mine + r * WN + (c ^ (r & (PIECES - 1))) * 4);
-      int64_t m = m0 + wm + pass * ROWS + r, n = n0 + wn + c * 4;
-      if (m >= p.m || n >= p.n) continue;
-      if (p.splits == 1) {
-        store(m, n, v);
-      } else if (p.n % 4 == 0) {
-        *(f32x4 *)(part + m * p.n + n) = v;
-      } else {
+    for (int r = row; r < ROWS; r += DOWN * U) {
+      f32x4 v[U];
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-          if (n + e < p.n) part[m * p.n + n + e] = v[e];
-      }
+      for (int u = 0; u < U; u++)
+        v[u] = *(const f32x4 *)(mine + (r + u * DOWN) * WN +
+                                (piece ^ ((r + u * DOWN) & (PIECES - 1))) * 4);
+      finish(m0 + wm + pass * ROWS + r, DOWN, n0 + wn + piece * 4, v);
     }
   }
 }
@@ -294,7 +407,7 @@ __global__ __launch_bounds__(256) void gemm_join(GemmArgs p) {
   int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= p.m * fours) return;
   int64_t m = at / fours, n = at % fours * 4;
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  f32x4 sum[1] = {{0.f, 0.f, 0.f, 0.f}}, &v = sum[0];
   const float *q = p.work + m * p.n + n;
   if (n + 4 <= p.n && p.n % 4 == 0) {
     for (int s = 0; s < p.splits; s++) v += *(const f32x4 *)(q + (int64_t)s * p.m * p.n);
@@ -304,11 +417,12 @@ __global__ __launch_bounds__(256) void gemm_join(GemmArgs p) {
       for (int e = 0; e < 4; e++)
         if (n + e < p.n) v[e] += q[(int64_t)s * p.m * p.n + e];
   }
-  Epilogue<T> store(p);
-  store(m, n, v);
+  p.splits = 1;
+  Epilogue<T> finish(p);
+  finish(m, 0, n, sum);
 }
 
-/* Few rows (m <= 64): b is read once, at the memory's rate, straight into the
+/* Few rows (m <= 32): b is read once, at the memory's rate, straight into the
  * matrix cores' registers.  A workgroup takes a strip of n; its eight waves
  * share k between them, a step of 64 bytes of a's k at a time, and join in
  * LDS.  FM is the number of 16-row pieces of a.
@@ -322,7 +436,8 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
   constexpr int V = Vec<T>::N, WAVES = 8;
   constexpr int FN = BKC ? 1 : V;          /* products a step */
   constexpr int STRIP = 16 * FN;           /* columns of y */
-  constexpr int C = BKC ? (FM == 4 ? 4 : 8) : 1; /* steps a wave takes at once */
+  /* steps a wave has in flight, twice: 8 KB of b at least */
+  constexpr int C = BKC ? (FM == 1 ? 8 : 4) : sizeof(T) == 4 ? 2 : 1;
   constexpr int LOADS = BKC ? 1 : V;       /* of b a step */
   typedef typename Vec<T>::type vec;
   __shared__ f32x4 lds[WAVES][16][STRIP / 4];
@@ -332,12 +447,9 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
   int64_t n0 = (int64_t)blockIdx.x * STRIP;
   int64_t all = (p.k + 4 * V - 1) / (4 * V);
   int64_t s0 = all * blockIdx.y / p.splits, s1 = all * (blockIdx.y + 1) / p.splits;
-  const char *a = (const char *)p.a;
   const char *b = (const char *)p.b + n0 * (BKC ? p.ldb : 1) * (int64_t)sizeof(T);
   int64_t b_left = p.b_extent - (b - (const char *)p.b);
-  int a_records = (int)min(p.a_extent, (int64_t)0x7ffffff0);
-  __amdgpu_buffer_rsrc_t ra =
-      __builtin_amdgcn_make_buffer_rsrc((void *)a, 0, a_records, 0x00020000);
+  u32x4 ra = window(p.a, p.a_extent);
 
   uint32_t a_off[FM], b_off[LOADS];
 #pragma unroll
@@ -359,15 +471,12 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
     uint32_t at = (uint32_t)(s * 64);
 #pragma unroll
     for (int f = 0; f < FM; f++)
-      q.a[f] = __builtin_amdgcn_raw_buffer_load_b128(ra, in ? a_off[f] + at : OUT_OF_RANGE, 0, 0);
+      q.a[f] = load16(ra, in ? a_off[f] + at : OUT_OF_RANGE);
     int64_t skip = BKC ? 0 : s * 4 * V * p.ldb * (int64_t)sizeof(T);
-    int records = (int)min(max(b_left - skip, (int64_t)0), (int64_t)0x7ffffff0);
-    __amdgpu_buffer_rsrc_t rb =
-        __builtin_amdgcn_make_buffer_rsrc((void *)(b + skip), 0, records, 0x00020000);
+    u32x4 rb = window(b + skip, b_left - skip);
 #pragma unroll
     for (int t = 0; t < LOADS; t++)
-      q.b[t] = __builtin_amdgcn_raw_buffer_load_b128(
-          rb, (BKC ? in : s < s1) ? b_off[t] + (BKC ? at : 0) : OUT_OF_RANGE, 0, 0);
+      q.b[t] = load16(rb, (BKC ? in : s < s1) ? b_off[t] + (BKC ? at : 0) : OUT_OF_RANGE);
   };
 
   f32x4 acc[FM][FN] = {};
@@ -392,16 +501,24 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
       for (int j = 0; j < FN; j++) acc[f][j] = mma(fb[j], fa, acc[f][j]);
     }
   };
-  for (int64_t s = s0 + wave * C; s < s1; s += WAVES * C) {
-    Step q[C];
+  Step even[C], odd[C];
+  auto take = [&](Step(&now)[C], Step(&then)[C], int64_t s) {
 #pragma unroll
-    for (int c = 0; c < C; c++) fetch(q[c], s + c);
+    for (int c = 0; c < C; c++) fetch(then[c], s + WAVES * C + c);
+    __builtin_amdgcn_sched_barrier(0); /* the loads go out before the products */
 #pragma unroll
-    for (int c = 0; c < C; c++) multiply(q[c]);
+    for (int c = 0; c < C; c++) multiply(now[c]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  int64_t s = s0 + wave * C;
+#pragma unroll
+  for (int c = 0; c < C; c++) fetch(even[c], s + c);
+  for (; s < s1; s += 2 * WAVES * C) { /* steps past s1 are zeros */
+    take(even, odd, s);
+    take(odd, even, s + WAVES * C);
   }
 
-  Epilogue<T> store(p);
-  float *part = p.work + (int64_t)blockIdx.y * p.m * p.n;
+  Epilogue<T> finish(p, blockIdx.y);
 #pragma unroll
   for (int f = 0; f < FM; f++) {
     if (f) __syncthreads();
@@ -418,16 +535,10 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
       int r = q / (STRIP / 4), c = q % (STRIP / 4);
       int64_t m = f * 16 + r, n = n0 + c * 4;
       if (m >= p.m || n >= p.n) continue;
-      f32x4 v = lds[0][r][c];
+      f32x4 v[1] = {lds[0][r][c]};
 #pragma unroll
-      for (int w = 1; w < WAVES; w++) v += lds[w][r][c];
-      if (p.splits == 1) {
-        store(m, n, v);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          if (n + e < p.n) part[m * p.n + n + e] = v[e];
-      }
+      for (int w = 1; w < WAVES; w++) v[0] += lds[w][r][c];
+      finish(m, 0, n, v);
     }
   }
 }
@@ -474,8 +585,7 @@ void launch_rows(const GemmArgs &p, hipStream_t stream) {
   constexpr int STRIP = BKC ? 16 : 16 * Vec<T>::N;
   dim3 grid((unsigned)((p.n + STRIP - 1) / STRIP), (unsigned)p.splits);
   if (p.m <= 16) gemm_rows<T, BKC, 1><<<grid, 512, 0, stream>>>(p);
-  else if (p.m <= 32) gemm_rows<T, BKC, 2><<<grid, 512, 0, stream>>>(p);
-  else gemm_rows<T, BKC, 4><<<grid, 512, 0, stream>>>(p);
+  else gemm_rows<T, BKC, 2><<<grid, 512, 0, stream>>>(p);
 }
 
 template <typename T, bool AKC, bool BKC>
@@ -484,11 +594,13 @@ void launch_tile(const GemmArgs &p, hipStream_t stream) {
     return dim3((unsigned)(((p.m + tm - 1) / tm) * ((p.n + tn - 1) / tn)), (unsigned)p.splits);
   };
   if (p.plan == 0)
-    gemm_tile<T, AKC, BKC, 256, 256, 2, 4><<<blocks(256, 256), 512, 0, stream>>>(p);
+    gemm_tile<T, AKC, BKC, 256, 256, 2, 4, 2><<<blocks(256, 256), 512, 0, stream>>>(p);
   else if (p.plan == 1)
-    gemm_tile<T, AKC, BKC, 128, 128, 2, 2><<<blocks(128, 128), 256, 0, stream>>>(p);
+    gemm_tile<T, AKC, BKC, 128, 128, 2, 2, 2><<<blocks(128, 128), 256, 0, stream>>>(p);
+  else if (p.plan == 2)
+    gemm_tile<T, AKC, BKC, 64, 128, 2, 2, 3><<<blocks(64, 128), 256, 0, stream>>>(p);
   else
-    gemm_tile<T, AKC, BKC, 64, 64, 2, 2><<<blocks(64, 64), 256, 0, stream>>>(p);
+    gemm_tile<T, AKC, BKC, 32, 128, 1, 4, 4><<<blocks(32, 128), 256, 0, stream>>>(p);
 }
 
 template <typename T>
@@ -540,7 +652,7 @@ __global__ __launch_bounds__(256) void slope_rows(SlopeArgs p) {
     if (p.act != ACT_NONE) {
       load_vec<T>(z + r * p.ldz + col, n, u);
 #pragma unroll
-      for (int e = 0; e < V; e++) g[e] *= slope(u[e], p.act);
+      for (int e = 0; e < V; e++) g[e] *= slope<T>(u[e], p.act);
     }
 #pragma unroll
     for (int e = 0; e < V; e++) sum[e] += g[e];
@@ -603,33 +715,26 @@ int vgpu_ops_slope(const SlopeArgs *args, void *stream) {
  * each part keeps enough steps. */
 void vgpu_ops_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t a_kc, int32_t b_kc,
                         int32_t bare, int32_t *plan, int32_t *splits) {
-  const int side[3] = {256, 128, 64};
   int64_t size = dtype == DT_F32 ? 4 : 2;
-  int64_t stages = (k * size + STAGE_BYTES - 1) / STAGE_BYTES;
+  int64_t steps = (k * size + STEP_BYTES - 1) / STEP_BYTES;
   *splits = 1;
   if (k <= OUTER_K && !a_kc && !b_kc && bare && m <= 65535 * 4 * OUTER_ROWS) {
     *plan = PLAN_OUTER;
     return;
   }
-  if (m <= 64 && a_kc) {
+  if (a_kc && m <= 32 && (!b_kc || m <= 16 || n * k * size <= 1 << 24)) {
     *plan = PLAN_ROWS;
     int64_t strip = b_kc ? 16 : 256 / size, strips = (n + strip - 1) / strip;
-    int64_t steps = stages * 2;
-    *splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({512 / strips, steps / 64, 64}));
+    *splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({256 / strips, steps / 64, 64}));
     return;
   }
-  int64_t tiles = 0;
-  for (*plan = 0; *plan < 3; ++*plan) {
-    int s = side[*plan];
-    tiles = ((m + s - 1) / s) * ((n + s - 1) / s);
-    if (tiles >= 256) break;
-  }
-  if (*plan == 3) {
-    *plan = tiles >= 128 ? 2 : (m > 64 && n > 64 ? 1 : 2);
-    int s = side[*plan];
-    tiles = ((m + s - 1) / s) * ((n + s - 1) / s);
-    *splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, stages / 4, 64}));
-  }
+  auto tiles = [&](int64_t tm, int64_t tn) { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); };
+  if (m <= 32) *plan = 3;
+  else if (tiles(256, 256) >= 200) *plan = 0;
+  else if (tiles(128, 128) >= 400) *plan = 1;
+  else *plan = 2;
+  int64_t t = *plan == 3 ? 2 * tiles(32, 128) : *plan == 2 ? tiles(64, 128) : 512;
+  *splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({512 / t, steps / 32, 64}));
 }
 
 int vgpu_ops_gemm(const GemmArgs *args, void *stream) {
@@ -637,7 +742,7 @@ int vgpu_ops_gemm(const GemmArgs *args, void *stream) {
   if (p.m <= 0 || p.n <= 0 || p.k < 0 || p.splits < 1 || p.plan < 0 ||
       p.plan > PLAN_OUTER || (p.splits > 1 && !p.work))
     return OPS_BAD_ARG;
-  if (p.plan == PLAN_ROWS && (p.m > 64 || !p.a_kc)) return OPS_BAD_ARG;
+  if (p.plan == PLAN_ROWS && (p.m > 32 || !p.a_kc)) return OPS_BAD_ARG;
   if (p.plan == PLAN_OUTER && (p.k > OUTER_K || p.a_kc || p.b_kc || p.bias || p.res || p.z ||
                                p.act || p.splits > 1 || p.m > 65535 * 4 * OUTER_ROWS))
     return OPS_BAD_ARG;
