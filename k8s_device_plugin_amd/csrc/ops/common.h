@@ -52,6 +52,17 @@ __device__ inline void load_vec(const T *p, int n, float *out) {
   }
 }
 
+/* The same, unconverted. */
+template <typename T>
+__device__ inline typename Loose<T>::type load_raw(const T *p, int n) {
+  typename Loose<T>::type v = {};
+  if (n >= Vec<T>::N) return *(const typename Loose<T>::type *)p;
+#pragma unroll
+  for (int i = 0; i < Vec<T>::N; i++)
+    if (i < n) v[i] = p[i];
+  return v;
+}
+
 template <typename T>
 __device__ inline void store_vec(T *p, int n, const float *in) {
   constexpr int V = Vec<T>::N;
@@ -148,8 +159,8 @@ struct SlopeArgs {
 };
 
 /* Layer norm of each (row, group): x [rows, groups*d].  mean and rstd hold
- * rows*groups values, part 2 x parts x groups*d partial sums of the weight's
- * and bias's gradients. */
+ * rows*groups values; with more than one part, part holds 2 x parts x groups*d
+ * partial sums of the weight's and bias's gradients. */
 struct NormArgs {
   const void *x, *weight, *bias, *dy;
   void *y, *dx, *dweight, *dbias;
@@ -160,20 +171,21 @@ struct NormArgs {
   float eps;
 };
 
-/* Distillation from a teacher's top logits.  rows_loss and lse hold one value a
- * row, slot_p and slot_i `top` values a row, part 2 x chunks a row; count is
- * the number of rows with a target. */
+/* Distillation from a teacher's top logits.  rows_loss, state and lse hold one
+ * value a row, slot_p and slot_i `top` values a row, part 2 x chunks a row;
+ * counts holds, for each 16 rows, how many of them have a target. */
 struct DistillArgs {
   const void *x, *index, *teacher;
   void *dx;
   const float *grad; /* of the loss: one value, or one a row */
-  float *rows_loss, *lse, *slot_p, *loss, *count;
+  float *rows_loss, *state, *lse, *slot_p, *loss, *counts;
   int32_t *slot_i;
   float *part;
   int64_t ldx, lddx, ldi, ldt, rows, v;
   int32_t dtype, ttype, index_bytes, top;
   int32_t chunks, reduction; /* 0 none, 1 sum, 2 mean */
-  float temperature;
+  int32_t written;           /* dx holds the gradient for an upstream one of 1 */
+  float temperature, scale;  /* scale: of the loss that is one number */
 };
 
 /* Column sums of part [parts, width] in a fixed order: 16 runs of rows a

@@ -7,8 +7,14 @@
  * without mass has loss 0 and gradient 0 whatever its logits hold; an index
  * past the vocabulary makes the row's loss and gradient NaN.
  *
- * Bound by memory: the logits are read once forward with the running maximum
- * and sum of the softmax, and once backward beside the gradient's write.
+ * Bound by memory.  Without a gradient the logits are read once, with the
+ * running maximum and sum of the softmax.  With one, and a loss that is one
+ * number, the workgroup that has read a row keeps it in registers and goes on
+ * to write its gradient for an upstream gradient of 1, so that the logits are
+ * read once for both.  (A second reading from the last-level cache costs as
+ * much as one from memory: the way there is what bounds it.)  The backward
+ * pass has then nothing left to do, unless the upstream gradient turns out to
+ * be another number, and writes the gradient anew.
  */
 #include "common.h"
 
@@ -19,26 +25,40 @@ namespace {
 
 constexpr int MOST_SLOTS = 1024;
 
-/* 16-bit logits carry 2^-9 of error themselves: the short exp costs nothing
- * against that and a third of the instructions. */
+/* Logits enter the softmax as x c.  In fp32 c is 1/T and the exponential expf.
+ * 16-bit logits carry 2^-9 of error themselves, so theirs is the hardware's
+ * power of two, with log2(e) in c: one multiply-add and one instruction. */
 template <typename T>
-__device__ inline float exp_of(float v) {
-  if constexpr (sizeof(T) == 4) return expf(v);
-  else return __expf(v);
-}
+struct Unit {
+  static constexpr bool TWO = sizeof(T) == 2;
+  static __device__ float c(float temperature) { return (TWO ? 1.44269504089f : 1.f) / temperature; }
+  static __device__ float exp(float v) { return TWO ? __builtin_amdgcn_exp2f(v) : expf(v); }
+  static __device__ float from_natural(float v) { return TWO ? v * 1.44269504089f : v; }
+  static __device__ float to_natural(float v) { return TWO ? v * 0.69314718056f : v; }
+};
 
-/* The running maximum and the sum of exp relative to it. */
+/* The running maximum and the sum of exp relative to it.  It starts at the
+ * lowest finite number, so that -inf adds nothing and NaN makes the sum NaN
+ * without being asked for. */
 struct Run {
   float m, s;
 };
 
 template <typename T>
 __device__ inline Run join(Run a, Run b) {
-  Run r;
-  r.m = fmaxf(a.m, b.m);
-  if (a.m != a.m || b.m != b.m) r.m = NAN; /* fmaxf drops a NaN */
-  r.s = (a.s ? a.s * exp_of<T>(a.m - r.m) : 0.f) + (b.s ? b.s * exp_of<T>(b.m - r.m) : 0.f);
-  return r;
+  float m = fmaxf(a.m, b.m);
+  return {m, a.s * Unit<T>::exp(a.m - m) + b.s * Unit<T>::exp(b.m - m)};
+}
+
+__device__ inline Run no_run() { return {-3.402823466e38f, 0.f}; }
+
+__device__ inline Run wave_neighbour(Run r, int o) {
+  return {__shfl_xor(r.m, o, 64), __shfl_xor(r.s, o, 64)};
+}
+
+__device__ inline int64_t index_at(const DistillArgs &p, int64_t row, int k) {
+  return p.index_bytes == 8 ? ((const int64_t *)p.index)[row * p.ldi + k]
+                            : ((const int32_t *)p.index)[row * p.ldi + k];
 }
 
 __device__ inline float any_f(const void *p, int64_t i, int dtype) {
@@ -47,213 +67,373 @@ __device__ inline float any_f(const void *p, int64_t i, int dtype) {
   return to_f<fp16>(((const fp16 *)p)[i]);
 }
 
-/* One wave: the row's loss from its maximum and sum, and the slots' mass for
- * the backward pass, where a class that is named twice is folded into its
- * first slot so that no two slots write to one place. */
-template <typename T>
-__device__ void finish(const DistillArgs &p, int64_t row, Run all, float *sp, int *si) {
-  int lane = threadIdx.x % 64;
-  float inv_t = 1.f / p.temperature;
-  const T *x = (const T *)p.x + row * p.ldx;
-  /* no finite logit at all: as the formula, NaN */
-  float lse = all.m == -INFINITY ? NAN : all.m + logf(all.s);
+/* A row's state: no slot with mass, a target, an index past the vocabulary. */
+constexpr float NO_TARGET = 0.f, TARGET = 1.f, BAD_INDEX = 2.f;
+constexpr int SLOT_ROWS = 16; /* rows a workgroup of distill_slots */
 
-  float high = -INFINITY;
-  bool bad = false, nan = false;
-  for (int k = lane; k < p.top; k += 64) {
-    int64_t i = p.index_bytes == 8 ? ((const int64_t *)p.index)[row * p.ldi + k]
-                                   : ((const int32_t *)p.index)[row * p.ldi + k];
-    float t = p.teacher ? any_f(p.teacher, row * p.ldt + k, p.ttype) * inv_t : 0.f;
-    bool here = i >= 0 && t != -INFINITY;
-    bad |= i >= p.v;
-    nan |= here && t != t;
-    si[k] = here && i < p.v ? (int)i : -1;
-    sp[k] = here ? t : -INFINITY;
-    high = fmaxf(high, sp[k]);
-  }
-#pragma unroll
-  for (int o = 32; o; o >>= 1) high = fmaxf(high, __shfl_xor(high, o, 64));
-  bool some = __any(high != -INFINITY || nan);
-  bad = __any(bad);
-  if (bad) lse = NAN;
-  some |= bad;
-  float mass = 0.f;
-  for (int k = lane; k < p.top; k += 64) mass += expf(sp[k] - high);
-  mass = wave_sum(mass);
-  float log_mass = logf(mass), loss = 0.f;
-  for (int k = lane; k < p.top; k += 64) {
-    float log_p = sp[k] - high - log_mass;
-    float q = expf(sp[k] - high) / mass;
-    if (some && si[k] >= 0 && q != 0.f)
-      loss += q * (log_p - (to_f<T>(x[si[k]]) * inv_t - lse));
-    sp[k] = q;
-  }
-  loss = wave_sum(loss);
-  if (bad) loss = NAN;
-  if (lane == 0) {
-    p.rows_loss[row] = some ? loss * p.temperature * p.temperature : 0.f;
-    if (p.lse) p.lse[row] = lse;
-  }
-  if (!p.slot_p) return;
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); /* other lanes' slots */
-  __builtin_amdgcn_wave_barrier();
-  for (int k = lane; k < p.top; k += 64) {
-    int i = si[k];
-    float q = sp[k];
-    for (int j = 0; i >= 0 && j < p.top; j++) {
-      if (si[j] != i || j == k) continue;
-      if (j < k) i = -1; /* folded into slot j */
-      else q += sp[j];
+/* What the teacher says of a row, a wave each: the slots' masses, and
+ * sum_k p_k (log p_k - x[i_k]/T), to which the loss adds the log of the
+ * softmax's sum.  A class that is named twice is folded into its first slot,
+ * so that no two slots write to one place of the gradient. */
+template <typename T>
+__global__ __launch_bounds__(1024) void distill_slots(DistillArgs p) {
+  extern __shared__ float slots[]; /* of each wave: top masses, top classes */
+  __shared__ int targets[SLOT_ROWS];
+  int lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64;
+  float *sp = slots + (int64_t)wave * 2 * p.top;
+  int *si = (int *)(sp + p.top);
+  float inv_t = 1.f / p.temperature;
+  for (int q = wave; q < SLOT_ROWS; q += waves) {
+    int64_t row = (int64_t)blockIdx.x * SLOT_ROWS + q;
+    if (row >= p.rows) {
+      if (lane == 0) targets[q] = 0;
+      continue;
     }
-    /* a row without mass is told by the first slot, whose mass is -1 */
-    p.slot_p[row * p.top + k] = some ? q : -1.f;
-    p.slot_i[row * p.top + k] = some ? i : -1;
+    const T *x = (const T *)p.x + row * p.ldx;
+    float high = -INFINITY;
+    bool bad = false, some = false;
+    for (int k = lane; k < p.top; k += 64) {
+      int64_t i = index_at(p, row, k);
+      float t = p.teacher ? any_f(p.teacher, row * p.ldt + k, p.ttype) * inv_t : 0.f;
+      bool here = i >= 0 && t != -INFINITY;
+      bad |= i >= p.v;
+      some |= here;
+      si[k] = here && i < p.v ? (int)i : -1;
+      sp[k] = here ? t : -INFINITY;
+      high = fmaxf(high, sp[k]);
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) high = fmaxf(high, __shfl_xor(high, o, 64));
+    bad = __any(bad);
+    some = __any(some);
+    float state = bad ? BAD_INDEX : some ? TARGET : NO_TARGET;
+    float mass = 0.f;
+    for (int k = lane; k < p.top; k += 64) mass += expf(sp[k] - high);
+    mass = wave_sum(mass);
+    float log_mass = logf(mass), loss = 0.f;
+    for (int k = lane; k < p.top; k += 64) {
+      float log_p = sp[k] - high - log_mass, m = expf(sp[k] - high) / mass;
+      if (some && si[k] >= 0 && m != 0.f) loss += m * (log_p - to_f<T>(x[si[k]]) * inv_t);
+      sp[k] = m;
+    }
+    loss = wave_sum(loss);
+    if (lane == 0) {
+      targets[q] = state != NO_TARGET;
+      p.rows_loss[row] = loss;
+      p.state[row] = state;
+    }
+    if (!p.slot_p) continue;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); /* other lanes' slots */
+    __builtin_amdgcn_wave_barrier();
+    for (int k = lane; k < p.top; k += 64) {
+      int i = si[k];
+      float m = sp[k];
+      for (int j = 0; i >= 0 && j < p.top; j++) {
+        if (si[j] != i || j == k) continue;
+        if (j < k) i = -1; /* folded into slot j */
+        else m += sp[j];
+      }
+      p.slot_p[row * p.top + k] = m;
+      p.slot_i[row * p.top + k] = i;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); /* read before the next row's */
+    __builtin_amdgcn_wave_barrier();
   }
+  __syncthreads();
+  if (threadIdx.x || !p.counts) return;
+  int n = 0;
+  for (int q = 0; q < SLOT_ROWS; q++) n += targets[q];
+  p.counts[blockIdx.x] = (float)n;
+}
+
+/* Ends a row: its loss from the teacher's part and the softmax's sum, one
+ * thread's work.  Gives the log of the sum. */
+template <typename T>
+__device__ inline float finish(const DistillArgs &p, int64_t row, Run all) {
+  /* of no finite logit at all it is -inf, and what follows from it NaN */
+  float lse = Unit<T>::to_natural(all.m) + logf(all.s), state = p.state[row];
+  if (state == BAD_INDEX) lse = NAN;
+  p.rows_loss[row] =
+      state == NO_TARGET ? 0.f : (p.rows_loss[row] + lse) * p.temperature * p.temperature;
+  if (p.lse) p.lse[row] = lse;
+  return lse;
+}
+
+/* A vector as its bits. */
+template <typename T>
+struct Bits {
+  static __device__ u32x4 load(const T *p) {
+    return __builtin_bit_cast(u32x4, *(const typename Loose<T>::type *)p);
+  }
+  static __device__ float get(u32x4 q, int e) {
+    return to_f<T>(__builtin_bit_cast(typename Vec<T>::type, q)[e]);
+  }
+  static __device__ u32x4 nothing() { /* -inf */
+    typename Vec<T>::type v;
+#pragma unroll
+    for (int e = 0; e < Vec<T>::N; e++) v[e] = (T)-INFINITY;
+    return __builtin_bit_cast(u32x4, v);
+  }
+};
+
+/* N vectors' part of the running maximum and sum. */
+template <typename T, int N>
+__device__ inline Run scan_vecs(const u32x4 *q, float c, Run r) {
+  constexpr int V = Vec<T>::N;
+  float top = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < N; u++)
+#pragma unroll
+    for (int e = 0; e < V; e++) top = fmaxf(top, Bits<T>::get(q[u], e));
+  float m = fmaxf(r.m, top * c), s = r.s * Unit<T>::exp(r.m - m);
+#pragma unroll
+  for (int u = 0; u < N; u++)
+#pragma unroll
+    for (int e = 0; e < V; e++) s += Unit<T>::exp(fmaf(Bits<T>::get(q[u], e), c, -m));
+  return {m, s};
+}
+
+/* N vectors TH apart from i on, as far as whole ones go; -inf for the others. */
+template <typename T, int TH, int N>
+__device__ inline void load_vecs(const T *x, int64_t i, int64_t whole, u32x4 *q) {
+#pragma unroll
+  for (int u = 0; u < N; u++)
+    q[u] = i + u * TH < whole ? Bits<T>::load(x + (i + u * TH) * Vec<T>::N) : Bits<T>::nothing();
+}
+
+/* The classes behind the last whole vector, as one vector. */
+template <typename T>
+__device__ inline u32x4 load_tail(const T *x, int64_t v) {
+  constexpr int V = Vec<T>::N;
+  typename Vec<T>::type q;
+#pragma unroll
+  for (int e = 0; e < V; e++) q[e] = v / V * V + e < v ? x[v / V * V + e] : (T)-INFINITY;
+  return __builtin_bit_cast(u32x4, q);
+}
+
+/* The running maximum and sum over vectors i, i + TH, ... below `to`, of
+ * which all but the row's last are whole. */
+template <typename T, int TH>
+__device__ inline Run scan(const DistillArgs &p, const T *x, int64_t i, int64_t to, float c, Run r) {
+  constexpr int U = 4;
+  int64_t whole = min(to, p.v / Vec<T>::N);
+  u32x4 q[U];
+  for (; i < whole; i += U * TH) {
+    load_vecs<T, TH, U>(x, i, whole, q);
+    r = scan_vecs<T, U>(q, c, r);
+  }
+  if (threadIdx.x == 0 && whole < to) {
+    q[0] = load_tail<T>(x, p.v);
+    r = scan_vecs<T, 1>(q, c, r);
+  }
+  return r;
+}
+
+/* Of all TH threads; the first wave has the result. */
+template <typename T, int TH>
+__device__ inline Run join_all(Run r) {
+  __shared__ Run lds[TH / 64];
+#pragma unroll
+  for (int o = 32; o; o >>= 1) r = join<T>(r, wave_neighbour(r, o));
+  if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = r;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    r = lds[0];
+#pragma unroll
+    for (int w = 1; w < TH / 64; w++) r = join<T>(r, lds[w]);
+  }
+  return r;
+}
+
+template <typename T>
+__device__ inline void write_vec(u32x4 q, T *dx, int n, float c, float lse,
+                                 float scale) {
+  constexpr int V = Vec<T>::N;
+  float v[V];
+#pragma unroll
+  for (int e = 0; e < V; e++) v[e] = scale * Unit<T>::exp(fmaf(Bits<T>::get(q, e), c, -lse));
+  store_vec<T>(dx, n, v);
+}
+
+/* The gradient of the same vectors; lse in the exponential's unit. */
+template <typename T, int TH>
+__device__ inline void write(const DistillArgs &p, const T *x, T *dx, int64_t i, int64_t to,
+                             float c, float lse, float scale) {
+  constexpr int U = 4, V = Vec<T>::N;
+  int64_t whole = min(to, p.v / V);
+  u32x4 q[U];
+  for (; i < whole; i += U * TH) {
+    load_vecs<T, TH, U>(x, i, whole, q);
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (i + u * TH < whole) write_vec<T>(q[u], dx + (i + u * TH) * V, V, c, lse, scale);
+  }
+  if (threadIdx.x == 0 && whole < to)
+    write_vec<T>(load_tail<T>(x, p.v), dx + whole * V, (int)(p.v - whole * V), c, lse, scale);
+}
+
+template <typename T, int TH>
+__device__ inline void write_zeros(const DistillArgs &p, T *dx, int64_t i, int64_t to) {
+  constexpr int V = Vec<T>::N;
+  float zero[V] = {};
+  for (; i < to; i += TH) store_vec<T>(dx + i * V, (int)min((int64_t)V, p.v - i * V), zero);
+}
+
+/* A class that the teacher names: its place in the row, its logit and mass. */
+template <typename T>
+struct Named {
+  int at;
+  float x, mass;
+  __device__ Named(const DistillArgs &p, int64_t row, const T *logits, int k) : at(-1), x(0.f), mass(0.f) {
+    if (k >= p.top) return;
+    at = p.slot_i[row * p.top + k];
+    mass = p.slot_p[row * p.top + k];
+    if (at >= 0) x = to_f<T>(logits[at]);
+  }
+  /* from the unrounded q; behind a barrier after the row's other stores */
+  __device__ void write(T *dx, int64_t from, int64_t to, float c, float lse, float scale) const {
+    if (at < 0 || at < from || at >= to) return;
+    dx[at] = from_f<T>(scale * (Unit<T>::exp(fmaf(x, c, -lse)) - mass));
+  }
+};
+
+/* The number of rows with a target, by one wave; all lanes get it. */
+__device__ inline float count_rows(const DistillArgs &p) {
+  float n = 0.f;
+  for (int64_t i = threadIdx.x % 64; i < (p.rows + SLOT_ROWS - 1) / SLOT_ROWS; i += 64)
+    n += p.counts[i];
+  return wave_sum(n);
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void distill_forward(DistillArgs p) {
-  constexpr int V = Vec<T>::N, U = 4;
-  __shared__ Run lds[4];
-  __shared__ float sp[MOST_SLOTS];
-  __shared__ int si[MOST_SLOTS];
+  constexpr int V = Vec<T>::N;
   int64_t row = blockIdx.y + (int64_t)blockIdx.z * 65535;
   if (row >= p.rows) return;
-  float inv_t = 1.f / p.temperature;
   const T *x = (const T *)p.x + row * p.ldx;
   int64_t vecs = (p.v + V - 1) / V;
   int64_t from = vecs * blockIdx.x / p.chunks, to = vecs * (blockIdx.x + 1) / p.chunks;
-  Run r = {-INFINITY, 0.f};
-  for (int64_t i = from + threadIdx.x; i < to; i += 256 * U) {
-    float v[U][V];
-#pragma unroll
-    for (int u = 0; u < U; u++) {
-      int64_t at = i + u * 256;
-      int n = at < to ? (int)min((int64_t)V, p.v - at * V) : 0;
-      load_vec<T>(x + at * V, n, v[u]);
-#pragma unroll
-      for (int e = 0; e < V; e++) v[u][e] = e < n ? v[u][e] * inv_t : -INFINITY;
-    }
-    float m = r.m;
-    bool nan = false;
-#pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-      for (int e = 0; e < V; e++) {
-        m = fmaxf(m, v[u][e]);
-        nan |= v[u][e] != v[u][e];
-      }
-    if (nan) m = NAN;
-    if (m == -INFINITY) continue;
-    float s = r.s ? r.s * exp_of<T>(r.m - m) : 0.f;
-#pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-      for (int e = 0; e < V; e++) s += exp_of<T>(v[u][e] - m);
-    r.m = m;
-    r.s = s;
-  }
-#pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    Run q;
-    q.m = __shfl_xor(r.m, o, 64);
-    q.s = __shfl_xor(r.s, o, 64);
-    r = join<T>(r, q);
-  }
-  if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = r;
-  __syncthreads();
-  if (threadIdx.x >= 64) return;
-  r = join<T>(join<T>(lds[0], lds[1]), join<T>(lds[2], lds[3]));
+  Run r = scan<T, 256>(p, x, from + threadIdx.x, to, Unit<T>::c(p.temperature), no_run());
+  r = join_all<T, 256>(r);
+  if (threadIdx.x) return;
   if (p.chunks == 1) {
-    finish<T>(p, row, r, sp, si);
-  } else if (threadIdx.x == 0) {
+    finish<T>(p, row, r);
+  } else {
     p.part[(row * p.chunks + blockIdx.x) * 2] = r.m;
     p.part[(row * p.chunks + blockIdx.x) * 2 + 1] = r.s;
   }
 }
 
+/* A row's loss and gradient.  The first 16 vectors of each thread stay in
+ * registers in between; what a row has beyond them is read again. */
+template <typename T, int TH>
+__global__ __launch_bounds__(TH) void distill_both(DistillArgs p) {
+  constexpr int V = Vec<T>::N, KEEP = 16, U = 4;
+  __shared__ float told[2];
+  int64_t row = blockIdx.y + (int64_t)blockIdx.z * 65535;
+  if (row >= p.rows) return;
+  const T *x = (const T *)p.x + row * p.ldx;
+  T *dx = (T *)p.dx + row * p.lddx;
+  int64_t whole = p.v / V, vecs = (p.v + V - 1) / V, i = threadIdx.x;
+  float c = Unit<T>::c(p.temperature);
+  u32x4 kept[KEEP];
+  load_vecs<T, TH, KEEP>(x, i, whole, kept);
+  Named<T> named(p, row, x, threadIdx.x);
+  float state = p.state[row], scale = p.temperature * p.scale;
+  if (p.reduction == 2 && threadIdx.x < 64) scale /= fmaxf(count_rows(p), 1.f);
+  Run r = no_run();
+#pragma unroll
+  for (int k = 0; k < KEEP; k += U) {
+    __builtin_amdgcn_sched_barrier(0); /* four vectors unpacked at a time */
+#pragma unroll
+    for (int u = 0; u < U; u++) asm volatile("" : "+v"(kept[k + u]));
+    r = scan_vecs<T, U>(kept + k, c, r);
+  }
+  r = join_all<T, TH>(scan<T, TH>(p, x, i + KEEP * TH, vecs, c, r));
+  if (threadIdx.x == 0) {
+    told[0] = Unit<T>::from_natural(finish<T>(p, row, r));
+    told[1] = scale;
+  }
+  __syncthreads();
+  float lse = told[0];
+  scale = told[1];
+  if (state == NO_TARGET) {
+    write_zeros<T, TH>(p, dx, i, vecs);
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < KEEP; k++) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" : "+v"(kept[k])); /* unpacked anew, not kept unpacked */
+    if (i + k * TH < whole) write_vec<T>(kept[k], dx + (i + k * TH) * V, V, c, lse, scale);
+  }
+  write<T, TH>(p, x, dx, i + KEEP * TH, vecs, c, lse, scale);
+  __threadfence_block();
+  __syncthreads();
+  named.write(dx, 0, p.v, c, lse, scale);
+  for (int k = threadIdx.x + TH; k < p.top; k += TH)
+    Named<T>(p, row, x, k).write(dx, 0, p.v, c, lse, scale);
+}
+
 /* A wave a row: joins the chunks in their order. */
 template <typename T>
 __global__ __launch_bounds__(64) void distill_join(DistillArgs p) {
-  __shared__ float sp[MOST_SLOTS];
-  __shared__ int si[MOST_SLOTS];
   int64_t row = blockIdx.x;
-  Run r = {-INFINITY, 0.f};
+  Run r = no_run();
   for (int c = threadIdx.x; c < p.chunks; c += 64) {
-    Run q;
-    q.m = p.part[(row * p.chunks + c) * 2];
-    q.s = p.part[(row * p.chunks + c) * 2 + 1];
-    r = join<T>(r, q);
+    const float *q = p.part + (row * p.chunks + c) * 2;
+    r = join<T>(r, Run{q[0], q[1]});
   }
 #pragma unroll
-  for (int o = 32; o; o >>= 1) {
-    Run q;
-    q.m = __shfl_xor(r.m, o, 64);
-    q.s = __shfl_xor(r.s, o, 64);
-    r = join<T>(r, q);
-  }
-  finish<T>(p, row, r, sp, si);
+  for (int o = 32; o; o >>= 1) r = join<T>(r, wave_neighbour(r, o));
+  if (threadIdx.x == 0) finish<T>(p, row, r);
 }
 
-/* The rows' losses to one, and how many rows had a target. */
+/* The rows' losses to one. */
 __global__ __launch_bounds__(1024) void distill_total(DistillArgs p) {
-  __shared__ float lds[2][16];
-  float s = 0.f, n = 0.f;
-  for (int64_t r = threadIdx.x; r < p.rows; r += 1024) {
-    s += p.rows_loss[r];
-    n += p.slot_p[r * p.top] >= 0.f || p.slot_p[r * p.top] != p.slot_p[r * p.top] ? 1.f : 0.f;
-  }
+  __shared__ float lds[16];
+  float s = 0.f;
+  for (int64_t r = threadIdx.x; r < p.rows; r += 1024) s += p.rows_loss[r];
   s = wave_sum(s);
-  n = wave_sum(n);
-  if (threadIdx.x % 64 == 0) {
-    lds[0][threadIdx.x / 64] = s;
-    lds[1][threadIdx.x / 64] = n;
-  }
+  if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = s;
   __syncthreads();
+  if (threadIdx.x >= 64) return;
+  float n = p.reduction == 2 ? fmaxf(count_rows(p), 1.f) : 1.f;
   if (threadIdx.x) return;
-  for (int w = 1; w < 16; w++) {
-    s += lds[0][w];
-    n += lds[1][w];
-  }
-  *p.loss = p.reduction == 2 ? s / fmaxf(n, 1.f) : s;
-  *p.count = n;
+  for (int w = 1; w < 16; w++) s += lds[w];
+  *p.loss = s * p.scale / n;
 }
 
+/* Pieces of rows in turn; nothing to do where the forward pass has written
+ * the gradient for an upstream gradient of 1 and that is what came. */
 template <typename T>
 __global__ __launch_bounds__(256) void distill_backward(DistillArgs p) {
   constexpr int V = Vec<T>::N;
-  int64_t row = blockIdx.y + (int64_t)blockIdx.z * 65535;
-  if (row >= p.rows) return;
-  float inv_t = 1.f / p.temperature;
-  const T *x = (const T *)p.x + row * p.ldx;
-  T *dx = (T *)p.dx + row * p.lddx;
-  const float *slot_p = p.slot_p + row * p.top;
-  const int32_t *slot_i = p.slot_i + row * p.top;
-  int64_t vecs = (p.v + V - 1) / V;
-  int64_t from = vecs * blockIdx.x / p.chunks, to = vecs * (blockIdx.x + 1) / p.chunks;
-  bool some = slot_p[0] != -1.f;
-  float scale = p.grad[p.reduction ? 0 : row] * p.temperature;
-  if (p.reduction == 2) scale /= fmaxf(*p.count, 1.f);
-  float lse = p.lse[row];
-  for (int64_t i = from + threadIdx.x; i < to; i += 256) {
-    int n = (int)min((int64_t)V, p.v - i * V);
-    float v[V];
-    if (some) load_vec<T>(x + i * V, n, v);
-#pragma unroll
-    for (int e = 0; e < V; e++) v[e] = some ? scale * exp_of<T>(v[e] * inv_t - lse) : 0.f;
-    store_vec<T>(dx + i * V, n, v);
+  if (p.written && *p.grad == 1.f) return;
+  __shared__ float told;
+  if (threadIdx.x < 64) {
+    float n = p.reduction == 2 ? fmaxf(count_rows(p), 1.f) : 1.f;
+    if (threadIdx.x == 0) told = n;
   }
-  if (!some) return;
-  /* The few classes that the teacher names, from the unrounded q; the
-   * barrier orders them behind this workgroup's own stores. */
-  __threadfence_block();
   __syncthreads();
-  int64_t first = from * V, last = min(to * V, p.v);
-  for (int k = threadIdx.x; k < p.top; k += 256) {
-    int64_t c = slot_i[k];
-    if (c < first || c >= last) continue;
-    float q = exp_of<T>(to_f<T>(x[c]) * inv_t - lse);
-    dx[c] = from_f<T>(scale * (q - slot_p[k]));
+  int64_t vecs = (p.v + V - 1) / V;
+  float c = Unit<T>::c(p.temperature);
+  for (int64_t q = blockIdx.x; q < p.rows * p.chunks; q += gridDim.x) {
+    int64_t row = q / p.chunks, piece = q % p.chunks;
+    int64_t from = vecs * piece / p.chunks, to = vecs * (piece + 1) / p.chunks;
+    const T *x = (const T *)p.x + row * p.ldx;
+    T *dx = (T *)p.dx + row * p.lddx;
+    if (p.state[row] == NO_TARGET) {
+      write_zeros<T, 256>(p, dx, from + threadIdx.x, to);
+      continue;
+    }
+    float scale = p.grad[p.reduction ? 0 : row] * (p.temperature * p.scale / told);
+    float lse = Unit<T>::from_natural(p.lse[row]);
+    write<T, 256>(p, x, dx, from + threadIdx.x, to, c, lse, scale);
+    __threadfence_block();
+    __syncthreads();
+    for (int k = threadIdx.x; k < p.top; k += 256)
+      Named<T>(p, row, x, k).write(dx, from * V, min(to * V, p.v), c, lse, scale);
   }
 }
 
@@ -264,11 +444,23 @@ dim3 rows_grid(int chunks, int64_t rows) {
 
 template <typename T>
 int run(const DistillArgs &p, hipStream_t s) {
-  if (p.dx) {
-    distill_backward<T><<<rows_grid(p.chunks, p.rows), 256, 0, s>>>(p);
+  if (p.grad) {
+    int64_t pieces = p.rows * p.chunks;
+    /* few workgroups where most often there is nothing to do */
+    int64_t most = p.written ? 4096 : (int64_t)1 << 30;
+    distill_backward<T><<<(unsigned)std::min(pieces, most), 256, 0, s>>>(p);
     return OPS_LAUNCHED();
   }
-  distill_forward<T><<<rows_grid(p.chunks, p.rows), 256, 0, s>>>(p);
+  int waves = std::min(16, 65536 / (p.top * 8)); /* as far as 64 KB of LDS go */
+  distill_slots<T><<<(unsigned)((p.rows + SLOT_ROWS - 1) / SLOT_ROWS), waves * 64,
+                     waves * p.top * 8, s>>>(p);
+  /* the fewest threads whose registers hold the row */
+  dim3 grid = rows_grid(p.chunks, p.rows);
+  int64_t bytes = p.v * sizeof(T);
+  if (!p.dx) distill_forward<T><<<grid, 256, 0, s>>>(p);
+  else if (bytes <= 256 * 256) distill_both<T, 256><<<grid, 256, 0, s>>>(p);
+  else if (bytes <= 512 * 256) distill_both<T, 512><<<grid, 512, 0, s>>>(p);
+  else distill_both<T, 1024><<<grid, 1024, 0, s>>>(p);
   if (p.chunks > 1) distill_join<T><<<(unsigned)p.rows, 64, 0, s>>>(p);
   if (p.reduction) distill_total<<<1, 1024, 0, s>>>(p);
   return OPS_LAUNCHED();
@@ -278,8 +470,9 @@ int run(const DistillArgs &p, hipStream_t s) {
 
 extern "C" {
 
-/* Into how many workgroups a row is cut: one where the rows alone fill the
- * card, else pieces of no less than 4096 classes. */
+/* Into how many pieces a row is cut.  Forward: one where the rows alone fill
+ * the card, else pieces of no less than 4096 classes.  Backward: pieces that
+ * workgroups take in turn. */
 int32_t vgpu_ops_distill_chunks(int64_t rows, int64_t v, int32_t backward) {
   int64_t want = backward ? std::max<int64_t>((v + 16383) / 16384, 2048 / rows)
                           : (rows >= 1024 ? 1 : 2048 / rows);
@@ -292,10 +485,12 @@ int vgpu_ops_distill(const DistillArgs *args, void *stream) {
       p.top <= 0 || p.top > MOST_SLOTS || p.chunks < 1 || !(p.temperature > 0.f) ||
       (p.index_bytes != 4 && p.index_bytes != 8) || p.reduction < 0 || p.reduction > 2)
     return OPS_BAD_ARG;
-  if (p.dx ? !(p.grad && p.lse && p.slot_p && p.slot_i && (p.reduction != 2 || p.count))
-           : !p.rows_loss || (p.chunks > 1 && !p.part) ||
-                 (p.reduction && !(p.loss && p.count && p.slot_p && p.slot_i)))
+  if (!p.state) return OPS_BAD_ARG;
+  if (p.grad ? !(p.dx && p.lse && p.slot_p && p.slot_i)
+             : !(p.rows_loss && p.index) || !p.slot_p != !p.slot_i || (p.chunks > 1 && (!p.part || p.dx)) ||
+                   (p.reduction && !p.loss) || (p.dx && !(p.slot_p && p.slot_i && p.reduction)))
     return OPS_BAD_ARG;
+  if (p.reduction == 2 && !p.counts) return OPS_BAD_ARG;
   hipStream_t s = (hipStream_t)stream;
   if (p.dtype == DT_F32) return run<float>(p, s);
   if (p.dtype == DT_BF16) return run<bf16>(p, s);

@@ -10,6 +10,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -109,31 +110,51 @@ __global__ __launch_bounds__(block_of<TH>()) void norm_forward(NormArgs p) {
   }
 }
 
-/* Each row (or wave) of the grid takes every parts-th row, keeps its columns'
- * sums of dy h and dy in registers and writes them once, so x and dy are read
- * a single time for all three gradients. */
+/* Each workgroup takes every parts-th row, or four, keeps its columns' sums of
+ * dy h and dy in registers and writes them once, so x and dy are read a single
+ * time for all three gradients.  The next row is asked for before this one's
+ * sums are taken.  A single workgroup writes the gradients themselves. */
 template <typename T, typename W, int TH, int VECS>
 __global__ __launch_bounds__(block_of<TH>()) void norm_backward(NormArgs p) {
-  constexpr int V = Vec<T>::N;
-  __shared__ float lds[2 * (TH / 64)];
+  constexpr int V = Vec<T>::N, R = rows_at_once<TH>(), WAVES = TH / 64;
+  __shared__ float lds[2][2 * WAVES];
+  __shared__ float waves[TH == 64 ? R - 1 : 1][TH == 64 ? 64 * VECS * V : 1];
   int lane = threadIdx.x % TH;
-  int64_t part = (int64_t)blockIdx.x * rows_at_once<TH>() + threadIdx.x / TH;
   int64_t group = blockIdx.y, d = p.d;
   const W *w = (const W *)p.weight + group * d;
-  float dw[VECS][V] = {}, db[VECS][V] = {};
-  for (int64_t row = part; row < p.rows; row += p.parts) {
+  typedef typename Loose<T>::type raw;
+  raw rx[VECS], rg[VECS];
+  float row_mean = 0.f, row_rstd = 0.f;
+  auto fetch = [&](int64_t row) {
+    if (row >= p.rows) return;
     const T *x = (const T *)p.x + row * p.ldx + group * d;
     const T *dy = (const T *)p.dy + row * p.lddy + group * d;
-    float mean = p.mean[row * p.groups + group], rstd = p.rstd[row * p.groups + group];
-    float h[VECS][V], a[VECS][V];
-    float s[2] = {0.f, 0.f};
+    row_mean = p.mean[row * p.groups + group];
+    row_rstd = p.rstd[row * p.groups + group];
 #pragma unroll
     for (int i = 0; i < VECS; i++) {
       int64_t at = (int64_t)(i * TH + lane) * V;
       int n = (int)min((int64_t)V, d - at);
-      load_vec<T>(x + at, n, h[i]);
-      load_vec<T>(dy + at, n, a[i]);
+      rx[i] = load_raw<T>(x + at, n);
+      rg[i] = load_raw<T>(dy + at, n);
     }
+  };
+  float dw[VECS][V] = {}, db[VECS][V] = {};
+  int64_t step = (int64_t)p.parts * R;
+  int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / TH;
+  fetch(row);
+  for (int turn = 0; row < p.rows; row += step, turn ^= 1) {
+    float mean = row_mean, rstd = row_rstd;
+    float h[VECS][V], a[VECS][V];
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < VECS; i++)
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        h[i][e] = to_f<T>(rx[i][e]);
+        a[i][e] = to_f<T>(rg[i][e]);
+      }
+    fetch(row + step);
 #pragma unroll
     for (int i = 0; i < VECS; i++) {
       int64_t at = (int64_t)(i * TH + lane) * V;
@@ -155,7 +176,22 @@ __global__ __launch_bounds__(block_of<TH>()) void norm_backward(NormArgs p) {
       }
     }
     if (!p.dx) continue; /* the same for all threads */
-    row_sum<TH>(s, lds);
+    /* the row before used the other half of lds, and every wave has passed
+     * the barrier since */
+#pragma unroll
+    for (int c = 0; c < 2; c++) s[c] = wave_sum(s[c]);
+    if constexpr (WAVES > 1) {
+      if (threadIdx.x % 64 == 0)
+#pragma unroll
+        for (int c = 0; c < 2; c++) lds[turn][c * WAVES + threadIdx.x / 64] = s[c];
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        s[c] = 0.f;
+#pragma unroll
+        for (int q = 0; q < WAVES; q++) s[c] += lds[turn][c * WAVES + q];
+      }
+    }
     float ma = s[0] / d, mah = s[1] / d;
     T *dx = (T *)p.dx + row * p.lddx + group * d;
 #pragma unroll
@@ -168,17 +204,46 @@ __global__ __launch_bounds__(block_of<TH>()) void norm_backward(NormArgs p) {
       store_vec<T>(dx + at, n, o);
     }
   }
-  if (!p.part) return;
-  float *pw = p.part + part * p.groups * d + group * d, *pb = pw + (int64_t)p.parts * p.groups * d;
+  if (!p.dweight && !p.dbias) return;
+  if constexpr (TH == 64) { /* the four waves' sums, in their order */
+    int wave = threadIdx.x / 64;
+    auto add = [&](float(&v)[VECS][V]) {
+      __syncthreads();
+      if (wave)
 #pragma unroll
-  for (int i = 0; i < VECS; i++) {
-    int64_t at = (int64_t)(i * TH + lane) * V;
-    int n = (int)min((int64_t)V, d - at);
+        for (int i = 0; i < VECS; i++)
 #pragma unroll
-    for (int c = 0; c < V; c += 4) {
-      store_vec<float>(pw + at + c, n - c, dw[i] + c);
-      store_vec<float>(pb + at + c, n - c, db[i] + c);
+          for (int e = 0; e < V; e++) waves[wave - 1][(i * V + e) * 64 + lane] = v[i][e];
+      __syncthreads();
+      if (!wave)
+#pragma unroll
+        for (int i = 0; i < VECS; i++)
+#pragma unroll
+          for (int e = 0; e < V; e++)
+            for (int q = 0; q < R - 1; q++) v[i][e] += waves[q][(i * V + e) * 64 + lane];
+    };
+    add(dw);
+    add(db);
+    if (wave) return;
+  }
+  auto write = [&](auto *out, float(&v)[VECS][V]) {
+    typedef std::remove_pointer_t<decltype(out)> D;
+    constexpr int VD = Vec<D>::N;
+#pragma unroll
+    for (int i = 0; i < VECS; i++) {
+      int64_t at = (int64_t)(i * TH + lane) * V;
+      int n = (int)min((int64_t)V, d - at);
+#pragma unroll
+      for (int c = 0; c < V; c += VD) store_vec<D>(out + group * d + at + c, n - c, v[i] + c);
     }
+  };
+  if (p.parts == 1) {
+    if (p.dweight) write((W *)p.dweight, dw);
+    if (p.dbias) write((W *)p.dbias, db);
+  } else {
+    int64_t width = p.groups * d;
+    write(p.part + blockIdx.x * width, dw);
+    write(p.part + (p.parts + blockIdx.x) * width, db);
   }
 }
 
@@ -196,7 +261,7 @@ void launch(const NormArgs &p, hipStream_t s) {
   constexpr int R = rows_at_once<TH>();
   if (p.dy)
     norm_backward<T, W, TH, VECS>
-        <<<dim3(p.parts / R, (unsigned)p.groups), block_of<TH>(), 0, s>>>(p);
+        <<<dim3(p.parts, (unsigned)p.groups), block_of<TH>(), 0, s>>>(p);
   else
     norm_forward<T, W, TH, VECS>
         <<<dim3((unsigned)((p.rows + R - 1) / R), (unsigned)p.groups), block_of<TH>(), 0, s>>>(p);
@@ -212,7 +277,7 @@ void dispatch(const NormArgs &p, hipStream_t s) {
   else if (p.d <= 256 * 32) launch<T, W, 256, 32>(p, s);
   else if (p.d <= 512 * 32) launch<T, W, 512, 32>(p, s);
   else launch<T, W, 1024, 32>(p, s);
-  if (p.dy && p.part) {
+  if (p.dy && p.parts > 1 && (p.dweight || p.dbias)) {
     int64_t width = p.groups * p.d;
     norm_join<W><<<dim3((unsigned)((width + 63) / 64), 2), 1024, 0, s>>>(p);
   }
@@ -230,19 +295,20 @@ int run(const NormArgs &p, hipStream_t s) {
 
 extern "C" {
 
-/* How many partial sums of the weight's gradient: enough rows in flight for
- * 256 CUs, no more than there are rows, whole workgroups. */
+/* How many workgroups share the rows: two a CU, and four rows in a row's
+ * place each, so that up to four (or, of short rows, sixteen) rows need no
+ * partial sums. */
 int32_t vgpu_ops_norm_parts(int64_t rows, int64_t groups, int64_t d) {
-  int64_t at_once = d <= 2048 ? 4 : 1;
-  int64_t most = (d <= 2048 ? 2048 : 512) / std::min<int64_t>(groups, 32);
-  int64_t parts = std::max<int64_t>(1, std::min(rows, most));
-  return (int32_t)((parts + at_once - 1) / at_once * at_once);
+  int64_t at_once = d <= 64 * 32 ? 4 : 1, share = 4 * at_once;
+  int64_t most = std::max<int64_t>(1, 512 / groups);
+  return (int32_t)std::max<int64_t>(1, std::min((rows + share - 1) / share, most));
 }
 
 int vgpu_ops_norm(const NormArgs *args, void *stream) {
   const NormArgs &p = *args;
   if (p.rows <= 0 || p.rows >= (int64_t)1 << 31 || p.groups <= 0 || p.groups > 65535 || p.d <= 0 ||
-      p.d > 1024 * 32 || (p.dy ? p.parts != vgpu_ops_norm_parts(p.rows, p.groups, p.d) : !p.y))
+      p.d > 1024 * 32 ||
+      (p.dy ? p.parts < 1 || (p.parts > 1 && (p.dweight || p.dbias) && !p.part) : !p.y))
     return OPS_BAD_ARG;
   hipStream_t s = (hipStream_t)stream;
   if (p.dtype == DT_F32) return run<float>(p, s);

@@ -36,9 +36,9 @@ NormArgs = _struct(
     d=(c_float, "eps"))
 DistillArgs = _struct(
     "DistillArgs",
-    a=(c_void_p, "x index teacher dx grad rows_loss lse slot_p loss count slot_i part"),
+    a=(c_void_p, "x index teacher dx grad rows_loss state lse slot_p loss counts slot_i part"),
     b=(c_int64, "ldx lddx ldi ldt rows v"),
-    c=(c_int32, "dtype ttype index_bytes top chunks reduction"), d=(c_float, "temperature"))
+    c=(c_int32, "dtype ttype index_bytes top chunks reduction written"), d=(c_float, "temperature scale"))
 
 
 @lru_cache(maxsize=None)
@@ -66,13 +66,6 @@ def library() -> ctypes.CDLL:
     return lib
 
 
-@lru_cache(maxsize=None)
-def _check_arch(device: int) -> None:
-    arch = torch.cuda.get_device_properties(device).gcnArchName
-    if not arch.startswith("gfx950"):
-        raise RuntimeError(f"the head operators are built for gfx950, not {arch}")
-
-
 def on_gpu(*tensors) -> bool:
     """Whether the kernels run: ordinary tensors on a GPU, and nothing that
     traces or transforms the call.  Otherwise the plain formula runs."""
@@ -83,18 +76,39 @@ def on_gpu(*tensors) -> bool:
                 or torch._C._are_functorch_transforms_active())
 
 
-def launch(name: str, args, device: torch.device) -> None:
+_entries = {}   # name -> bound function
+_devices = set()  # whose architecture has been looked at
+
+
+def _bind(name):
+    return _entries.setdefault(name, getattr(library(), "vgpu_ops_" + name))
+
+
+def _look_at(index):
+    arch = torch.cuda.get_device_properties(index).gcnArchName
+    if not arch.startswith("gfx950"):
+        raise RuntimeError(f"the head operators are built for gfx950, not {arch}")
+    _devices.add(index)
+
+
+def launch(name: str, device: torch.device, *args) -> None:
     """Runs an entry point on the device's current stream."""
     index = device.index
-    if index != torch.cuda.current_device():
+    if index not in _devices:
+        _look_at(index)
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
-            return launch(name, args, device)
-    _check_arch(index)
-    rc = getattr(library(), "vgpu_ops_" + name)(
-        ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+            return launch(name, device, *args)
+    rc = (_entries.get(name) or _bind(name))(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         raise RuntimeError(f"vgpu_ops_{name}: " + ("refused the arguments" if rc < 0
                                                    else f"HIP error {rc}"))
+
+
+@lru_cache(maxsize=4096)
+def plan(name: str, *sizes) -> int:
+    """What a launch of these sizes needs; a function of the sizes alone."""
+    return getattr(library(), "vgpu_ops_" + name)(*sizes)
 
 
 def needs_grad(*tensors) -> bool:
@@ -113,7 +127,8 @@ def ptr(t) -> int | None:
 
 def same_device(**tensors) -> None:
     devices = {name: t.device for name, t in tensors.items() if t is not None}
-    if len(set(devices.values())) > 1:
+    one = next(iter(devices.values()))
+    if any(d != one for d in devices.values()):
         raise ValueError("tensors on different devices: "
                          + ", ".join(f"{n} on {d}" for n, d in devices.items()))
 

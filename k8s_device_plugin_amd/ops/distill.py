@@ -9,6 +9,8 @@ in fp32.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _native
@@ -18,7 +20,8 @@ REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 MOST_SLOTS = 1024
 
 
-def distill_loss(logits, index, teacher=None, *, temperature=1.0, reduction="mean"):
+def distill_loss(logits, index, teacher=None, *, temperature=1.0, reduction="mean",
+                 scale=1.0):
     """The loss of ``logits`` [..., V] against a teacher whose top classes
     are ``index`` [..., K] (int32 or int64) with logits ``teacher`` [..., K].
 
@@ -30,14 +33,21 @@ def distill_loss(logits, index, teacher=None, *, temperature=1.0, reduction="mea
     ``index[..., 0]``.
 
     reduction: "none" gives float32 [...], "sum" their sum, "mean" the sum
-    divided by the number of rows that have a slot (at least 1).  T^2 keeps
-    gradients of one size over temperatures.  Differentiable in logits alone;
-    K at most 1024.  On the CPU, and while a call is traced or transformed,
+    divided by the number of rows that have a slot (at least 1), times
+    ``scale``.  T^2 keeps gradients of one size over temperatures.
+    Differentiable in logits alone; K at most 1024.
+
+    Where a gradient is wanted of a loss that is one number, it is written
+    along with the loss, for an upstream gradient of 1, and held until
+    backward.  Another upstream gradient costs a second writing: a factor that
+    is known before, as 1/n for n accumulated steps, belongs in ``scale``.  On the CPU, and while a call is traced or transformed,
     the formula is run by torch.  Runs on the current stream of the logits'
     device; can be captured into a graph.  Results do not depend on the run.
     """
     if reduction not in REDUCTIONS:
         raise ValueError(f"reduction {reduction!r}: one of {', '.join(REDUCTIONS)}")
+    if not math.isfinite(scale) or (scale != 1 and reduction == "none"):
+        raise ValueError(f"scale {scale} with reduction {reduction!r}")
     if not 1e-4 <= temperature <= 1e4:
         raise ValueError(f"temperature {temperature}: wanted 1e-4 to 1e4")
     if logits.dim() < 1 or logits.shape[-1] == 0:
@@ -59,7 +69,7 @@ def distill_loss(logits, index, teacher=None, *, temperature=1.0, reduction="mea
         raise ValueError(f"{top} slots: at most {MOST_SLOTS}")
     _native.same_device(logits=logits, index=index, teacher=teacher)
     if not _native.on_gpu(logits, index, teacher) or logits.numel() == 0 or top == 0:
-        return _plain(logits, index, teacher, temperature, reduction)
+        return _plain(logits, index, teacher, temperature, reduction, scale)
     for t in (logits, teacher):
         if t is not None and t.dtype not in DTYPES:
             raise TypeError(
@@ -67,11 +77,11 @@ def distill_loss(logits, index, teacher=None, *, temperature=1.0, reduction="mea
     if logits.shape[-1] >= 1 << 31:
         raise ValueError(f"{logits.shape[-1]} classes: at most 2^31 - 1")
     if _native.needs_grad(logits):
-        return _Distill.apply(logits, index, teacher, temperature, reduction)
-    return _forward(logits, index, teacher, temperature, REDUCTIONS[reduction], False)[0]
+        return _Distill.apply(logits, index, teacher, temperature, reduction, scale)
+    return _forward(logits, index, teacher, temperature, REDUCTIONS[reduction], scale, False)[0]
 
 
-def _plain(logits, index, teacher, temperature, reduction):
+def _plain(logits, index, teacher, temperature, reduction, scale):
     kind = logits.dtype if logits.dtype == torch.float64 else torch.float32
     if teacher is None:
         teacher = torch.zeros_like(index, dtype=torch.float32)
@@ -88,7 +98,7 @@ def _plain(logits, index, teacher, temperature, reduction):
     rows = torch.where(some, rows, 0.0) * torch.where(bad, torch.nan, 1.0)
     if reduction == "none":
         return rows
-    total = rows.sum()
+    total = rows.sum() * scale
     return total if reduction == "sum" else total / some.sum().clamp_min(1)
 
 
@@ -98,67 +108,79 @@ def _inputs(logits, index, teacher):
             None if teacher is None else rows_of(teacher, top))
 
 
-def _forward(logits, index, teacher, temperature, reduction, keep):
-    """The loss, and what backward needs: one buffer of the rows' log sums,
-    the slots' masses and classes and the number of rows with a target."""
+def _forward(logits, index, teacher, temperature, reduction, scale, keep):
+    """The loss; and, to keep for backward, a buffer of the rows' states and
+    log sums, the slots' masses and classes and the counts of rows with a
+    target, and the gradient for an upstream gradient of 1, where writing it
+    now is cheapest."""
     x, i, t = _inputs(logits, index, teacher)
     rows, v = x.shape
     top = i.shape[1]
     device = logits.device
-    chunks = _native.library().vgpu_ops_distill_chunks(rows, v, 0)
+    chunks = _native.plan("distill_chunks", rows, v, 0)
+    # one workgroup a row has it in registers when its gradient can be
+    # written; few long rows are better cut in pieces, and wait for backward
+    dx = None
+    if keep and reduction and chunks == 1:
+        dx = torch.empty(logits.shape, dtype=logits.dtype, device=device)
     part = (torch.empty(rows * chunks * 2, dtype=torch.float32, device=device)
             if chunks > 1 else None)
     rows_loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=device)
-    loss = rows_loss
-    saved = at = None
-    if keep or reduction:
-        saved = torch.empty(rows + 2 * rows * top + 1, dtype=torch.float32, device=device)
-        at = saved.data_ptr()
-    if reduction:
-        loss = torch.empty((), dtype=torch.float32, device=device)
-    launch("distill", _arguments(
-        x, i, t, at, rows, v, top, temperature, reduction, chunks, rows_loss=rows_loss.data_ptr(),
-        loss=loss.data_ptr(), part=ptr(part)), device)
-    return loss, saved
-
-
-def _arguments(x, i, t, at, rows, v, top, temperature, reduction, chunks, **more):
-    a = DistillArgs(x=x.data_ptr(), index=ptr(i), teacher=ptr(t), ldx=x.stride(0), rows=rows, v=v,
-                    dtype=DTYPES[x.dtype], top=top, chunks=chunks, reduction=reduction,
-                    temperature=temperature, index_bytes=8, **more)
-    if at:
-        a.lse, a.slot_p = at, at + 4 * rows
-        a.slot_i, a.count = at + 4 * rows * (1 + top), at + 4 * rows * (1 + 2 * top)
-    if i is not None:
-        a.ldi, a.index_bytes = i.stride(0), i.element_size()
+    loss = torch.empty((), dtype=torch.float32, device=device) if reduction else rows_loss
+    saved = torch.empty((rows * (2 + 2 * top) if keep else rows) + (rows + 15) // 16,
+                        dtype=torch.float32, device=device)
+    a = _arguments(x, saved, rows, v, top, temperature, reduction, scale, chunks, keep)
+    a.index, a.ldi, a.index_bytes = i.data_ptr(), i.stride(0), i.element_size()
     if t is not None:
-        a.ldt, a.ttype = t.stride(0), DTYPES[t.dtype]
+        a.teacher, a.ldt, a.ttype = t.data_ptr(), t.stride(0), DTYPES[t.dtype]
+    a.rows_loss, a.loss, a.part = rows_loss.data_ptr(), loss.data_ptr(), ptr(part)
+    if dx is not None:
+        a.dx, a.lddx = dx.data_ptr(), v
+    launch("distill", device, a)
+    return loss, saved, dx
+
+
+def _arguments(x, saved, rows, v, top, temperature, reduction, scale, chunks, keep):
+    a = DistillArgs(x=x.data_ptr(), ldx=x.stride(0), rows=rows, v=v, dtype=DTYPES[x.dtype], top=top,
+                    chunks=chunks, reduction=reduction, temperature=temperature, scale=scale,
+                    index_bytes=8)
+    a.state = at = saved.data_ptr()
+    at += 4 * rows
+    if keep:
+        a.lse, a.slot_p, a.slot_i = at, at + 4 * rows, at + 4 * rows * (1 + top)
+        at += 4 * rows * (1 + 2 * top)
+    a.counts = at
     return a
 
 
 class _Distill(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, index, teacher, temperature, reduction):
-        loss, saved = _forward(logits, index, teacher, temperature, REDUCTIONS[reduction], True)
-        ctx.temperature, ctx.reduction = temperature, reduction
+    def forward(ctx, logits, index, teacher, temperature, reduction, scale):
+        ctx.how = temperature, reduction, scale
+        loss, saved, ctx.dx = _forward(logits, index, teacher, temperature, REDUCTIONS[reduction],
+                                       scale, True)
         ctx.save_for_backward(logits, index, teacher, saved)
         return loss
 
     @staticmethod
     def backward(ctx, grad):
         logits, index, teacher, saved = ctx.saved_tensors
+        # handed out once: what a caller does to it must not reach a second
+        # backward pass, which writes its own
+        dx, ctx.dx = ctx.dx, None
         if torch.is_grad_enabled():
-            found = _native.gradients_of(
-                lambda x: _plain(x, index, teacher, ctx.temperature, ctx.reduction), (logits,),
-                (True,), grad)
-            return (*found, None, None, None, None)
+            found = _native.gradients_of(lambda x: _plain(x, index, teacher, *ctx.how), (logits,),
+                                         (True,), grad)
+            return (*found, None, None, None, None, None)
         x = rows_of(logits, logits.shape[-1])
         rows, v = x.shape
         grad = grad.contiguous()
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        chunks = _native.library().vgpu_ops_distill_chunks(rows, v, 1)
-        launch("distill", _arguments(
-            x, None, None, saved.data_ptr(), rows, v, index.shape[-1], ctx.temperature,
-            REDUCTIONS[ctx.reduction], chunks, dx=dx.data_ptr(), lddx=v, grad=grad.data_ptr()),
-            logits.device)
-        return dx, None, None, None, None
+        temperature, reduction, scale = ctx.how
+        a = _arguments(x, saved, rows, v, index.shape[-1], temperature, REDUCTIONS[reduction],
+                       scale, _native.plan("distill_chunks", rows, v, 1), True)
+        a.written = dx is not None
+        if dx is None:
+            dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        a.dx, a.lddx, a.grad = dx.data_ptr(), v, grad.data_ptr()
+        launch("distill", logits.device, a)
+        return dx, None, None, None, None, None

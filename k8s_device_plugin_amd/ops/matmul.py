@@ -97,12 +97,8 @@ def _operand(t, any_axis=True):
     if wide * size >= 1 << 23:
         raise ValueError(f"linear: {k} values to sum over, the most is {(1 << 23) // size - 8}")
     out = torch.empty((rows, wide), dtype=t.dtype, device=t.device)
-    with torch.cuda.device(t.device):
-        rc = _native.library().vgpu_ops_repack(
-            t.data_ptr(), s0, s1, rows, k, out.data_ptr(), wide, DTYPES[t.dtype],
-            torch._C._cuda_getCurrentRawStream(t.device.index))
-    if rc:
-        raise RuntimeError(f"vgpu_ops_repack: error {rc}")
+    launch("repack", t.device, t.data_ptr(), s0, s1, rows, k, out.data_ptr(), wide,
+           DTYPES[t.dtype])
     return out, wide, 1, rows * wide * size, wide
 
 
@@ -121,11 +117,11 @@ def _gemm(a, b, out, bias=None, residual=None, act=0, z=None):
     plan, splits = _plan(m, n, k, dtype, a_kc, b_kc, bare)
     work = (torch.empty(splits * m * n, dtype=torch.float32, device=out.device)
             if splits > 1 else None)
-    launch("gemm", GemmArgs(
+    launch("gemm", out.device, GemmArgs(
         a.data_ptr(), b.data_ptr(), lda, ldb, a_extent, b_extent, m, n, k, ptr(bias),
         ptr(residual), residual.stride(0) if residual is not None else 0, out.data_ptr(),
         out.stride(0), ptr(z), z.stride(0) if z is not None else 0, ptr(work),
-        dtype, a_kc, b_kc, act, plan, splits), out.device)
+        dtype, a_kc, b_kc, act, plan, splits))
 
 
 def _forward(x, weight, bias, residual, act, keep):
@@ -155,13 +151,13 @@ def _slope(dy, z, act, want_dz, want_db, dtype):
     wide = -(-n // lanes) * lanes
     dz = torch.empty((m, wide), dtype=dtype, device=dy.device) if want_dz else None
     db = part = None
-    parts = _native.library().vgpu_ops_slope_parts(m, n, code)
+    parts = _native.plan("slope_parts", m, n, code)
     if want_db:
         db = torch.empty(n, dtype=dtype, device=dy.device)
         part = torch.empty(parts * n, dtype=torch.float32, device=dy.device)
-    launch("slope", SlopeArgs(
+    launch("slope", dy.device, SlopeArgs(
         dy.data_ptr(), ptr(z), ptr(dz), ptr(db), ptr(part), dy.stride(0),
-        z.stride(0) if z is not None else 0, wide, m, n, code, act, parts), dy.device)
+        z.stride(0) if z is not None else 0, wide, m, n, code, act, parts))
     return dz, db
 
 

@@ -78,10 +78,10 @@ def _forward(x, weight, bias, groups, eps, keep):
     weight, bias = _vector(weight), _vector(bias)
     kind = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
     at = ptr(stats)
-    launch("norm", NormArgs(
+    launch("norm", x.device, NormArgs(
         x2.data_ptr(), ptr(weight), ptr(bias), None, y.data_ptr(), None, None, None,
         at, at and at + 4 * rows * groups, None, x2.stride(0), width, 0, 0, rows, groups,
-        width // groups, DTYPES[x.dtype], DTYPES[kind], 0, eps), x.device)
+        width // groups, DTYPES[x.dtype], DTYPES[kind], 0, eps))
     return y, stats
 
 
@@ -108,14 +108,13 @@ class _LayerNorm(torch.autograd.Function):
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
         dw = torch.empty(width, dtype=weight.dtype, device=x.device) if need_w else None
         db = torch.empty(width, dtype=bias.dtype, device=x.device) if need_b else None
-        parts = _native.library().vgpu_ops_norm_parts(rows, groups, d)
+        parts = _native.plan("norm_parts", rows, groups, d)
         part = (torch.empty(2 * parts * width, dtype=torch.float32, device=x.device)
-                if need_w or need_b else None)
+                if parts > 1 and (need_w or need_b) else None)
         kind = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
         weight = _vector(weight)
-        launch("norm", NormArgs(
+        launch("norm", x.device, NormArgs(
             x2.data_ptr(), ptr(weight), None, dy2.data_ptr(), None, ptr(dx), ptr(dw), ptr(db),
             stats.data_ptr(), stats.data_ptr() + 4 * rows * groups, ptr(part), x2.stride(0), 0,
-            dy2.stride(0), width, rows, groups, d, DTYPES[x.dtype], DTYPES[kind], parts, ctx.eps),
-            x.device)
+            dy2.stride(0), width, rows, groups, d, DTYPES[x.dtype], DTYPES[kind], parts, ctx.eps))
         return dx, dw, db, None, None

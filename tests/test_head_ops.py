@@ -401,10 +401,11 @@ def exact_rows(x64, index, teacher, t):
     return torch.stack(rows)
 
 
-def check_distill(logits, index, teacher, t=1.0, reduction="mean", upstream=None):
+def check_distill(logits, index, teacher, t=1.0, reduction="mean", upstream=None, scale=1.0):
     leaf = logits.detach().requires_grad_()
-    loss = ops.distill_loss(leaf, index, teacher, temperature=t, reduction=reduction)
-    again = ops.distill_loss(logits.detach(), index, teacher, temperature=t, reduction=reduction)
+    loss = ops.distill_loss(leaf, index, teacher, temperature=t, reduction=reduction, scale=scale)
+    again = ops.distill_loss(logits.detach(), index, teacher, temperature=t, reduction=reduction,
+                             scale=scale)
     assert torch.equal(loss.detach(), again) and loss.dtype == torch.float32
     v, top = logits.shape[-1], index.shape[-1]
     flat, i2, t2 = logits.detach().reshape(-1, v).cpu(), index.reshape(-1, top).cpu(), teacher.reshape(-1, top).cpu()
@@ -412,7 +413,7 @@ def check_distill(logits, index, teacher, t=1.0, reduction="mean", upstream=None
     rows = exact_rows(x64, i2, t2, t)
     some = ((i2 >= 0) & (t2 != -float("inf"))).any(1)
     count = max(1, int(some.sum())) if reduction == "mean" else 1
-    want = rows if reduction == "none" else rows.sum() / count
+    want = rows if reduction == "none" else rows.sum() * (scale / count)
     g = torch.ones(()) if upstream is None else upstream
     grad, = torch.autograd.grad(loss, leaf, g.to(loss.device).expand_as(loss))
     dx, = torch.autograd.grad(want, x64, g.double().expand_as(want))
@@ -430,10 +431,10 @@ def check_distill(logits, index, teacher, t=1.0, reduction="mean", upstream=None
     if reduction == "none":
         slack = rows_off
     else:
-        slack = (rows_off.sum() + (len(rows) + 4) * U * rows.detach().abs().sum()) / count
+        slack = (rows_off.sum() + (len(rows) + 4) * U * rows.detach().abs().sum()) * abs(scale) / count
     within(loss.detach().cpu().reshape(want.shape), want.detach(), slack)
     q = (torch.where(some[:, None], s, torch.zeros_like(s)) - lse).exp() * some[:, None]
-    each = (g.double().abs().expand(rows.shape) * t / count)[:, None]
+    each = (g.double().abs().expand(rows.shape) * t * abs(scale) / count)[:, None]
     # p's mass on a class is at most q + |dx| / each
     mass = q + dx.abs() / each.clamp_min(1e-300)
     slack = each * (q * (lse_off + 8 * U * (4 + (s.nan_to_num(0, 0, 0) - lse).abs())) + mass * (p_off + 8 * U))
@@ -455,7 +456,7 @@ def distill_inputs(rows, v, top, dtype, device, seed=0, masked=0.0, itype=torch.
 @pytest.mark.parametrize("rows,v,top,t,reduction", [
     (1, 1, 1, 1.0, "mean"), (1, 2, 2, 2.0, "none"), (3, 21, 5, 1.5, "sum"), (20, 1000, 1, 1.0, "mean"),
     (7, 1001, 64, 2.0, "mean"), (5, 4097, 20, 4.0, "none"), (2, 33333, 100, 0.5, "mean"),
-    (1, 70001, 1024, 1.0, "sum"), (70, 515, 70, 1.0, "mean"), (1030, 40, 3, 1.0, "mean")])
+    (1, 70001, 1024, 1.0, "sum"), (1030, 4100, 300, 1.0, "mean"), (40, 4000, 1024, 1.0, "sum"), (70, 515, 70, 1.0, "mean"), (1030, 40, 3, 1.0, "mean")])
 def test_distill(device, dtype, rows, v, top, t, reduction):
     check_distill(*distill_inputs(rows, v, top, dtype, device, seed=v), t, reduction)
     check_distill(*distill_inputs(rows, v, top, dtype, device, seed=v + 1, masked=0.4,
@@ -482,6 +483,9 @@ def test_distill_masks_duplicates_and_extremes(device, dtype, reduction):
     check_distill(logits, index, teacher, 2.0, reduction, upstream=torch.tensor(-0.37))
     if reduction == "none":
         check_distill(logits, index, teacher, 1.0, reduction, upstream=normal(seeded(5), 8))
+    else:
+        check_distill(logits, index, teacher, 2.0, reduction, scale=-1.75)
+        check_distill(logits, index, teacher, 2.0, reduction, torch.tensor(3.0), scale=0.125)
 
 
 @pytest.mark.parametrize("device,dtype", PAIRS)
@@ -573,6 +577,9 @@ def test_distill_refusals(device):
     for bad in (0.0, -1.0, float("nan"), float("inf")):
         with pytest.raises(ValueError, match="temperature"):
             ops.distill_loss(logits, index, teacher, temperature=bad)
+    for bad, how in ((2.0, "none"), (float("nan"), "mean"), (float("inf"), "sum")):
+        with pytest.raises(ValueError, match="scale"):
+            ops.distill_loss(logits, index, teacher, scale=bad, reduction=how)
     with pytest.raises(ValueError, match="does not fit"):
         ops.distill_loss(logits, index[:, :2], teacher)
     with pytest.raises(ValueError, match="does not fit"):
@@ -761,3 +768,22 @@ def test_missing_library_is_an_error(monkeypatch, tmp_path):
     with pytest.raises(RuntimeError, match="make native"):
         _native.library()
     _native.library.cache_clear()
+
+
+@pytest.mark.parametrize("device,dtype", PAIRS)
+@pytest.mark.parametrize("rows,v", [(20, 1000), (600, 9001)])
+def test_distill_backward_twice(device, dtype, rows, v):
+    """The gradient that a first backward pass hands out is the caller's: a
+    second pass does not see what was done to it."""
+    logits, index, teacher = distill_inputs(rows, v, 3, dtype, device)
+    leaf = logits.requires_grad_()
+    loss = ops.distill_loss(leaf, index, teacher, temperature=2.0)
+    first, = torch.autograd.grad(loss, leaf, retain_graph=True)
+    kept = first.clone()
+    first.mul_(7)
+    second, = torch.autograd.grad(loss, leaf, retain_graph=True)
+    assert torch.equal(second, kept)
+    leaf.grad = None
+    loss.backward(retain_graph=True)
+    loss.backward()
+    assert torch.equal(leaf.grad, kept + kept)
