@@ -123,7 +123,21 @@ __global__ __launch_bounds__(block_of<TH>()) void norm_backward(NormArgs p) {
   int64_t group = blockIdx.y, d = p.d;
   const W *w = (const W *)p.weight + group * d;
   typedef typename Loose<T>::type raw;
+  constexpr int VW = Vec<W>::N;
   raw rx[VECS], rg[VECS];
+  typename Loose<W>::type rw[VECS][V / VW];
+  /* the weight stays in registers: loads end in their order, so one inside
+   * the loop would wait for the next row's */
+#pragma unroll
+  for (int i = 0; i < VECS; i++)
+#pragma unroll
+    for (int c = 0; c < V; c += VW) {
+      int64_t at = (int64_t)(i * TH + lane) * V + c;
+      if (p.weight) rw[i][c / VW] = load_raw<W>(w + at, (int)min((int64_t)VW, d - at));
+      else
+#pragma unroll
+        for (int e = 0; e < VW; e++) rw[i][c / VW][e] = (W)1.f;
+    }
   float row_mean = 0.f, row_rstd = 0.f;
   auto fetch = [&](int64_t row) {
     if (row >= p.rows) return;
@@ -159,18 +173,12 @@ __global__ __launch_bounds__(block_of<TH>()) void norm_backward(NormArgs p) {
     for (int i = 0; i < VECS; i++) {
       int64_t at = (int64_t)(i * TH + lane) * V;
       int n = (int)min((int64_t)V, d - at);
-      float t[V];
-      if (p.weight) {
-        constexpr int VW = Vec<W>::N;
-#pragma unroll
-        for (int c = 0; c < V; c += VW) load_vec<W>(w + at + c, n - c, t + c);
-      }
 #pragma unroll
       for (int e = 0; e < V; e++) {
         h[i][e] = e < n ? (h[i][e] - mean) * rstd : 0.f;
         dw[i][e] += a[i][e] * h[i][e];
         db[i][e] += a[i][e];
-        if (p.weight) a[i][e] *= t[e];
+        a[i][e] *= to_f<W>(rw[i][e / VW][e % VW]);
         s[0] += a[i][e];
         s[1] += a[i][e] * h[i][e];
       }
@@ -267,15 +275,17 @@ void launch(const NormArgs &p, hipStream_t s) {
         <<<dim3((unsigned)((p.rows + R - 1) / R), (unsigned)p.groups), block_of<TH>(), 0, s>>>(p);
 }
 
-/* The fewest threads whose registers hold the row, 32 values each at most. */
+/* The fewest threads whose registers hold the row, with 16 values each or (of
+ * one wave's rows, and the widest) 32.  16384 x 8192 bf16 backward: 165 us with
+ * 512 threads of 16, 170 with 256 of 32; forward 109 and 114. */
 template <typename T, typename W>
 void dispatch(const NormArgs &p, hipStream_t s) {
   if (p.d <= 64 * 8) launch<T, W, 64, 8>(p, s);
   else if (p.d <= 64 * 16) launch<T, W, 64, 16>(p, s);
   else if (p.d <= 64 * 32) launch<T, W, 64, 32>(p, s);
   else if (p.d <= 256 * 16) launch<T, W, 256, 16>(p, s);
-  else if (p.d <= 256 * 32) launch<T, W, 256, 32>(p, s);
-  else if (p.d <= 512 * 32) launch<T, W, 512, 32>(p, s);
+  else if (p.d <= 512 * 16) launch<T, W, 512, 16>(p, s);
+  else if (p.d <= 1024 * 16) launch<T, W, 1024, 16>(p, s);
   else launch<T, W, 1024, 32>(p, s);
   if (p.dy && p.parts > 1 && (p.dweight || p.dbias)) {
     int64_t width = p.groups * p.d;
@@ -295,12 +305,13 @@ int run(const NormArgs &p, hipStream_t s) {
 
 extern "C" {
 
-/* How many workgroups share the rows: two a CU, and four rows in a row's
- * place each, so that up to four (or, of short rows, sixteen) rows need no
- * partial sums. */
+/* How many workgroups share the rows: one a CU, since each one's partial sums
+ * are written and read again (16384 x 8192 bf16: 165 us with 256, 181 with 512,
+ * 195 with 1024); four rows in a row's place each, so that up to four (or, of
+ * short rows, sixteen) rows need no partial sums. */
 int32_t vgpu_ops_norm_parts(int64_t rows, int64_t groups, int64_t d) {
   int64_t at_once = d <= 64 * 32 ? 4 : 1, share = 4 * at_once;
-  int64_t most = std::max<int64_t>(1, 512 / groups);
+  int64_t most = std::max<int64_t>(1, 256 / groups);
   return (int32_t)std::max<int64_t>(1, std::min((rows + share - 1) / share, most));
 }
 
