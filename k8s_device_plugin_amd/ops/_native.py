@@ -58,7 +58,8 @@ def library() -> ctypes.CDLL:
     lib.vgpu_ops_repack.argtypes = [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
                                     c_int64, c_int32, c_void_p]
     lib.vgpu_ops_gemm_plan.argtypes = [c_int64, c_int64, c_int64, c_int32, c_int32, c_int32,
-                                       c_int32, POINTER(c_int32), POINTER(c_int32)]
+                                       c_int32, POINTER(c_int32), POINTER(c_int32),
+                                       POINTER(c_int64)]
     lib.vgpu_ops_gemm_plan.restype = None
     lib.vgpu_ops_slope_parts.argtypes = [c_int64, c_int64, c_int32]
     lib.vgpu_ops_norm_parts.argtypes = [c_int64, c_int64, c_int64]

@@ -70,10 +70,10 @@ def formula(x, weight, bias, residual, activation):
 
 @lru_cache(maxsize=4096)
 def _plan(m, n, k, dtype, a_kc, b_kc, bare):
-    plan, splits = ctypes.c_int32(), ctypes.c_int32()
+    plan, splits, rows = ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int64()
     _native.library().vgpu_ops_gemm_plan(m, n, k, dtype, a_kc, b_kc, bare, ctypes.byref(plan),
-                                         ctypes.byref(splits))
-    return plan.value, splits.value
+                                         ctypes.byref(splits), ctypes.byref(rows))
+    return plan.value, splits.value, rows.value
 
 
 def _operand(t, any_axis=True):
@@ -108,13 +108,17 @@ def _gemm(a, b, out, bias=None, residual=None, act=0, z=None):
     dtype = DTYPES[out.dtype]
     # few rows are read with k contiguous, but for the short sums of a
     # weight's gradient
-    a, lda, a_kc, a_extent, ka = _operand(a, m > 64 or a.shape[1] <= 32)
+    a, lda, a_kc, a_extent, ka = _operand(a, m > 32 or a.shape[1] <= 32)
     b, ldb, b_kc, b_extent, kb = _operand(b)
     # a k that one side pads with zeros ends beyond the other's extent, which
     # reads as zeros there too
     k = max(ka, kb)
     bare = bias is None and residual is None and z is None and not act
-    plan, splits = _plan(m, n, k, dtype, a_kc, b_kc, bare)
+    plan, splits, rows = _plan(m, n, k, dtype, a_kc, b_kc, bare)
+    if rows < m:
+        _gemm(a[rows:], b, out[rows:], bias, None if residual is None else residual[rows:], act,
+              None if z is None else z[rows:])
+        m = rows
     work = (torch.empty(splits * m * n, dtype=torch.float32, device=out.device)
             if splits > 1 else None)
     launch("gemm", out.device, GemmArgs(

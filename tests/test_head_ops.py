@@ -197,7 +197,7 @@ def test_linear_long_sums_and_many_tiles(dtype):
     """Sizes that reach every tile, the split over k and its join."""
     gen = torch.Generator(device="cuda").manual_seed(0)
     for m, k, n in ((2, 25088, 256), (48, 8200, 520), (96, 6000, 96), (300, 4096, 260),
-                    (1030, 520, 2056), (4100, 72, 4104)):
+                    (1030, 520, 2056), (4100, 72, 4104), (4099, 2048, 4096), (519, 3000, 8200)):
         x = torch.randn(m, k, generator=gen, device="cuda").to(dtype)
         w = (torch.randn(n, k, generator=gen, device="cuda") * k ** -0.5).to(dtype)
         b = torch.randn(n, generator=gen, device="cuda").to(dtype)
