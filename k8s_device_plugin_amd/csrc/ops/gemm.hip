@@ -61,14 +61,16 @@ __device__ inline u32x4 load16(u32x4 from, uint32_t offset) {
 
 /* 16 bytes a lane straight to LDS, at `to` + 16 lane.  Written out because the
  * compiler, which cannot tell this buffer from the ones being read, would wait
- * for it before the next read of LDS; land_and_meet() does the waiting. */
+ * for it before the next read of LDS; land_and_meet() does the waiting.  It
+ * has no result.  m0 is no register that the compiler keeps values in: it
+ * writes it anew before each instruction of its own that reads it. */
 __device__ inline void load16_to_lds(u32x4 from, uint32_t offset, char *to) {
   uint32_t at = (uint32_t)(uintptr_t)(lds_void *)to;
   asm volatile(
       "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
       :
       : "s"(at), "v"(offset), "s"(from)
-      : "memory", "m0");
+      : "memory");
 }
 
 /* One operand's tile of R rows (of m or n) by STEPS steps of k in LDS, filled
@@ -375,7 +377,7 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_tile(GemmArgs p) {
   constexpr int ROWS = FIT >= WM ? WM : FIT >= WM / 2 ? WM / 2 : WM / 4;
   static_assert(ROWS % 16 == 0 && ROWS <= FIT, "whole fragments a pass");
   static_assert(64 % PIECES == 0, "a lane keeps its columns");
-  constexpr int DOWN = 64 / PIECES, U = ROWS / DOWN < 4 ? ROWS / DOWN : 4;
+  constexpr int DOWN = 64 / PIECES, U = ROWS / DOWN < 8 ? ROWS / DOWN : 8;
   float *mine = (float *)(lds + wave * PIECE_LDS);
   Epilogue<T> finish(p, blockIdx.y);
   int row = lane / PIECES, piece = lane % PIECES;
