@@ -40,6 +40,11 @@ struct Loose {
 };
 
 template <typename T>
+struct Loose4 { /* four of them */
+  typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+};
+
+template <typename T>
 __device__ inline void load_vec(const T *p, int n, float *out) {
   constexpr int V = Vec<T>::N;
   if (n >= V) {
@@ -107,13 +112,29 @@ __device__ inline float logistic(float z) {
 }
 
 /* y = act(z); the slope is dy/dz.  gelu is z Phi(z). */
-template <typename T>
-__device__ inline float activate(float z, int act) {
+template <typename T, int ACT>
+__device__ inline float activate(float z) {
   float e;
-  if (act == ACT_RELU) return z > 0.f || z != z ? z : 0.f;
-  if (act == ACT_GELU) return z * normal_cdf<T>(z, &e);
-  if (act == ACT_SILU) return z * logistic<T>(z);
+  if (ACT == ACT_RELU) return z > 0.f || z != z ? z : 0.f;
+  if (ACT == ACT_GELU) return z * normal_cdf<T>(z, &e);
+  if (ACT == ACT_SILU) return z * logistic<T>(z);
   return z;
+}
+
+/* Of a whole array, so that its elements' chains run beside each other. */
+template <typename T, int ACT, int N>
+__device__ inline void activate_each(f32x4 (&v)[N]) {
+#pragma unroll
+  for (int q = 0; q < N; q++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[q][e] = activate<T, ACT>(v[q][e]);
+}
+
+template <typename T, int N>
+__device__ inline void activate_all(f32x4 (&v)[N], int act) {
+  if (act == ACT_RELU) activate_each<T, ACT_RELU>(v);
+  else if (act == ACT_GELU) activate_each<T, ACT_GELU>(v);
+  else if (act == ACT_SILU) activate_each<T, ACT_SILU>(v);
 }
 
 template <typename T>

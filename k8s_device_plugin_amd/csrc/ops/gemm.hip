@@ -26,31 +26,61 @@ constexpr int PLAN_ROWS = 4, PLAN_OUTER = 5;
 template <typename T>
 struct Frag {
   typename Vec<T>::type v;
-  /* instructions that read one from LDS */
-  static constexpr int reads(bool kc) { return kc ? 1 : sizeof(T) == 4 ? 4 : 2; }
 };
 
-__device__ inline f32x4 mma(const Frag<bf16> &a, const Frag<bf16> &b, f32x4 c) {
+/* The matrix instructions of one pair of fragments: one, or four in fp32,
+ * where step j takes element j of every lane: both operands number k alike, so
+ * the order in which k is summed is free. */
+template <typename T>
+constexpr int PARTS = sizeof(T) == 4 ? 4 : 1;
+
+__device__ inline f32x4 mma(const Frag<bf16> &a, const Frag<bf16> &b, f32x4 c, int) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
 }
-__device__ inline f32x4 mma(const Frag<fp16> &a, const Frag<fp16> &b, f32x4 c) {
+__device__ inline f32x4 mma(const Frag<fp16> &a, const Frag<fp16> &b, f32x4 c, int) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.v, b.v, c, 0, 0, 0);
 }
-/* Step j takes element j of every lane: both operands number k alike, so the
- * order in which k is summed is free. */
-__device__ inline f32x4 mma(const Frag<float> &a, const Frag<float> &b, f32x4 c) {
+__device__ inline f32x4 mma(const Frag<float> &a, const Frag<float> &b, f32x4 c, int j) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
+}
+
+/* The same with the sum held in the accumulation registers for good.  Where
+ * all 256 of them are sums the compiler would move some back and forth in
+ * every step.  It cannot see what these write: the caller keeps other products
+ * between two into the same sum, and waits (settle) before it reads one. */
+__device__ inline void mma_pinned(const Frag<bf16> &a, const Frag<bf16> &b, f32x4 &c, int) {
+  asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a.v), "v"(b.v));
+}
+__device__ inline void mma_pinned(const Frag<fp16> &a, const Frag<fp16> &b, f32x4 &c, int) {
+  asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a.v), "v"(b.v));
+}
+__device__ inline void mma_pinned(const Frag<float> &a, const Frag<float> &b, f32x4 &c, int j) {
+  float x = a.v[j], y = b.v[j];
+  asm volatile("v_mfma_f32_16x16x4_f32 %0, %1, %2, %0" : "+a"(c) : "v"(x), "v"(y));
+}
+/* Between other writes or reads of pinned sums and the products: 32 wait
+ * states, more than the longest of these takes to write its sum.  The empty
+ * statements keep the compiler's own moves on their side of it. */
+template <int M, int N>
+__device__ inline void settle(f32x4 (&c)[M][N]) {
+  auto hold = [&] {
 #pragma unroll
-  for (int j = 0; j < 4; j++)
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
-  return c;
+    for (int i = 0; i < M; i++)
+#pragma unroll
+      for (int j = 0; j < N; j++) asm volatile("" : "+a"(c[i][j]));
+  };
+  hold();
+  asm volatile("s_nop 15\n\ts_nop 15");
+  hold();
 }
 
 /* A window on memory of which nothing past `extent` bytes is read: a buffer's
  * descriptor (base, no stride, size in bytes, raw 32-bit data). */
 __device__ inline u32x4 window(const void *base, int64_t extent) {
   uintptr_t at = (uintptr_t)base;
-  return u32x4{(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu,
-               (uint32_t)min(max(extent, (int64_t)0), (int64_t)0x7ffffff0), 0x00020000u};
+  auto same = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+  return u32x4{same((uint32_t)at), same((uint32_t)(at >> 32) & 0xffffu),
+               same((uint32_t)min(max(extent, (int64_t)0), (int64_t)0x7ffffff0)), 0x00020000u};
 }
 
 __device__ inline u32x4 load16(u32x4 from, uint32_t offset) {
@@ -59,18 +89,18 @@ __device__ inline u32x4 load16(u32x4 from, uint32_t offset) {
   return __builtin_amdgcn_raw_buffer_load_b128(rsrc, offset, 0, 0);
 }
 
-/* 16 bytes a lane straight to LDS, at `to` + 16 lane.  Written out because the
- * compiler, which cannot tell this buffer from the ones being read, would wait
- * for it before the next read of LDS; land_and_meet() does the waiting.  It
- * has no result.  m0 is no register that the compiler keeps values in: it
- * writes it anew before each instruction of its own that reads it. */
-__device__ inline void load16_to_lds(u32x4 from, uint32_t offset, char *to) {
-  uint32_t at = (uint32_t)(uintptr_t)(lds_void *)to;
+/* 16 bytes a lane straight to LDS, at `to` + SKIP + 16 lane.  Written out
+ * because the compiler, which cannot tell this buffer from the ones being read,
+ * would wait for it before the next read of LDS; land_and_meet() does the
+ * waiting.  It has no result.  m0 is no register that the compiler keeps values
+ * in: it writes it anew before each instruction of its own that reads it. */
+template <int SKIP>
+__device__ inline void load16_to_lds(u32x4 from, uint32_t offset, uint32_t to) {
   asm volatile(
-      "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+      "s_add_u32 m0, %0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
       :
-      : "s"(at), "v"(offset), "s"(from)
-      : "memory");
+      : "s"(to), "v"(offset), "s"(from), "n"(SKIP)
+      : "memory", "scc");
 }
 
 /* One operand's tile of R rows (of m or n) by STEPS steps of k in LDS, filled
@@ -92,13 +122,11 @@ struct Tile {
   static constexpr int ROW_CHUNKS = KC ? STAGE / 16 : R / E;
   static_assert(LOADS * THREADS * 16 == BYTES, "whole loads");
   static_assert((ROW_CHUNKS & (ROW_CHUNKS - 1)) == 0, "the xor stays in the row");
-  /* A thread's chunks lie ROWS rows apart.  The xor repeats every 16 rows, so
-   * but for WAYS of them their offsets differ by whole rows alone. */
-  static constexpr int ROWS = THREADS / ROW_CHUNKS;
-  static constexpr int WAYS = ROWS >= 16 ? 1 : 16 / ROWS;
-  static_assert(LOADS % WAYS == 0 || LOADS < WAYS, "rows alike");
-  uint32_t off[WAYS], stride; /* bytes */
-  int kpos;                   /* first k of the thread's first chunk */
+  static constexpr int ROWS = THREADS / ROW_CHUNKS; /* between a thread's chunks */
+  uint32_t off[LOADS];                              /* bytes */
+  int kpos; /* k contiguous: first k of the thread's chunks, which the xor,
+               repeating every 16 rows, leaves alike */
+  static_assert(!KC || ROWS % 16 == 0, "chunks alike");
 
   static __device__ int spread(int row) {
     int x;
@@ -109,24 +137,20 @@ struct Tile {
   }
 
   __device__ void init(int64_t ld, int tid) {
-    int r = tid / ROW_CHUNKS;
-    stride = (uint32_t)(ld * sizeof(T));
-    kpos = KC ? ((tid % ROW_CHUNKS) ^ spread(r)) * E : r;
+    int r = tid / ROW_CHUNKS, c = tid % ROW_CHUNKS;
+    kpos = (c ^ spread(r)) * E;
 #pragma unroll
-    for (int w = 0; w < WAYS; w++)
-      off[w] = (r + w * ROWS) * stride + ((tid % ROW_CHUNKS) ^ spread(r + w * ROWS)) * 16;
+    for (int i = 0; i < LOADS; i++)
+      off[i] = (r + i * ROWS) * (uint32_t)(ld * sizeof(T)) + (c ^ spread(r + i * ROWS)) * 16;
   }
 
-  /* One of a stage's loads.  Chunks past the end of k come as zeros, and so
-   * does what lies past the operand's end.  Rows past m or n only feed results
-   * that are not stored. */
-  __device__ void load(int i, u32x4 from, int k_left, char *lds, int wave) const {
-    uint32_t skip = i / WAYS * WAYS * ROWS * stride;
-    /* added anew every time: kept, the sums would cost a register a load */
-    asm volatile("" : "+s"(skip));
-    bool in = kpos < (KC ? k_left : k_left - i * ROWS);
-    uint32_t o = (in ? off[i % WAYS] : OUT_OF_RANGE) + skip;
-    load16_to_lds(from, o, lds + (i * THREADS + wave * 64) * 16);
+  /* One of a stage's loads.  What lies past the operand's end comes as zeros:
+   * with k strided that is all past the end of k, with k contiguous chunks
+   * past it are asked for there.  Rows past m or n only feed results that are
+   * not stored. */
+  template <int I>
+  __device__ void load(u32x4 from, int k_left, uint32_t lds) const {
+    load16_to_lds<I * THREADS * 16>(from, !KC || kpos < k_left ? off[I] : OUT_OF_RANGE, lds);
   }
 
   /* The fragment of rows row0 .. row0+15 at one of the stage's steps. */
@@ -158,80 +182,80 @@ struct Tile {
   }
 };
 
-/* Finishes COUNT rows of the same four neighbouring columns, `step` rows
- * apart: bias, activation, residual, store, or the partial sums of a split.
- * All that is read is asked for before any of it is used.  Accesses of four
- * need no alignment beyond the element's. */
+/* Finishes rows of four neighbouring columns: bias, activation, residual,
+ * store, or the partial sums of a split.  Accesses of four need no alignment
+ * beyond the element's. */
 template <typename T>
 struct Epilogue {
-  typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  template <typename D>
+  using Four = typename Loose4<D>::type;
   const GemmArgs &p;
   float *part; /* of this split, or null */
 
   __device__ Epilogue(const GemmArgs &args, int split = 0)
       : p(args), part(args.splits > 1 ? args.work + (int64_t)split * args.m * args.n : nullptr) {}
 
+  /* COUNT rows, `step` apart, all there and four columns wide: everything is
+   * asked for before anything is used. */
   template <int COUNT>
-  __device__ void operator()(int64_t m, int step, int64_t col, f32x4 (&v)[COUNT]) const {
-    int width = (int)min((int64_t)4, p.n - col);
-    if (width <= 0) return;
+  __device__ void rows(int64_t m, int step, int64_t col, f32x4 (&v)[COUNT]) const {
     if (part) {
 #pragma unroll
       for (int q = 0; q < COUNT; q++)
-        if (m + q * step < p.m) put(part + (m + q * step) * p.n + col, width, v[q]);
+        *(Four<float> *)(part + (m + q * step) * p.n + col) = v[q];
       return;
     }
-    f32x4 res[COUNT];
+    Four<T> res[COUNT], bias;
     if (p.res)
 #pragma unroll
       for (int q = 0; q < COUNT; q++)
-        if (m + q * step < p.m)
-          res[q] = get((const T *)p.res + (m + q * step) * p.ldr + col, width);
-    if (p.bias) {
-      f32x4 b = get((const T *)p.bias + col, width);
+        res[q] = *(const Four<T> *)((const T *)p.res + (m + q * step) * p.ldr + col);
+    if (p.bias) bias = *(const Four<T> *)((const T *)p.bias + col);
+    if (p.bias)
 #pragma unroll
-      for (int q = 0; q < COUNT; q++) v[q] += b;
-    }
+      for (int q = 0; q < COUNT; q++) v[q] += wide(bias);
     if (p.z)
 #pragma unroll
       for (int q = 0; q < COUNT; q++)
-        if (m + q * step < p.m) put((T *)p.z + (m + q * step) * p.ldz + col, width, v[q]);
-    if (p.act != ACT_NONE)
-#pragma unroll
-      for (int q = 0; q < COUNT; q++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[q][e] = activate<T>(v[q][e], p.act);
+        *(Four<T> *)((T *)p.z + (m + q * step) * p.ldz + col) = narrow(v[q]);
+    activate_all<T>(v, p.act);
     if (p.res)
 #pragma unroll
-      for (int q = 0; q < COUNT; q++) v[q] += res[q];
+      for (int q = 0; q < COUNT; q++) v[q] += wide(res[q]);
 #pragma unroll
     for (int q = 0; q < COUNT; q++)
-      if (m + q * step < p.m) put((T *)p.y + (m + q * step) * p.ldy + col, width, v[q]);
+      *(Four<T> *)((T *)p.y + (m + q * step) * p.ldy + col) = narrow(v[q]);
   }
 
-  static __device__ f32x4 get(const T *at, int width) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (width == 4) {
-      four t = *(const four *)at;
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = to_f<T>(t[e]);
-    } else {
-      for (int e = 0; e < width; e++) v[e] = to_f<T>(at[e]);
+  /* What there is of one row's four. */
+  __device__ void one(int64_t m, int64_t col, f32x4 v) const {
+    if (m >= p.m) return;
+    if (col + 4 <= p.n) {
+      f32x4 row[1] = {v};
+      rows(m, 0, col, row);
+      return;
     }
-    return v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (col + e >= p.n) return;
+      if (part) {
+        part[m * p.n + col + e] = v[e];
+        continue;
+      }
+      f32x4 u[1] = {{v[e], 0.f, 0.f, 0.f}};
+      if (p.bias) u[0][0] += to_f<T>(((const T *)p.bias)[col + e]);
+      if (p.z) ((T *)p.z)[m * p.ldz + col + e] = from_f<T>(u[0][0]);
+      activate_all<T>(u, p.act);
+      if (p.res) u[0][0] += to_f<T>(((const T *)p.res)[m * p.ldr + col + e]);
+      ((T *)p.y)[m * p.ldy + col + e] = from_f<T>(u[0][0]);
+    }
   }
 
-  template <typename D>
-  static __device__ void put(D *at, int width, f32x4 v) {
-    typedef D quad __attribute__((ext_vector_type(4), aligned(sizeof(D))));
-    if (width == 4) {
-      quad t;
-#pragma unroll
-      for (int e = 0; e < 4; e++) t[e] = from_f<D>(v[e]);
-      *(quad *)at = t;
-    } else {
-      for (int e = 0; e < width; e++) at[e] = from_f<D>(v[e]);
-    }
+  static __device__ f32x4 wide(Four<T> t) {
+    return f32x4{to_f<T>(t[0]), to_f<T>(t[1]), to_f<T>(t[2]), to_f<T>(t[3])};
+  }
+  static __device__ Four<T> narrow(f32x4 v) {
+    return Four<T>{from_f<T>(v[0]), from_f<T>(v[1]), from_f<T>(v[2]), from_f<T>(v[3])};
   }
 };
 
@@ -246,6 +270,15 @@ __device__ inline void tile_of(int block, int blocks, int tiles_m, int tiles_n, 
   int in = t - first * tiles_n;
   *tm = first + in % height;
   *tn = in / height;
+}
+
+/* f(0), f(1), ... with constants. */
+template <int N, int I = 0, typename F>
+__device__ inline void each(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    each<N, I + 1>(f);
+  }
 }
 
 /* Waits until at most N of the wave's loads to LDS are in flight and its LDS
@@ -270,6 +303,7 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_tile(GemmArgs p) {
   using TA = Tile<T, AKC, TM, THREADS>;
   using TB = Tile<T, BKC, TN, THREADS>;
   constexpr int LOADS = TA::LOADS + TB::LOADS, BYTES = TA::BYTES + TB::BYTES;
+  constexpr bool PINNED = FM * FN == 64; /* a wave's sums fill 256 registers */
   __shared__ __attribute__((aligned(1024))) char lds[BUFFERS * BYTES];
 
   int tid = threadIdx.x, lane = tid & 63;
@@ -286,8 +320,8 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_tile(GemmArgs p) {
   TB tb;
   ta.init(p.lda, tid);
   tb.init(p.ldb, tid);
-  /* past this part's last stage the loads bring zeros, so that their number
-   * stays the same */
+  /* past this part's last stage the loads bring zeros from empty windows, so
+   * that their number stays the same */
   struct Source {
     u32x4 a, b;
     int left;
@@ -296,13 +330,17 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_tile(GemmArgs p) {
     int64_t k = (int64_t)s * BK;
     int64_t oa = (AKC ? m0 * p.lda + k : k * p.lda + m0) * (int64_t)sizeof(T);
     int64_t ob = (BKC ? n0 * p.ldb + k : k * p.ldb + n0) * (int64_t)sizeof(T);
-    return Source{window((const char *)p.a + oa, p.a_extent - oa),
-                  window((const char *)p.b + ob, p.b_extent - ob),
-                  s < s1 ? (int)min(p.k - k, (int64_t)BK) : 0};
+    bool some = s < s1;
+    return Source{window((const char *)p.a + oa, some ? p.a_extent - oa : 0),
+                  window((const char *)p.b + ob, some ? p.b_extent - ob : 0),
+                  (int)min(p.k - k, (int64_t)BK)};
   };
-  auto load = [&](int i, const Source &q, char *at) {
-    if (i < TA::LOADS) ta.load(i, q.a, q.left, at, wave);
-    else tb.load(i - TA::LOADS, q.b, q.left, at + TA::BYTES, wave);
+  uint32_t lds_at = (uint32_t)(uintptr_t)(lds_void *)lds;
+  auto load = [&](auto i, const Source &q, int buffer) {
+    constexpr int I = decltype(i)::value;
+    uint32_t at = lds_at + buffer * BYTES + wave * 1024;
+    if constexpr (I < TA::LOADS) ta.template load<I>(q.a, q.left, at);
+    else tb.template load<I - TA::LOADS>(q.b, q.left, at + TA::BYTES);
   };
 
   f32x4 acc[FM][FN] = {};
@@ -314,58 +352,57 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_tile(GemmArgs p) {
     if (f < FN) h.b[f] = TB::frag(at + TA::BYTES, wn + f * 16, step, lane);
     else h.a[f - FN] = TA::frag(at, wm + (f - FN) * 16, step, lane);
   };
-  auto multiply = [&](const Step &h) {
-#pragma unroll
-    for (int i = 0; i < FM; i++)
-#pragma unroll
-      for (int j = 0; j < FN; j++) acc[i][j] = mma(h.b[j], h.a[i], acc[i][j]);
+  /* Product number q of a step; those into one sum lie FM FN apart. */
+  auto multiply = [&](const Step &h, int q) {
+    int part = q / (FM * FN), i = q / FN % FM, j = q % FN;
+    if constexpr (PINNED) mma_pinned(h.b[j], h.a[i], acc[i][j], part);
+    else acc[i][j] = mma(h.b[j], h.a[i], acc[i][j], part);
   };
-  /* Deals a step's reads, and the loads that stand between them, out between
-   * its products: in a row they would hold up the matrix cores of all waves. */
-  constexpr int FRAGS = FM + FN;
-  constexpr int PRODUCTS = FM * FN * (sizeof(T) == 4 ? 4 : 1);
-  constexpr int EACH = PRODUCTS / FRAGS > 0 ? PRODUCTS / FRAGS : 1;
-  auto deal = [] {
-#pragma unroll
-    for (int f = 0; f < FRAGS; f++) {
-      if (f < FN) __builtin_amdgcn_sched_group_barrier(0x100, Frag<T>::reads(BKC), 0);
-      else __builtin_amdgcn_sched_group_barrier(0x100, Frag<T>::reads(AKC), 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
-    }
+  /* A step's products, with the reads of the next one and the loads dealt out
+   * between them: in a row they would hold up the matrix cores of all waves. */
+  constexpr int FRAGS = FM + FN, PRODUCTS = FM * FN * PARTS<T>;
+  constexpr int TURNS = FRAGS > LOADS ? FRAGS : LOADS;
+  auto step = [&](const Step &now, Step &then, const char *from, int which, const Source *q,
+                  int to) {
     __builtin_amdgcn_sched_barrier(0);
+    each<TURNS>([&](auto turn) {
+      constexpr int F = decltype(turn)::value, P0 = PRODUCTS * F / TURNS,
+                    P1 = PRODUCTS * (F + 1) / TURNS;
+      if (F < FRAGS) read(F, then, from, which);
+#pragma unroll
+      for (int m = P0; m < P1; m++) {
+        if constexpr (F < LOADS)
+          if (q && m == P0 + (P1 - P0) / 2) load(turn, *q, to);
+        multiply(now, m);
+      }
+      if constexpr (P0 == P1 && F < LOADS)
+        if (q) load(turn, *q, to);
+      __builtin_amdgcn_sched_barrier(0);
+    });
   };
   int buffer = 0;
   /* the stage whose first step is in `now`; leaves the next one's there */
   auto stage = [&](int s, Step &now, Step &then) {
-    char *at = lds + buffer * BYTES;
+    int at = buffer;
     buffer = buffer + 1 == BUFFERS ? 0 : buffer + 1;
-    char *ahead = lds + buffer * BYTES;
     Source q = source(s + BUFFERS);
-#pragma unroll
-    for (int f = 0; f < FRAGS; f++) read(f, then, at, 1);
-    multiply(now);
-    deal();
+    step(now, then, lds + at * BYTES, 1, nullptr, 0);
     land_and_meet<(BUFFERS - 2) * LOADS>();
-#pragma unroll
-    for (int f = 0; f < (FRAGS > LOADS ? FRAGS : LOADS); f++) {
-      if (f < FRAGS) read(f, now, ahead, 0);
-      if (f < LOADS) load(f, q, at);
-    }
-    multiply(then);
-    deal();
+    step(then, now, lds + buffer * BYTES, 0, &q, at);
   };
 
 #pragma unroll
   for (int i = 0; i < BUFFERS; i++) {
     Source q = source(s0 + i);
-#pragma unroll
-    for (int f = 0; f < LOADS; f++) load(f, q, lds + i * BYTES);
+    each<LOADS>([&](auto f) { load(f, q, i); });
   }
   land_and_meet<(BUFFERS - 1) * LOADS>();
 #pragma unroll
   for (int f = 0; f < FRAGS; f++) read(f, even, lds, 0);
+  if constexpr (PINNED) settle(acc);
   for (int s = s0; s < s1; s++) stage(s, even, odd);
   land_and_meet<0>();
+  if constexpr (PINNED) settle(acc);
 
   /* b is the first operand of the product, so a lane holds 4 neighbouring
    * columns of row lane%16.  Each wave turns its part through its own piece
@@ -390,14 +427,21 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_tile(GemmArgs p) {
         int r = i * 16 + (lane & 15), c = (j * 4 + (lane >> 4)) ^ (r & (PIECES - 1));
         *(f32x4 *)(mine + r * WN + c * 4) = acc[pass * (ROWS / 16) + i][j];
       }
+    auto at = [&](int r) {
+      return *(const f32x4 *)(mine + r * WN + (piece ^ (r & (PIECES - 1))) * 4);
+    };
+    int64_t m = m0 + wm + pass * ROWS, n = n0 + wn + piece * 4;
+    if (m + ROWS <= p.m && n0 + wn + WN <= p.n) {
 #pragma unroll 1
-    for (int r = row; r < ROWS; r += DOWN * U) {
-      f32x4 v[U];
+      for (int r = row; r < ROWS; r += DOWN * U) {
+        f32x4 v[U];
 #pragma unroll
-      for (int u = 0; u < U; u++)
-        v[u] = *(const f32x4 *)(mine + (r + u * DOWN) * WN +
-                                (piece ^ ((r + u * DOWN) & (PIECES - 1))) * 4);
-      finish(m0 + wm + pass * ROWS + r, DOWN, n0 + wn + piece * 4, v);
+        for (int u = 0; u < U; u++) v[u] = at(r + u * DOWN);
+        finish.rows(m + r, DOWN, n, v);
+      }
+    } else {
+#pragma unroll 1
+      for (int r = row; r < ROWS; r += DOWN) finish.one(m + r, n, at(r));
     }
   }
 }
@@ -409,7 +453,7 @@ __global__ __launch_bounds__(256) void gemm_join(GemmArgs p) {
   int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= p.m * fours) return;
   int64_t m = at / fours, n = at % fours * 4;
-  f32x4 sum[1] = {{0.f, 0.f, 0.f, 0.f}}, &v = sum[0];
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
   const float *q = p.work + m * p.n + n;
   if (n + 4 <= p.n && p.n % 4 == 0) {
     for (int s = 0; s < p.splits; s++) v += *(const f32x4 *)(q + (int64_t)s * p.m * p.n);
@@ -421,7 +465,7 @@ __global__ __launch_bounds__(256) void gemm_join(GemmArgs p) {
   }
   p.splits = 1;
   Epilogue<T> finish(p);
-  finish(m, 0, n, sum);
+  finish.one(m, n, v);
 }
 
 /* Few rows (m <= 32): b is read once, at the memory's rate, straight into the
@@ -500,7 +544,9 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
       Frag<T> fa;
       fa.v = __builtin_bit_cast(vec, q.a[f]);
 #pragma unroll
-      for (int j = 0; j < FN; j++) acc[f][j] = mma(fb[j], fa, acc[f][j]);
+      for (int j = 0; j < FN; j++)
+#pragma unroll
+        for (int e = 0; e < PARTS<T>; e++) acc[f][j] = mma(fb[j], fa, acc[f][j], e);
     }
   };
   Step even[C], odd[C];
@@ -537,10 +583,10 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
       int r = q / (STRIP / 4), c = q % (STRIP / 4);
       int64_t m = f * 16 + r, n = n0 + c * 4;
       if (m >= p.m || n >= p.n) continue;
-      f32x4 v[1] = {lds[0][r][c]};
+      f32x4 v = lds[0][r][c];
 #pragma unroll
-      for (int w = 1; w < WAVES; w++) v[0] += lds[w][r][c];
-      finish(m, 0, n, v);
+      for (int w = 1; w < WAVES; w++) v += lds[w][r][c];
+      finish.one(m, n, v);
     }
   }
 }
@@ -596,7 +642,7 @@ void launch_tile(const GemmArgs &p, hipStream_t stream) {
     return dim3((unsigned)(((p.m + tm - 1) / tm) * ((p.n + tn - 1) / tn)), (unsigned)p.splits);
   };
   if (p.plan == 0)
-    gemm_tile<T, AKC, BKC, 256, 256, 2, 4, 2><<<blocks(256, 256), 512, 0, stream>>>(p);
+    gemm_tile<T, AKC, BKC, 256, 256, 2, 2, 2><<<blocks(256, 256), 256, 0, stream>>>(p);
   else if (p.plan == 1)
     gemm_tile<T, AKC, BKC, 128, 128, 2, 2, 2><<<blocks(128, 128), 256, 0, stream>>>(p);
   else if (p.plan == 2)
