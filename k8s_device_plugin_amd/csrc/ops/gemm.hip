@@ -296,7 +296,7 @@ __device__ inline void land_and_meet() {
  * stage says both that the next stage has landed and that this one has been
  * read, and its buffer is filled again at once. */
 template <typename T, bool AKC, bool BKC, int TM, int TN, int WR, int WC, int BUFFERS>
-__global__ __launch_bounds__(WR *WC * 64) void gemm_tile(GemmArgs p) {
+__global__ __launch_bounds__(WR *WC * 64, TM == 256 ? 1 : 2) void gemm_tile(GemmArgs p) {
   constexpr int THREADS = WR * WC * 64;
   constexpr int BK = STEPS * STEP_BYTES / sizeof(T);
   constexpr int FM = TM / WR / 16, FN = TN / WC / 16;
@@ -352,9 +352,10 @@ __global__ __launch_bounds__(WR *WC * 64) void gemm_tile(GemmArgs p) {
     if (f < FN) h.b[f] = TB::frag(at + TA::BYTES, wn + f * 16, step, lane);
     else h.a[f - FN] = TA::frag(at, wm + (f - FN) * 16, step, lane);
   };
-  /* Product number q of a step; those into one sum lie FM FN apart. */
+  /* Product number q of a step, by rows, so that the last fragments are not
+   * needed at once; between two into one sum lie FN - 1 others at least. */
   auto multiply = [&](const Step &h, int q) {
-    int part = q / (FM * FN), i = q / FN % FM, j = q % FN;
+    int i = q / (FN * PARTS<T>), part = q / FN % PARTS<T>, j = q % FN;
     if constexpr (PINNED) mma_pinned(h.b[j], h.a[i], acc[i][j], part);
     else acc[i][j] = mma(h.b[j], h.a[i], acc[i][j], part);
   };
@@ -740,16 +741,16 @@ int run_slope(const SlopeArgs &p, hipStream_t s) {
  * stage and so much for itself.  A split writes and reads partial sums and
  * costs a launch.  The numbers are a least-squares fit to 2700 timings (m 40 to
  * 8192, n 1000 to 11000, k 1024 to 14336, all layouts); what it picks takes
- * 2% more than the best of them on average in 16 bits, 0.4% in fp32. */
+ * 3.3% more than the best of them on average in 16 bits, 0.2% in fp32. */
 double tile_time(int plan, int64_t splits, int64_t m, int64_t n, int64_t k, int size) {
   struct Cost {
     double stage, own; /* us */
   };
   static const int side[4][2] = {{256, 256}, {128, 128}, {64, 128}, {32, 128}};
-  static const Cost full[2][4] = {{{1.31, 7.9}, {0.96, 5.3}, {0.63, 4.6}, {0.43, 4.5}},
-                                  {{7.40, 4.9}, {3.74, 3.4}, {1.98, 2.7}, {1.10, 2.5}}};
-  static const Cost half[2][4] = {{{1.31, 7.9}, {0.67, 4.9}, {0.47, 3.8}, {0.36, 2.8}},
-                                  {{7.40, 4.9}, {2.03, 3.2}, {1.12, 1.8}, {0.71, 0.1}}};
+  static const Cost full[2][4] = {{{1.33, 7.9}, {0.86, 5.0}, {0.595, 3.7}, {0.417, 4.2}},
+                                  {{7.37, 5.9}, {3.71, 3.3}, {1.975, 2.3}, {1.096, 2.4}}};
+  static const Cost half[2][4] = {{{1.33, 7.9}, {0.56, 3.7}, {0.378, 3.1}, {0.321, 2.6}},
+                                  {{7.37, 5.9}, {1.99, 3.1}, {1.110, 1.2}, {0.657, 0.0}}};
   int64_t tiles = ((m + side[plan][0] - 1) / side[plan][0]) * ((n + side[plan][1] - 1) / side[plan][1]);
   int64_t stages = (k * size + STEPS * STEP_BYTES - 1) / (STEPS * STEP_BYTES);
   int64_t each = (stages + splits - 1) / splits, slots = plan == 0 ? 256 : 512;
@@ -758,7 +759,7 @@ double tile_time(int plan, int64_t splits, int64_t m, int64_t n, int64_t k, int 
   double time = turns * (each * f.stage + f.own);
   if (rest > 256) time += each * f.stage + f.own;
   else if (rest) time += each * h.stage + h.own;
-  if (splits > 1) time += 6. + m * n * splits * 0.9e-6;
+  if (splits > 1) time += (size == 4 ? 9. : 5.8) + m * n * splits * 0.9e-6;
   return time;
 }
 
