@@ -18,7 +18,7 @@ enum DType { DT_F32 = 0, DT_BF16 = 1, DT_FP16 = 2 };
 enum Act { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_SILU = 3 };
 
 /* What the entry points return beside HIP's own codes (which are >= 0). */
-enum { OPS_BAD_ARG = -1 };
+enum { OPS_BAD_ARG = -1, OPS_TOO_LONG = -2 };
 
 template <typename T>
 struct Vec { /* 16 bytes of T */
@@ -151,6 +151,13 @@ __device__ inline float slope(float z, int act) {
   return 1.f;
 }
 
+/* The kernels that a product may run on: tiles of 256 x 256, 128 x 128,
+ * 64 x 128 or 32 x 128 of y; few rows; a sum of at most OUTER_K terms. */
+enum { PLAN_TILES = 4, PLAN_ROWS = 4, PLAN_OUTER = 5 };
+constexpr int OUTER_K = 32, OUTER_ROWS = 8;
+constexpr int STEP_BYTES = 64; /* of k per row: what one fragment covers */
+constexpr int STEPS = 2;       /* a stage: whole lines of 128 bytes */
+
 /* y[m,n] = act(sum_k a[m,k] b[n,k] + bias[n]) + res[m,n].
  * a_kc: a's element (m,k) is at a[m*lda + k]; otherwise at a[k*lda + m].
  * Likewise b.  Extents are the bytes that may be read from a and b on. */
@@ -177,6 +184,22 @@ struct SlopeArgs {
   float *part;
   int64_t lddy, ldz, lddz, m, n;
   int32_t dtype, act, parts;
+};
+
+int launch_gemm(const GemmArgs &p, hipStream_t s);
+int launch_slope(const SlopeArgs &p, hipStream_t s);
+int launch_repack(const void *src, int64_t rs, int64_t cs, int64_t rows, int64_t cols, void *dst,
+                  int64_t ld, int size, hipStream_t s);
+
+/* y = act(x W^T + bias) + res, x [m,k] and W [n,k] of any strides (in
+ * elements), y and z [m,n] contiguous.  With dy, the backward pass instead: z
+ * is then what the slope is taken at, and dx [m,k], dw [n,k], db [n] what is
+ * written of the gradients, contiguous. */
+struct LinearArgs {
+  const void *x, *w, *bias, *res, *dy;
+  void *y, *z, *dx, *dw, *db, *work;
+  int64_t m, n, k, xs0, xs1, ws0, ws1, ldr, lddy, work_bytes;
+  int32_t dtype, act;
 };
 
 /* Layer norm of each (row, group): x [rows, groups*d].  mean and rstd hold

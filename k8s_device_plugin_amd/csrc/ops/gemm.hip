@@ -16,10 +16,6 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 namespace {
 
 constexpr uint32_t OUT_OF_RANGE = 0x80000000u; /* past any num_records below */
-constexpr int STEP_BYTES = 64; /* of k per row: what one fragment covers */
-constexpr int STEPS = 2;       /* a stage: whole lines of 128 bytes */
-/* 0 to 3: tiles of 256 x 256, 128 x 128, 64 x 128, 32 x 128 */
-constexpr int PLAN_ROWS = 4, PLAN_OUTER = 5;
 
 /* A fragment is what one lane gives one 64-byte step of k: 16 bytes.  Lane l
  * holds row l%16 and, of the step's k, the (l/16)-th quarter. */
@@ -595,7 +591,6 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
 /* A short sum (k <= 32) with k strided on both sides, as a weight's gradient
  * from few rows is: bound by writing y.  A wave holds 8 rows by 64 vectors of
  * columns; a's values are the same for the whole wave. */
-constexpr int OUTER_K = 32, OUTER_ROWS = 8;
 
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_outer(GemmArgs p) {
@@ -673,13 +668,14 @@ int run(const GemmArgs &p, hipStream_t stream) {
   return OPS_LAUNCHED();
 }
 
-/* [rows, cols] of any strides to rows of `ld` elements, zeros behind. */
+/* The bits of [rows, cols] of any strides to rows of `ld` elements, zeros
+ * behind. */
 template <typename T>
 __global__ __launch_bounds__(256) void repack(const T *src, int64_t rs, int64_t cs, int64_t rows,
                                               int64_t cols, T *dst, int64_t ld) {
   for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
     for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < ld; c += (int64_t)gridDim.x * 256)
-      dst[r * ld + c] = c < cols ? src[r * rs + c * cs] : (T)0;
+      dst[r * ld + c] = c < cols ? src[r * rs + c * cs] : T(0);
 }
 
 /* A workgroup's four waves share 64 vectors of columns; wave w takes rows w,
@@ -735,144 +731,27 @@ int run_slope(const SlopeArgs &p, hipStream_t s) {
   return OPS_LAUNCHED();
 }
 
-/* What a product takes in us with tiles of one kind, k in `splits` parts: in
- * turns of as many workgroups as the card holds (256 of the largest tile, 512
- * of the others; a last turn of up to 256 has a CU each), each of so much a
- * stage and so much for itself.  A split writes and reads partial sums and
- * costs a launch.  The numbers are a least-squares fit to 2700 timings (m 40 to
- * 8192, n 1000 to 11000, k 1024 to 14336, all layouts); what it picks takes
- * 3.3% more than the best of them on average in 16 bits, 0.2% in fp32. */
-double tile_time(int plan, int64_t splits, int64_t m, int64_t n, int64_t k, int size) {
-  struct Cost {
-    double stage, own; /* us */
-  };
-  static const int side[4][2] = {{256, 256}, {128, 128}, {64, 128}, {32, 128}};
-  static const Cost full[2][4] = {{{1.33, 7.9}, {0.86, 5.0}, {0.595, 3.7}, {0.417, 4.2}},
-                                  {{7.37, 5.9}, {3.71, 3.3}, {1.975, 2.3}, {1.096, 2.4}}};
-  static const Cost half[2][4] = {{{1.33, 7.9}, {0.56, 3.7}, {0.378, 3.1}, {0.321, 2.6}},
-                                  {{7.37, 5.9}, {1.99, 3.1}, {1.110, 1.2}, {0.657, 0.0}}};
-  int64_t tiles = ((m + side[plan][0] - 1) / side[plan][0]) * ((n + side[plan][1] - 1) / side[plan][1]);
-  int64_t stages = (k * size + STEPS * STEP_BYTES - 1) / (STEPS * STEP_BYTES);
-  int64_t each = (stages + splits - 1) / splits, slots = plan == 0 ? 256 : 512;
-  int64_t turns = tiles * splits / slots, rest = tiles * splits % slots;
-  const Cost &f = full[size == 4][plan], &h = half[size == 4][plan];
-  double time = turns * (each * f.stage + f.own);
-  if (rest > 256) time += each * f.stage + f.own;
-  else if (rest) time += each * h.stage + h.own;
-  if (splits > 1) time += (size == 4 ? 9. : 5.8) + m * n * splits * 0.9e-6;
-  return time;
-}
-
-double best_tiles(int64_t m, int64_t n, int64_t k, int size, int32_t *plan, int32_t *splits) {
-  static const int parts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
-  double best = 1e30;
-  for (int q = 0; q < 4; q++)
-    for (int s : parts) {
-      /* partial sums of no more than 1.5 GB */
-      if (s > 1 && ((double)m * n * s * 4 > 1.5e9 || k * size < s * STEPS * STEP_BYTES)) break;
-      double time = tile_time(q, s, m, n, k, size);
-      if (time < best) {
-        best = time;
-        *plan = q;
-        *splits = s;
-      }
-    }
-  return best;
-}
-
 }  // namespace
 
-extern "C" {
-
-/* Into how many runs of rows the columns' sums are cut: about four
- * workgroups a CU, and at least 8 rows each. */
-int32_t vgpu_ops_slope_parts(int64_t m, int64_t n, int32_t dtype) {
-  int64_t per = 64 * (dtype == DT_F32 ? 4 : 8), blocks = (n + per - 1) / per;
-  return (int32_t)std::max<int64_t>(1, std::min<int64_t>((m + 7) / 8, 1024 / blocks));
-}
-
-int vgpu_ops_slope(const SlopeArgs *args, void *stream) {
-  const SlopeArgs &p = *args;
-  if (p.m <= 0 || p.n <= 0 || p.parts < 1 || p.parts > 65535 || (p.dz && p.lddz < p.n) ||
-      (p.act != ACT_NONE && !p.z) || (p.dbias && !p.part))
-    return OPS_BAD_ARG;
-  hipStream_t s = (hipStream_t)stream;
+int launch_slope(const SlopeArgs &p, hipStream_t s) {
   if (p.dtype == DT_F32) return run_slope<float>(p, s);
   if (p.dtype == DT_BF16) return run_slope<bf16>(p, s);
-  if (p.dtype == DT_FP16) return run_slope<fp16>(p, s);
-  return OPS_BAD_ARG;
+  return run_slope<fp16>(p, s);
 }
 
-/* Which kernel, over how many parts k is split, and how many of the rows go
- * there: the others, a last band of up to 32, may go to a launch of their own
- * rather than to a row of tiles. */
-void vgpu_ops_gemm_plan(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t a_kc, int32_t b_kc,
-                        int32_t bare, int32_t *plan, int32_t *splits, int64_t *rows) {
-  int size = dtype == DT_F32 ? 4 : 2;
-  *splits = 1;
-  *rows = m;
-  if (k <= OUTER_K && !a_kc && !b_kc && bare && m <= 65535 * 4 * OUTER_ROWS) {
-    *plan = PLAN_OUTER;
-    return;
-  }
-  if (a_kc && m <= 32 && (!b_kc || m <= 16 || n * k * size <= 1 << 24)) {
-    *plan = PLAN_ROWS;
-    int64_t steps = (k * size + STEP_BYTES - 1) / STEP_BYTES;
-    int64_t strip = b_kc ? 16 : 256 / size, strips = (n + strip - 1) / strip;
-    *splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({256 / strips, steps / 64, 64}));
-    return;
-  }
-  double time = best_tiles(m, n, k, size, plan, splits);
-  int64_t band = m % 256;
-  if (m > 256 && band >= 1 && band <= 32) {
-    int32_t q, s;
-    /* the band reads b once more, at 4.5 TB/s */
-    double apart = best_tiles(m - band, n, k, size, &q, &s) + 6. + (double)n * k * size / 4.5e6;
-    if (apart < time) {
-      *plan = q;
-      *splits = s;
-      *rows = m - band;
-    }
-  }
-}
-
-int vgpu_ops_gemm(const GemmArgs *args, void *stream) {
-  const GemmArgs &p = *args;
-  if (p.m <= 0 || p.n <= 0 || p.k < 0 || p.splits < 1 || p.plan < 0 ||
-      p.plan > PLAN_OUTER || (p.splits > 1 && !p.work))
-    return OPS_BAD_ARG;
-  if (p.plan == PLAN_ROWS && (p.m > 32 || !p.a_kc)) return OPS_BAD_ARG;
-  if (p.plan == PLAN_OUTER && (p.k > OUTER_K || p.a_kc || p.b_kc || p.bias || p.res || p.z ||
-                               p.act || p.splits > 1 || p.m > 65535 * 4 * OUTER_ROWS))
-    return OPS_BAD_ARG;
-  int size = p.dtype == DT_F32 ? 4 : 2;
-  /* 16-byte loads at 32-bit offsets inside a tile; a k that is contiguous is
-   * read in whole chunks */
-  if ((uintptr_t)p.a % 16 || (uintptr_t)p.b % 16 || p.lda * size % 16 || p.ldb * size % 16 ||
-      ((p.a_kc || p.b_kc) && p.k * size % 16) || p.lda < 0 || p.ldb < 0 ||
-      p.lda * size >= (1 << 23) || p.ldb * size >= (1 << 23))
-    return OPS_BAD_ARG;
-  hipStream_t s = (hipStream_t)stream;
+int launch_gemm(const GemmArgs &p, hipStream_t s) {
   if (p.dtype == DT_F32) return run<float>(p, s);
   if (p.dtype == DT_BF16) return run<bf16>(p, s);
-  if (p.dtype == DT_FP16) return run<fp16>(p, s);
-  return OPS_BAD_ARG;
+  return run<fp16>(p, s);
 }
 
-int vgpu_ops_repack(const void *src, int64_t rs, int64_t cs, int64_t rows, int64_t cols, void *dst,
-                    int64_t ld, int32_t dtype, void *stream) {
-  if (rows <= 0 || cols < 0 || ld < cols || ld <= 0) return OPS_BAD_ARG;
+int launch_repack(const void *src, int64_t rs, int64_t cs, int64_t rows, int64_t cols, void *dst,
+                  int64_t ld, int size, hipStream_t s) {
   dim3 grid((unsigned)std::min<int64_t>((ld + 255) / 256, 1024),
             (unsigned)std::min<int64_t>(rows, 16384));
-  hipStream_t s = (hipStream_t)stream;
-  if (dtype == DT_F32)
-    repack<float><<<grid, 256, 0, s>>>((const float *)src, rs, cs, rows, cols, (float *)dst, ld);
-  else if (dtype == DT_BF16 || dtype == DT_FP16) /* bits only */
-    repack<uint16_t><<<grid, 256, 0, s>>>((const uint16_t *)src, rs, cs, rows, cols,
-                                          (uint16_t *)dst, ld);
+  if (size == 4)
+    repack<<<grid, 256, 0, s>>>((const uint32_t *)src, rs, cs, rows, cols, (uint32_t *)dst, ld);
   else
-    return OPS_BAD_ARG;
+    repack<<<grid, 256, 0, s>>>((const uint16_t *)src, rs, cs, rows, cols, (uint16_t *)dst, ld);
   return OPS_LAUNCHED();
 }
-
-}  // extern "C"

@@ -22,14 +22,9 @@ def _struct(name, **groups):
     return type(name, (ctypes.Structure,), {"_fields_": fields})
 
 
-GemmArgs = _struct(
-    "GemmArgs", a=(c_void_p, "a b"), b=(c_int64, "lda ldb a_extent b_extent m n k"),
-    c=(c_void_p, "bias res"), d=(c_int64, "ldr"), e=(c_void_p, "y"), f=(c_int64, "ldy"),
-    g=(c_void_p, "z"), h=(c_int64, "ldz"), i=(c_void_p, "work"),
-    j=(c_int32, "dtype a_kc b_kc act plan splits"))
-SlopeArgs = _struct(
-    "SlopeArgs", a=(c_void_p, "dy z dz dbias part"), b=(c_int64, "lddy ldz lddz m n"),
-    c=(c_int32, "dtype act parts"))
+LinearArgs = _struct(
+    "LinearArgs", a=(c_void_p, "x w bias res dy y z dx dw db work"),
+    b=(c_int64, "m n k xs0 xs1 ws0 ws1 ldr lddy work_bytes"), c=(c_int32, "dtype act"))
 NormArgs = _struct(
     "NormArgs", a=(c_void_p, "x weight bias dy y dx dweight dbias mean rstd part"),
     b=(c_int64, "ldx ldy lddy lddx rows groups d"), c=(c_int32, "dtype wtype parts"),
@@ -52,16 +47,10 @@ def library() -> ctypes.CDLL:
         raise RuntimeError(
             "libvgpu_ops.so is not built: run `make native` (hipcc, gfx950)")
     lib = ctypes.CDLL(str(path))
-    for name, struct in (("gemm", GemmArgs), ("slope", SlopeArgs), ("norm", NormArgs),
-                         ("distill", DistillArgs)):
+    for name, struct in (("linear", LinearArgs), ("norm", NormArgs), ("distill", DistillArgs)):
         getattr(lib, "vgpu_ops_" + name).argtypes = [POINTER(struct), c_void_p]
-    lib.vgpu_ops_repack.argtypes = [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
-                                    c_int64, c_int32, c_void_p]
-    lib.vgpu_ops_gemm_plan.argtypes = [c_int64, c_int64, c_int64, c_int32, c_int32, c_int32,
-                                       c_int32, POINTER(c_int32), POINTER(c_int32),
-                                       POINTER(c_int64)]
-    lib.vgpu_ops_gemm_plan.restype = None
-    lib.vgpu_ops_slope_parts.argtypes = [c_int64, c_int64, c_int32]
+    lib.vgpu_ops_linear_work.argtypes = [POINTER(LinearArgs)]
+    lib.vgpu_ops_linear_work.restype = c_int64
     lib.vgpu_ops_norm_parts.argtypes = [c_int64, c_int64, c_int64]
     lib.vgpu_ops_distill_chunks.argtypes = [c_int64, c_int64, c_int32]
     return lib
@@ -81,8 +70,11 @@ _entries = {}   # name -> bound function
 _devices = set()  # whose architecture has been looked at
 
 
-def _bind(name):
-    return _entries.setdefault(name, getattr(library(), "vgpu_ops_" + name))
+def entry(name: str):
+    found = _entries.get(name)
+    if found is None:
+        found = _entries[name] = getattr(library(), "vgpu_ops_" + name)
+    return found
 
 
 def _look_at(index):
@@ -100,7 +92,7 @@ def launch(name: str, device: torch.device, *args) -> None:
     if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
             return launch(name, device, *args)
-    rc = (_entries.get(name) or _bind(name))(*args, torch._C._cuda_getCurrentRawStream(index))
+    rc = entry(name)(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         raise RuntimeError(f"vgpu_ops_{name}: " + ("refused the arguments" if rc < 0
                                                    else f"HIP error {rc}"))
@@ -109,7 +101,7 @@ def launch(name: str, device: torch.device, *args) -> None:
 @lru_cache(maxsize=4096)
 def plan(name: str, *sizes) -> int:
     """What a launch of these sizes needs; a function of the sizes alone."""
-    return getattr(library(), "vgpu_ops_" + name)(*sizes)
+    return entry(name)(*sizes)
 
 
 def needs_grad(*tensors) -> bool:

@@ -7,16 +7,14 @@ rounded once.
 """
 from __future__ import annotations
 
-import ctypes
-from functools import lru_cache
-
 import torch
 import torch.nn.functional as F
 
 from . import _native
-from ._native import DTYPES, GemmArgs, SlopeArgs, launch, ptr, rows_of
+from ._native import DTYPES, LinearArgs, launch, ptr, rows_of
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+RELU = ACTIVATIONS["relu"]
 _PLAIN = {"none": lambda z: z, "relu": F.relu, "gelu": F.gelu, "silu": F.silu}
 
 
@@ -68,101 +66,41 @@ def formula(x, weight, bias, residual, activation):
     return y if residual is None else y + residual
 
 
-@lru_cache(maxsize=4096)
-def _plan(m, n, k, dtype, a_kc, b_kc, bare):
-    plan, splits, rows = ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int64()
-    _native.library().vgpu_ops_gemm_plan(m, n, k, dtype, a_kc, b_kc, bare, ctypes.byref(plan),
-                                         ctypes.byref(splits), ctypes.byref(rows))
-    return plan.value, splits.value, rows.value
+def _launch(a, device):
+    """Runs a call with the workspace that it takes."""
+    size = _native.entry("linear_work")(a)
+    if size:
+        if size < 0:
+            raise ValueError("linear: too many values to sum over" if size == -2
+                             else "linear: vgpu_ops_linear refused the arguments")
+        work = torch.empty(size, dtype=torch.uint8, device=device)
+        a.work, a.work_bytes = work.data_ptr(), size
+    launch("linear", device, a)
 
 
-def _operand(t, any_axis=True):
-    """A matrix [rows, k] as the kernel reads it: (tensor, ld, k contiguous,
-    bytes that may be read, k).  Loads are 16 bytes wide, so rows that do not
-    start on 16 bytes, or that end inside 16, are laid out anew with zeros
-    behind; so is a matrix that is contiguous along neither axis, or not along
-    k where any_axis is false."""
-    rows, k = t.shape
-    s0, s1 = t.stride()
-    size = t.element_size()
-    if t.data_ptr() % 16 == 0:
-        if rows == 1 and s1 == 1:
-            s0 = k
-        if s1 == 1 and k * size % 16 == 0 and s0 * size % 16 == 0 and s0 * size < 1 << 23:
-            return t, s0, 1, ((rows - 1) * s0 + k) * size, k
-        if any_axis and s0 == 1 and s1 >= rows and s1 * size % 16 == 0 and s1 * size < 1 << 23:
-            # the last row's last load is whole: its 16 bytes are one line's
-            return t, s1, 0, -(-((k - 1) * s1 + rows) * size // 16) * 16, k
-    wide = -(-k * size // 16) * 16 // size
-    if wide * size >= 1 << 23:
-        raise ValueError(f"linear: {k} values to sum over, the most is {(1 << 23) // size - 8}")
-    out = torch.empty((rows, wide), dtype=t.dtype, device=t.device)
-    launch("repack", t.device, t.data_ptr(), s0, s1, rows, k, out.data_ptr(), wide,
-           DTYPES[t.dtype])
-    return out, wide, 1, rows * wide * size, wide
-
-
-def _gemm(a, b, out, bias=None, residual=None, act=0, z=None):
-    """out [m, n] = act(a [m, k] b [n, k]^T + bias) + residual."""
-    m, n = out.shape
-    dtype = DTYPES[out.dtype]
-    # few rows are read with k contiguous, but for the short sums of a
-    # weight's gradient
-    a, lda, a_kc, a_extent, ka = _operand(a, m > 32 or a.shape[1] <= 32)
-    b, ldb, b_kc, b_extent, kb = _operand(b)
-    # a k that one side pads with zeros ends beyond the other's extent, which
-    # reads as zeros there too
-    k = max(ka, kb)
-    bare = bias is None and residual is None and z is None and not act
-    plan, splits, rows = _plan(m, n, k, dtype, a_kc, b_kc, bare)
-    if rows < m:
-        _gemm(a[rows:], b, out[rows:], bias, None if residual is None else residual[rows:], act,
-              None if z is None else z[rows:])
-        m = rows
-    work = (torch.empty(splits * m * n, dtype=torch.float32, device=out.device)
-            if splits > 1 else None)
-    launch("gemm", out.device, GemmArgs(
-        a.data_ptr(), b.data_ptr(), lda, ldb, a_extent, b_extent, m, n, k, ptr(bias),
-        ptr(residual), residual.stride(0) if residual is not None else 0, out.data_ptr(),
-        out.stride(0), ptr(z), z.stride(0) if z is not None else 0, ptr(work),
-        dtype, a_kc, b_kc, act, plan, splits))
+def _matrix(t, k):
+    return t if t.dim() == 2 else t.reshape(-1, k)
 
 
 def _forward(x, weight, bias, residual, act, keep):
     """y, and what backward needs for the activation's slope: the value before
     it, or, where y tells as much (relu without a residual), y itself."""
     n, k = weight.shape
+    x2 = _matrix(x, k)
     y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
-    y2 = y.view(-1, n)
     z = None
-    if keep and act and not (act == ACTIVATIONS["relu"] and residual is None):
+    if keep and act and not (act == RELU and residual is None):
         # rounded like y: the slope is taken where a separate layer would
         # have stored its input
-        z = torch.empty_like(y2)
+        z = torch.empty(y.shape, dtype=x.dtype, device=x.device)
     if bias is not None and n > 1 and bias.stride(0) != 1:
         bias = bias.contiguous()
-    _gemm(x.reshape(-1, k), weight, y2, bias,
-          None if residual is None else rows_of(residual, n), act, z)
-    return y, (y2 if z is None else z) if act else None
-
-
-def _slope(dy, z, act, want_dz, want_db, dtype):
-    """dz = dy act'(z) (rows padded with zeros to 16 bytes) and its columns'
-    sums."""
-    m, n = dy.shape
-    code = DTYPES[dtype]
-    lanes = 16 // dy.element_size()
-    wide = -(-n // lanes) * lanes
-    dz = torch.empty((m, wide), dtype=dtype, device=dy.device) if want_dz else None
-    db = part = None
-    parts = _native.plan("slope_parts", m, n, code)
-    if want_db:
-        db = torch.empty(n, dtype=dtype, device=dy.device)
-        part = torch.empty(parts * n, dtype=torch.float32, device=dy.device)
-    launch("slope", dy.device, SlopeArgs(
-        dy.data_ptr(), ptr(z), ptr(dz), ptr(db), ptr(part), dy.stride(0),
-        z.stride(0) if z is not None else 0, wide, m, n, code, act, parts))
-    return dz, db
+    r2 = None if residual is None else rows_of(residual, n)
+    _launch(LinearArgs(
+        x2.data_ptr(), weight.data_ptr(), ptr(bias), ptr(r2), None, y.data_ptr(), ptr(z), None,
+        None, None, None, x2.shape[0], n, k, *x2.stride(), *weight.stride(),
+        0 if r2 is None else r2.stride(0), 0, 0, DTYPES[x.dtype], act), x.device)
+    return y, (y if z is None else z) if act else None
 
 
 class _Linear(torch.autograd.Function):
@@ -184,23 +122,14 @@ class _Linear(torch.autograd.Function):
                 (need_x, need_w, need_b), dy)
             return (*found, dr, None)
         n, k = weight.shape
-        act = ACTIVATIONS[ctx.activation]
-        dz = rows_of(dy, n)
-        db = None
-        # the products read 16 bytes at a time: rows of dy that do not allow
-        # it are copied along with the slope
-        size = dy.element_size()
-        loose = n * size % 16 or dz.stride(0) * size % 16 or dz.data_ptr() % 16
-        products = need_x or need_w
-        if need_b or (products and (act or loose)):
-            copy = products and bool(act or loose)
-            out, db = _slope(dz, None if z is None else z.view(-1, n), act, copy, need_b, dy.dtype)
-            dz = out if copy else dz
-        dx = dw = None
-        if need_x:
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            _gemm(dz, weight.t(), dx.view(-1, k))
-        if need_w:
-            dw = torch.empty((n, k), dtype=x.dtype, device=x.device)
-            _gemm(dz[:, :n].t(), x.reshape(-1, k).t(), dw)
+        x2, dy2 = _matrix(x, k), rows_of(dy, n)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        dw = torch.empty((n, k), dtype=x.dtype, device=x.device) if need_w else None
+        db = torch.empty(n, dtype=x.dtype, device=x.device) if need_b else None
+        if need_x or need_w or need_b:
+            _launch(LinearArgs(
+                x2.data_ptr(), weight.data_ptr(), None, None, dy2.data_ptr(), None, ptr(z),
+                ptr(dx), ptr(dw), ptr(db), None, x2.shape[0], n, k, *x2.stride(),
+                *weight.stride(), 0, dy2.stride(0), 0, DTYPES[x.dtype],
+                ACTIVATIONS[ctx.activation]), x.device)
         return dx, dw, db, dr, None
