@@ -465,23 +465,23 @@ __global__ __launch_bounds__(256) void gemm_join(GemmArgs p) {
   finish.one(m, n, v);
 }
 
-/* Few rows (m <= 32): b is read once, at the memory's rate, straight into the
+/* Few rows (m <= 16): b is read once, at the memory's rate, straight into the
  * matrix cores' registers.  A workgroup takes a strip of n; its eight waves
  * share k between them, a step of 64 bytes of a's k at a time, and join in
- * LDS.  FM is the number of 16-row pieces of a.
+ * LDS.
  *
  * k contiguous in b: the strip is 16 rows of b, a step 16 rows by 64 bytes.
  * k strided: the strip is 16 lanes by 16 bytes of n, a step 4 V rows of k;
  * lane i holds V neighbouring columns, of which the j-th go to the j-th
  * product, so 16-bit values are only turned inside a lane. */
-template <typename T, bool BKC, int FM>
+template <typename T, bool BKC>
 __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
   constexpr int V = Vec<T>::N, WAVES = 8;
-  constexpr int FN = BKC ? 1 : V;          /* products a step */
-  constexpr int STRIP = 16 * FN;           /* columns of y */
-  /* steps a wave has in flight, twice: 8 KB of b at least */
-  constexpr int C = BKC ? (FM == 1 ? 8 : 4) : sizeof(T) == 4 ? 2 : 1;
-  constexpr int LOADS = BKC ? 1 : V;       /* of b a step */
+  constexpr int FN = BKC ? 1 : V;    /* products a step */
+  constexpr int STRIP = 16 * FN;     /* columns of y */
+  constexpr int LOADS = BKC ? 1 : V; /* of b a step */
+  /* steps a wave has in flight, twice: 8 KB of b */
+  constexpr int C = 8 / LOADS;
   typedef typename Vec<T>::type vec;
   __shared__ f32x4 lds[WAVES][16][STRIP / 4];
 
@@ -494,11 +494,8 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
   int64_t b_left = p.b_extent - (b - (const char *)p.b);
   u32x4 ra = window(p.a, p.a_extent);
 
-  uint32_t a_off[FM], b_off[LOADS];
-#pragma unroll
-  for (int f = 0; f < FM; f++)
-    a_off[f] = f * 16 + i < p.m ? (uint32_t)((f * 16 + i) * p.lda * sizeof(T)) + g * 16
-                                : OUT_OF_RANGE;
+  uint32_t a_off = i < p.m ? (uint32_t)(i * p.lda * sizeof(T)) + g * 16 : OUT_OF_RANGE;
+  uint32_t b_off[LOADS];
 #pragma unroll
   for (int t = 0; t < LOADS; t++) {
     if (BKC) b_off[t] = n0 + i < p.n ? (uint32_t)(i * p.ldb * sizeof(T)) + g * 16 : OUT_OF_RANGE;
@@ -507,14 +504,12 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
   }
 
   struct Step {
-    u32x4 a[FM], b[LOADS];
+    u32x4 a, b[LOADS];
   };
   auto fetch = [&](Step &q, int64_t s) {
     bool in = s < s1 && (s * 4 + g) * V < p.k; /* k ends on a whole chunk of a */
     uint32_t at = (uint32_t)(s * 64);
-#pragma unroll
-    for (int f = 0; f < FM; f++)
-      q.a[f] = load16(ra, in ? a_off[f] + at : OUT_OF_RANGE);
+    q.a = load16(ra, in ? a_off + at : OUT_OF_RANGE);
     int64_t skip = BKC ? 0 : s * 4 * V * p.ldb * (int64_t)sizeof(T);
     u32x4 rb = window(b + skip, b_left - skip);
 #pragma unroll
@@ -522,9 +517,10 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
       q.b[t] = load16(rb, (BKC ? in : s < s1) ? b_off[t] + (BKC ? at : 0) : OUT_OF_RANGE);
   };
 
-  f32x4 acc[FM][FN] = {};
+  f32x4 acc[FN] = {};
   auto multiply = [&](const Step &q) {
-    Frag<T> fb[FN];
+    Frag<T> fa, fb[FN];
+    fa.v = __builtin_bit_cast(vec, q.a);
     if constexpr (BKC) {
       fb[0].v = __builtin_bit_cast(vec, q.b[0]);
     } else {
@@ -537,14 +533,9 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
         for (int t = 0; t < V; t++) fb[j].v[t] = r[t][j];
     }
 #pragma unroll
-    for (int f = 0; f < FM; f++) {
-      Frag<T> fa;
-      fa.v = __builtin_bit_cast(vec, q.a[f]);
+    for (int e = 0; e < PARTS<T>; e++)
 #pragma unroll
-      for (int j = 0; j < FN; j++)
-#pragma unroll
-        for (int e = 0; e < PARTS<T>; e++) acc[f][j] = mma(fb[j], fa, acc[f][j], e);
-    }
+      for (int j = 0; j < FN; j++) acc[j] = mma(fb[j], fa, acc[j], e);
   };
   Step even[C], odd[C];
   auto take = [&](Step(&now)[C], Step(&then)[C], int64_t s) {
@@ -563,28 +554,21 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
     take(odd, even, s + WAVES * C);
   }
 
+#pragma unroll
+  for (int j = 0; j < FN; j++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) /* column (4 g + e) FN + j of the strip, row i */
+      ((float *)lds[wave][i])[(4 * g + e) * FN + j] = acc[j][e];
+  __syncthreads();
   Epilogue<T> finish(p, blockIdx.y);
+  for (int q = threadIdx.x; q < 16 * (STRIP / 4); q += 512) {
+    int r = q / (STRIP / 4), c = q % (STRIP / 4);
+    int64_t n = n0 + c * 4;
+    if (r >= p.m || n >= p.n) continue;
+    f32x4 v = lds[0][r][c];
 #pragma unroll
-  for (int f = 0; f < FM; f++) {
-    if (f) __syncthreads();
-#pragma unroll
-    for (int j = 0; j < FN; j++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        /* column (4 g + e) FN + j of the strip, row i */
-        int c = (4 * g + e) * FN + j;
-        ((float *)lds[wave][i])[c] = acc[f][j][e];
-      }
-    __syncthreads();
-    for (int q = threadIdx.x; q < 16 * (STRIP / 4); q += 512) {
-      int r = q / (STRIP / 4), c = q % (STRIP / 4);
-      int64_t m = f * 16 + r, n = n0 + c * 4;
-      if (m >= p.m || n >= p.n) continue;
-      f32x4 v = lds[0][r][c];
-#pragma unroll
-      for (int w = 1; w < WAVES; w++) v += lds[w][r][c];
-      finish.one(m, n, v);
-    }
+    for (int w = 1; w < WAVES; w++) v += lds[w][r][c];
+    finish.one(r, n, v);
   }
 }
 
@@ -628,8 +612,7 @@ template <typename T, bool BKC>
 void launch_rows(const GemmArgs &p, hipStream_t stream) {
   constexpr int STRIP = BKC ? 16 : 16 * Vec<T>::N;
   dim3 grid((unsigned)((p.n + STRIP - 1) / STRIP), (unsigned)p.splits);
-  if (p.m <= 16) gemm_rows<T, BKC, 1><<<grid, 512, 0, stream>>>(p);
-  else gemm_rows<T, BKC, 2><<<grid, 512, 0, stream>>>(p);
+  gemm_rows<T, BKC><<<grid, 512, 0, stream>>>(p);
 }
 
 template <typename T, bool AKC, bool BKC>

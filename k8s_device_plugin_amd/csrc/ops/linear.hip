@@ -68,7 +68,15 @@ Plan choose(int64_t m, int64_t n, int64_t k, int size, bool a_kc, bool b_kc, boo
     p.plan = PLAN_OUTER;
     return p;
   }
-  if (a_kc && m <= 32 && (!b_kc || m <= 16 || n * k * size <= 1 << 24)) {
+  /* Up to 16 rows stream b past the matrix cores while it is small, and beyond
+   * that where a row of it is long enough for its workgroup and a's few rows
+   * cost nothing beside it; tiles take the others.  us, rows and tiles, weights
+   * out of the cache: 1 x 4096 x 4096 bf16 12.3 and 15.8; 1 x 50000 -> 4096
+   * bf16 71 and 81; 16 of them 115 and 85; 1 x 4096 -> 50000 bf16 90 and 82.
+   * With k strided in b, 8 rows fp32: 14336 -> 4096 48 and 53, 4096 -> 50000
+   * 166 and 158. */
+  bool rows = b_kc ? n * k * size <= 1 << 26 || (m <= 4 && k * size >= 1 << 14) : n < 1 << 15;
+  if (a_kc && m <= 16 && rows) {
     p.plan = PLAN_ROWS;
     int64_t steps = (k * size + STEP_BYTES - 1) / STEP_BYTES;
     int64_t strip = b_kc ? 16 : 256 / size, strips = (n + strip - 1) / strip;
@@ -191,7 +199,7 @@ struct Call {
   }
   void product(const Matrix &a, const Matrix &b, const GemmArgs &out) {
     /* few rows are read with k contiguous, but for short sums */
-    Operand p = prepare(a, a.rows > 32 || a.k <= OUTER_K), q = prepare(b, true);
+    Operand p = prepare(a, a.rows > 16 || a.k <= OUTER_K), q = prepare(b, true);
     product(p, q, a.rows, b.rows, out);
   }
 
