@@ -215,14 +215,14 @@ struct NormArgs {
   float eps;
 };
 
-/* Distillation from a teacher's top logits.  rows_loss, state and lse hold one
- * value a row, slot_p and slot_i `top` values a row, part 2 x chunks a row;
+/* Distillation from a teacher's top logits.  rows_loss, state, origin, most
+ * and log_sum hold one value a row, slot_p and slot_i `top` values a row, part 2 x chunks a row;
  * counts holds, for each 16 rows, how many of them have a target. */
 struct DistillArgs {
   const void *x, *index, *teacher;
   void *dx;
   const float *grad; /* of the loss: one value, or one a row */
-  float *rows_loss, *state, *lse, *slot_p, *loss, *counts;
+  float *rows_loss, *state, *origin, *most, *log_sum, *slot_p, *loss, *counts;
   int32_t *slot_i;
   float *part;
   int64_t ldx, lddx, ldi, ldt, rows, v;

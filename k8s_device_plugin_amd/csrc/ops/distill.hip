@@ -34,20 +34,35 @@ struct Unit {
   static __device__ float c(float temperature) { return (TWO ? 1.44269504089f : 1.f) / temperature; }
   static __device__ float exp(float v) { return TWO ? __builtin_amdgcn_exp2f(v) : expf(v); }
   static __device__ float from_natural(float v) { return TWO ? v * 1.44269504089f : v; }
-  static __device__ float to_natural(float v) { return TWO ? v * 0.69314718056f : v; }
 };
 
-/* The running maximum and the sum of exp relative to it.  It starts at the
- * lowest finite number, so that -inf adds nothing and NaN makes the sum NaN
- * without being asked for. */
+/* exp((x - m) c - log_sum) around a row's greatest logit m.  For 16-bit logits
+ * of ordinary size in one multiply-add, x c - offset, whose rounding is then
+ * below 2^-14 of the result; logits of any size, as of a row masked with the
+ * type's lowest value, and those of fp32 are taken from m first. */
+template <typename T>
+struct Around {
+  float m, c, log_sum, offset;
+  bool near;
+  __device__ Around(float top, float scale, float log = 0.f)
+      : m(top), c(scale), log_sum(log), offset(top * scale + log),
+        near(Unit<T>::TWO && fabsf(offset) < 1024.f) {}
+  __device__ float operator()(float x) const {
+    return Unit<T>::exp(near ? fmaf(x, c, -offset) : fmaf(x - m, c, -log_sum));
+  }
+};
+
+/* The running maximum of x and the sum of exp relative to it.  It starts at
+ * the lowest finite number, so that -inf adds nothing and NaN makes the sum
+ * NaN without being asked for. */
 struct Run {
   float m, s;
 };
 
 template <typename T>
-__device__ inline Run join(Run a, Run b) {
+__device__ inline Run join(Run a, Run b, float c) {
   float m = fmaxf(a.m, b.m);
-  return {m, a.s * Unit<T>::exp(a.m - m) + b.s * Unit<T>::exp(b.m - m)};
+  return {m, a.s * Unit<T>::exp((a.m - m) * c) + b.s * Unit<T>::exp((b.m - m) * c)};
 }
 
 __device__ inline Run no_run() { return {-3.402823466e38f, 0.f}; }
@@ -72,8 +87,8 @@ constexpr float NO_TARGET = 0.f, TARGET = 1.f, BAD_INDEX = 2.f;
 constexpr int SLOT_ROWS = 16; /* rows a workgroup of distill_slots */
 
 /* What the teacher says of a row, a wave each: the slots' masses, and
- * sum_k p_k (log p_k - x[i_k]/T), to which the loss adds the log of the
- * softmax's sum.  A class that is named twice is folded into its first slot,
+ * sum_k p_k (log p_k - (x[i_k] - o)/T) with o = x[i] of one of the slots, to
+ * which the loss adds the log of the softmax's sum above o/T.  A class that is named twice is folded into its first slot,
  * so that no two slots write to one place of the gradient. */
 template <typename T>
 __global__ __launch_bounds__(1024) void distill_slots(DistillArgs p) {
@@ -110,10 +125,14 @@ __global__ __launch_bounds__(1024) void distill_slots(DistillArgs p) {
     float mass = 0.f;
     for (int k = lane; k < p.top; k += 64) mass += expf(sp[k] - high);
     mass = wave_sum(mass);
-    float log_mass = logf(mass), loss = 0.f;
+    float log_mass = logf(mass), loss = 0.f, origin = -INFINITY;
+    for (int k = lane; k < p.top; k += 64)
+      if (si[k] >= 0) origin = fmaxf(origin, to_f<T>(x[si[k]]));
+#pragma unroll
+    for (int o = 32; o; o >>= 1) origin = fmaxf(origin, __shfl_xor(origin, o, 64));
     for (int k = lane; k < p.top; k += 64) {
       float log_p = sp[k] - high - log_mass, m = expf(sp[k] - high) / mass;
-      if (some && si[k] >= 0 && m != 0.f) loss += m * (log_p - to_f<T>(x[si[k]]) * inv_t);
+      if (some && si[k] >= 0 && m != 0.f) loss += m * (log_p - (to_f<T>(x[si[k]]) - origin) * inv_t);
       sp[k] = m;
     }
     loss = wave_sum(loss);
@@ -121,6 +140,7 @@ __global__ __launch_bounds__(1024) void distill_slots(DistillArgs p) {
       targets[q] = state != NO_TARGET;
       p.rows_loss[row] = loss;
       p.state[row] = state;
+      p.origin[row] = origin;
     }
     if (!p.slot_p) continue;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"); /* other lanes' slots */
@@ -146,17 +166,21 @@ __global__ __launch_bounds__(1024) void distill_slots(DistillArgs p) {
   p.counts[blockIdx.x] = (float)n;
 }
 
-/* Ends a row: its loss from the teacher's part and the softmax's sum, one
- * thread's work.  Gives the log of the sum. */
+/* Ends a row, one thread's work: its loss from the teacher's part and the
+ * softmax's sum.  Gives the natural log of the sum relative to the maximum; of
+ * no finite logit at all that is -inf, and what follows from it NaN. */
 template <typename T>
 __device__ inline float finish(const DistillArgs &p, int64_t row, Run all) {
-  /* of no finite logit at all it is -inf, and what follows from it NaN */
-  float lse = Unit<T>::to_natural(all.m) + logf(all.s), state = p.state[row];
-  if (state == BAD_INDEX) lse = NAN;
+  float log_sum = logf(all.s), state = p.state[row];
+  if (state == BAD_INDEX) log_sum = NAN;
+  float above = (all.m - p.origin[row]) / p.temperature + log_sum;
   p.rows_loss[row] =
-      state == NO_TARGET ? 0.f : (p.rows_loss[row] + lse) * p.temperature * p.temperature;
-  if (p.lse) p.lse[row] = lse;
-  return lse;
+      state == NO_TARGET ? 0.f : (p.rows_loss[row] + above) * p.temperature * p.temperature;
+  if (p.most) {
+    p.most[row] = all.m;
+    p.log_sum[row] = log_sum;
+  }
+  return log_sum;
 }
 
 /* A vector as its bits. */
@@ -185,11 +209,19 @@ __device__ inline Run scan_vecs(const u32x4 *q, float c, Run r) {
   for (int u = 0; u < N; u++)
 #pragma unroll
     for (int e = 0; e < V; e++) top = fmaxf(top, Bits<T>::get(q[u], e));
-  float m = fmaxf(r.m, top * c), s = r.s * Unit<T>::exp(r.m - m);
+  float m = fmaxf(r.m, top), s = r.s * Unit<T>::exp((r.m - m) * c);
+  Around<T> part(m, c);
+  if (part.near) {
 #pragma unroll
-  for (int u = 0; u < N; u++)
+    for (int u = 0; u < N; u++)
 #pragma unroll
-    for (int e = 0; e < V; e++) s += Unit<T>::exp(fmaf(Bits<T>::get(q[u], e), c, -m));
+      for (int e = 0; e < V; e++) s += Unit<T>::exp(fmaf(Bits<T>::get(q[u], e), c, -part.offset));
+  } else {
+#pragma unroll
+    for (int u = 0; u < N; u++)
+#pragma unroll
+      for (int e = 0; e < V; e++) s += Unit<T>::exp((Bits<T>::get(q[u], e) - m) * c);
+  }
   return {m, s};
 }
 
@@ -231,34 +263,40 @@ __device__ inline Run scan(const DistillArgs &p, const T *x, int64_t i, int64_t 
 
 /* Of all TH threads; the first wave has the result. */
 template <typename T, int TH>
-__device__ inline Run join_all(Run r) {
+__device__ inline Run join_all(Run r, float c) {
   __shared__ Run lds[TH / 64];
 #pragma unroll
-  for (int o = 32; o; o >>= 1) r = join<T>(r, wave_neighbour(r, o));
+  for (int o = 32; o; o >>= 1) r = join<T>(r, wave_neighbour(r, o), c);
   if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = r;
   __syncthreads();
   if (threadIdx.x < 64) {
     r = lds[0];
 #pragma unroll
-    for (int w = 1; w < TH / 64; w++) r = join<T>(r, lds[w]);
+    for (int w = 1; w < TH / 64; w++) r = join<T>(r, lds[w], c);
   }
   return r;
 }
 
 template <typename T>
-__device__ inline void write_vec(u32x4 q, T *dx, int n, float c, float lse,
-                                 float scale) {
+__device__ inline void write_vec(u32x4 q, T *dx, int n, const Around<T> &part, float scale) {
   constexpr int V = Vec<T>::N;
   float v[V];
+  if (part.near) { /* asked once a vector: the same for the whole row */
 #pragma unroll
-  for (int e = 0; e < V; e++) v[e] = scale * Unit<T>::exp(fmaf(Bits<T>::get(q, e), c, -lse));
+    for (int e = 0; e < V; e++) v[e] = fmaf(Bits<T>::get(q, e), part.c, -part.offset);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; e++) v[e] = fmaf(Bits<T>::get(q, e) - part.m, part.c, -part.log_sum);
+  }
+#pragma unroll
+  for (int e = 0; e < V; e++) v[e] = scale * Unit<T>::exp(v[e]);
   store_vec<T>(dx, n, v);
 }
 
-/* The gradient of the same vectors; lse in the exponential's unit. */
+/* The gradient of the same vectors. */
 template <typename T, int TH>
 __device__ inline void write(const DistillArgs &p, const T *x, T *dx, int64_t i, int64_t to,
-                             float c, float lse, float scale) {
+                             const Around<T> &part, float scale) {
   constexpr int U = 4, V = Vec<T>::N;
   int64_t whole = min(to, p.v / V);
   u32x4 q[U];
@@ -266,10 +304,10 @@ __device__ inline void write(const DistillArgs &p, const T *x, T *dx, int64_t i,
     load_vecs<T, TH, U>(x, i, whole, q);
 #pragma unroll
     for (int u = 0; u < U; u++)
-      if (i + u * TH < whole) write_vec<T>(q[u], dx + (i + u * TH) * V, V, c, lse, scale);
+      if (i + u * TH < whole) write_vec<T>(q[u], dx + (i + u * TH) * V, V, part, scale);
   }
   if (threadIdx.x == 0 && whole < to)
-    write_vec<T>(load_tail<T>(x, p.v), dx + whole * V, (int)(p.v - whole * V), c, lse, scale);
+    write_vec<T>(load_tail<T>(x, p.v), dx + whole * V, (int)(p.v - whole * V), part, scale);
 }
 
 template <typename T, int TH>
@@ -291,9 +329,9 @@ struct Named {
     if (at >= 0) x = to_f<T>(logits[at]);
   }
   /* from the unrounded q; behind a barrier after the row's other stores */
-  __device__ void write(T *dx, int64_t from, int64_t to, float c, float lse, float scale) const {
+  __device__ void write(T *dx, int64_t from, int64_t to, const Around<T> &part, float scale) const {
     if (at < 0 || at < from || at >= to) return;
-    dx[at] = from_f<T>(scale * (Unit<T>::exp(fmaf(x, c, -lse)) - mass));
+    dx[at] = from_f<T>(scale * (part(x) - mass));
   }
 };
 
@@ -313,8 +351,8 @@ __global__ __launch_bounds__(256) void distill_forward(DistillArgs p) {
   const T *x = (const T *)p.x + row * p.ldx;
   int64_t vecs = (p.v + V - 1) / V;
   int64_t from = vecs * blockIdx.x / p.chunks, to = vecs * (blockIdx.x + 1) / p.chunks;
-  Run r = scan<T, 256>(p, x, from + threadIdx.x, to, Unit<T>::c(p.temperature), no_run());
-  r = join_all<T, 256>(r);
+  float c = Unit<T>::c(p.temperature);
+  Run r = join_all<T, 256>(scan<T, 256>(p, x, from + threadIdx.x, to, c, no_run()), c);
   if (threadIdx.x) return;
   if (p.chunks == 1) {
     finish<T>(p, row, r);
@@ -329,7 +367,7 @@ __global__ __launch_bounds__(256) void distill_forward(DistillArgs p) {
 template <typename T, int TH>
 __global__ __launch_bounds__(TH) void distill_both(DistillArgs p) {
   constexpr int V = Vec<T>::N, KEEP = 16, U = 4;
-  __shared__ float told[2];
+  __shared__ float told[3];
   int64_t row = blockIdx.y + (int64_t)blockIdx.z * 65535;
   if (row >= p.rows) return;
   const T *x = (const T *)p.x + row * p.ldx;
@@ -349,14 +387,15 @@ __global__ __launch_bounds__(TH) void distill_both(DistillArgs p) {
     for (int u = 0; u < U; u++) asm volatile("" : "+v"(kept[k + u]));
     r = scan_vecs<T, U>(kept + k, c, r);
   }
-  r = join_all<T, TH>(scan<T, TH>(p, x, i + KEEP * TH, vecs, c, r));
+  r = join_all<T, TH>(scan<T, TH>(p, x, i + KEEP * TH, vecs, c, r), c);
   if (threadIdx.x == 0) {
-    told[0] = Unit<T>::from_natural(finish<T>(p, row, r));
-    told[1] = scale;
+    told[0] = r.m;
+    told[1] = Unit<T>::from_natural(finish<T>(p, row, r));
+    told[2] = scale;
   }
   __syncthreads();
-  float lse = told[0];
-  scale = told[1];
+  Around<T> part(told[0], c, told[1]);
+  scale = told[2];
   if (state == NO_TARGET) {
     write_zeros<T, TH>(p, dx, i, vecs);
     return;
@@ -365,27 +404,28 @@ __global__ __launch_bounds__(TH) void distill_both(DistillArgs p) {
   for (int k = 0; k < KEEP; k++) {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" : "+v"(kept[k])); /* unpacked anew, not kept unpacked */
-    if (i + k * TH < whole) write_vec<T>(kept[k], dx + (i + k * TH) * V, V, c, lse, scale);
+    if (i + k * TH < whole) write_vec<T>(kept[k], dx + (i + k * TH) * V, V, part, scale);
   }
-  write<T, TH>(p, x, dx, i + KEEP * TH, vecs, c, lse, scale);
+  write<T, TH>(p, x, dx, i + KEEP * TH, vecs, part, scale);
   __threadfence_block();
   __syncthreads();
-  named.write(dx, 0, p.v, c, lse, scale);
+  named.write(dx, 0, p.v, part, scale);
   for (int k = threadIdx.x + TH; k < p.top; k += TH)
-    Named<T>(p, row, x, k).write(dx, 0, p.v, c, lse, scale);
+    Named<T>(p, row, x, k).write(dx, 0, p.v, part, scale);
 }
 
 /* A wave a row: joins the chunks in their order. */
 template <typename T>
 __global__ __launch_bounds__(64) void distill_join(DistillArgs p) {
   int64_t row = blockIdx.x;
+  float scale = Unit<T>::c(p.temperature);
   Run r = no_run();
   for (int c = threadIdx.x; c < p.chunks; c += 64) {
     const float *q = p.part + (row * p.chunks + c) * 2;
-    r = join<T>(r, Run{q[0], q[1]});
+    r = join<T>(r, Run{q[0], q[1]}, scale);
   }
 #pragma unroll
-  for (int o = 32; o; o >>= 1) r = join<T>(r, wave_neighbour(r, o));
+  for (int o = 32; o; o >>= 1) r = join<T>(r, wave_neighbour(r, o), scale);
   if (threadIdx.x == 0) finish<T>(p, row, r);
 }
 
@@ -428,12 +468,14 @@ __global__ __launch_bounds__(256) void distill_backward(DistillArgs p) {
       continue;
     }
     float scale = p.grad[p.reduction ? 0 : row] * (p.temperature * p.scale / told);
-    float lse = Unit<T>::from_natural(p.lse[row]);
-    write<T, 256>(p, x, dx, from + threadIdx.x, to, c, lse, scale);
+    Around<T> part(p.most[row], c, Unit<T>::from_natural(p.log_sum[row]));
+    Named<T> named(p, row, x, threadIdx.x);
+    write<T, 256>(p, x, dx, from + threadIdx.x, to, part, scale);
     __threadfence_block();
     __syncthreads();
-    for (int k = threadIdx.x; k < p.top; k += 256)
-      Named<T>(p, row, x, k).write(dx, from * V, min(to * V, p.v), c, lse, scale);
+    named.write(dx, from * V, min(to * V, p.v), part, scale);
+    for (int k = threadIdx.x + 256; k < p.top; k += 256)
+      Named<T>(p, row, x, k).write(dx, from * V, min(to * V, p.v), part, scale);
   }
 }
 
@@ -485,9 +527,9 @@ int vgpu_ops_distill(const DistillArgs *args, void *stream) {
       p.top <= 0 || p.top > MOST_SLOTS || p.chunks < 1 || !(p.temperature > 0.f) ||
       (p.index_bytes != 4 && p.index_bytes != 8) || p.reduction < 0 || p.reduction > 2)
     return OPS_BAD_ARG;
-  if (!p.state) return OPS_BAD_ARG;
-  if (p.grad ? !(p.dx && p.lse && p.slot_p && p.slot_i)
-             : !(p.rows_loss && p.index) || !p.slot_p != !p.slot_i || (p.chunks > 1 && (!p.part || p.dx)) ||
+  if (!p.state || !p.most != !p.log_sum) return OPS_BAD_ARG;
+  if (p.grad ? !(p.dx && p.most && p.slot_p && p.slot_i)
+             : !(p.rows_loss && p.index && p.origin) || !p.slot_p != !p.slot_i || (p.chunks > 1 && (!p.part || p.dx)) ||
                    (p.reduction && !p.loss) || (p.dx && !(p.slot_p && p.slot_i && p.reduction)))
     return OPS_BAD_ARG;
   if (p.reduction == 2 && !p.counts) return OPS_BAD_ARG;

@@ -31,7 +31,8 @@ NormArgs = _struct(
     d=(c_float, "eps"))
 DistillArgs = _struct(
     "DistillArgs",
-    a=(c_void_p, "x index teacher dx grad rows_loss state lse slot_p loss counts slot_i part"),
+    a=(c_void_p, "x index teacher dx grad rows_loss state origin most log_sum slot_p loss counts slot_i "
+                 "part"),
     b=(c_int64, "ldx lddx ldi ldt rows v"),
     c=(c_int32, "dtype ttype index_bytes top chunks reduction written"), d=(c_float, "temperature scale"))
 

@@ -91,7 +91,9 @@ def _plain(logits, index, teacher, temperature, reduction, scale):
     t = torch.where(here, teacher.to(kind) / temperature, -torch.inf)
     t = torch.where(here.any(-1, keepdim=True), t, 0.0)
     log_p = torch.log_softmax(t, -1)
-    x = torch.where(some.unsqueeze(-1), logits.to(kind) / temperature, 0.0)
+    x = torch.where(some.unsqueeze(-1), logits.to(kind), 0.0)
+    most = x.detach().amax(-1, keepdim=True)  # so that no finite logit leaves its range
+    x = (x - torch.where(most.isfinite(), most, 0.0)) / temperature
     log_q = torch.log_softmax(x, -1).gather(-1, index.long().clamp(0, logits.shape[-1] - 1))
     p = torch.where(here, log_p.exp(), 0.0)
     rows = torch.where(p != 0, p * (log_p - log_q), 0.0).sum(-1) * temperature ** 2
@@ -127,7 +129,7 @@ def _forward(logits, index, teacher, temperature, reduction, scale, keep):
             if chunks > 1 else None)
     rows_loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=device)
     loss = torch.empty((), dtype=torch.float32, device=device) if reduction else rows_loss
-    saved = torch.empty((rows * (2 + 2 * top) if keep else rows) + (rows + 15) // 16,
+    saved = torch.empty(rows * (4 + 2 * top if keep else 2) + (rows + 15) // 16,
                         dtype=torch.float32, device=device)
     a = _arguments(x, saved, rows, v, top, temperature, reduction, scale, chunks, keep)
     a.index, a.ldi, a.index_bytes = i.data_ptr(), i.stride(0), i.element_size()
@@ -144,11 +146,13 @@ def _arguments(x, saved, rows, v, top, temperature, reduction, scale, chunks, ke
     a = DistillArgs(x=x.data_ptr(), ldx=x.stride(0), rows=rows, v=v, dtype=DTYPES[x.dtype], top=top,
                     chunks=chunks, reduction=reduction, temperature=temperature, scale=scale,
                     index_bytes=8)
-    a.state = at = saved.data_ptr()
-    at += 4 * rows
+    row = 4 * rows
+    at = saved.data_ptr()
+    a.state, a.origin = at, at + row
+    at += 2 * row
     if keep:
-        a.lse, a.slot_p, a.slot_i = at, at + 4 * rows, at + 4 * rows * (1 + top)
-        at += 4 * rows * (1 + 2 * top)
+        a.most, a.log_sum, a.slot_p, a.slot_i = at, at + row, at + 2 * row, at + (2 + top) * row
+        at += (2 + 2 * top) * row
     a.counts = at
     return a
 

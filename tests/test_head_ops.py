@@ -489,6 +489,32 @@ def test_distill_masks_duplicates_and_extremes(device, dtype, reduction):
 
 
 @pytest.mark.parametrize("device,dtype", PAIRS)
+@pytest.mark.parametrize("t", [0.5, 1.0, 3.0])
+@pytest.mark.parametrize("v", [40, 9000])
+def test_distill_row_of_the_lowest_value(device, dtype, t, v):
+    """A row whose classes are all masked with the type's lowest value has a
+    softmax all the same: they weigh alike, and the loss is log v."""
+    logits, index, _ = distill_inputs(4, v, 1, dtype, device)
+    logits[1] = torch.finfo(dtype).min
+    logits[2] = -torch.finfo(dtype).min
+    logits[3] = torch.finfo(dtype).min
+    logits[3, v // 2:] = -float("inf")
+    index[3] = 1
+    leaf = logits.requires_grad_()
+    rows = ops.distill_loss(leaf, index, temperature=t, reduction="none")
+    want = t * t * torch.tensor([math.log(v), math.log(v), math.log(v // 2)], dtype=torch.float64,
+                                device=device)
+    # the sum of up to v ones is exact, its log and the product a few u off
+    within(rows.detach()[1:], want, 16 * U * want)
+    grad, = torch.autograd.grad(rows, leaf, torch.ones_like(rows))
+    want = torch.full((4, v), t / v, dtype=torch.float64, device=device)
+    want[3] = t / (v // 2)
+    want[3, v // 2:] = 0
+    want.scatter_add_(1, index, torch.full_like(want[:, :1], -t))
+    within(grad[1:], want[1:], 16 * U * (want[1:].abs() + t / v))
+
+
+@pytest.mark.parametrize("device,dtype", PAIRS)
 def test_distill_class_that_is_masked_in_the_student(device, dtype):
     """-inf in the logits: no mass, and a loss of +inf where the teacher has some."""
     logits, index, teacher = distill_inputs(3, 50, 3, dtype, device)

@@ -1,6 +1,10 @@
 """The zoo's heads run through the head operators and keep what they were:
 the parameters' names, the numbers, and what may be done with a model."""
 import json
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -9,6 +13,7 @@ import torch.nn.functional as F
 
 from k8s_device_plugin_amd.models import zoo
 
+REPO = Path(__file__).resolve().parent.parent
 GPU = pytest.param("cuda", marks=pytest.mark.gpu)
 
 
@@ -27,7 +32,7 @@ class TorchHead(nn.Module):
         return self.c(x)
 
 
-def close(a, b, dtype=torch.float32):
+def close(a, b):
     """Two fp32 evaluations of sums of up to 25088 terms, through 3 layers."""
     return (a.double() - b.double()).norm() <= 3 * 25088 * 2.0 ** -24 * b.double().norm()
 
@@ -111,3 +116,36 @@ def test_models_still_script_and_run_in_64_bits(device):
     out = fc(torch.randn(2, 3, 8, device=device, dtype=torch.float64))
     assert out.dtype == torch.float64
     zoo.loss_of(zoo.CASES["lstm_train"], out, torch.tensor([0, 1], device=device)).backward()
+
+
+@pytest.mark.gpu
+def test_heads_under_enforcement(tmp_path):
+    """The operators' launches and memory go through the preloaded library as
+    any other's: the same numbers under a quota, and an allocation beyond it
+    still fails."""
+    code = (
+        "import json, torch\n"
+        "from k8s_device_plugin_amd.models import zoo\n"
+        "torch.manual_seed(0)\n"
+        "head = zoo.VGG16().classifier.eval().cuda()\n"
+        "x = torch.randn(3, 25088, device='cuda', requires_grad=True)\n"
+        "loss = zoo.loss_of(zoo.CASES['vgg16_train'], head(x), torch.tensor([1, 2, 3], device='cuda'))\n"
+        "loss.backward()\n"
+        "sums = [float(p.grad.double().sum()) for p in head.parameters()] + [float(loss)]\n"
+        "err = 'none'\n"
+        "try: torch.empty(9 << 30, dtype=torch.uint8, device='cuda')\n"
+        "except torch.cuda.OutOfMemoryError: err = 'oom'\n"
+        "print(json.dumps({'sums': sums, 'err': err}))\n")
+    csrc = REPO / "k8s_device_plugin_amd" / "csrc"
+
+    def child(**env):
+        out = subprocess.run([sys.executable, "-c", code], env={**os.environ, **env},
+                             capture_output=True, text=True, timeout=240, cwd=REPO)
+        assert out.returncode == 0, out.stderr[-2000:]
+        return json.loads(out.stdout.strip().splitlines()[-1])
+
+    free = child()
+    held = child(LD_PRELOAD=str(csrc / "libvgpu-hip.so"), VGPU_DEVICE_MEMORY_LIMIT="8192m",
+                 VGPU_DEVICE_MEMORY_SHARED_CACHE=str(tmp_path / "region.cache"))
+    assert held["sums"] == free["sums"]
+    assert (free["err"], held["err"]) == ("none", "oom")
