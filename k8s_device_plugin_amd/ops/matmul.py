@@ -24,6 +24,7 @@ def linear(x, weight, bias=None, *, activation="none", residual=None):
     x [..., K], weight [N, K], bias [N] and residual [..., N], all of one type
     (float32, bfloat16 or float16 on a GPU) and on one device; any strides.
     activation: "none", "relu", "gelu" (with the error function) or "silu".
+    A row of x, and with gradients one of the result, is shorter than 8 MiB.
     Under autocast the operands are cast as for torch's own linear.  On the
     CPU, and while a call is traced or transformed, the formula is run by
     torch.  Runs on the current stream of x's device; can be captured into a
@@ -56,6 +57,9 @@ def linear(x, weight, bias=None, *, activation="none", residual=None):
     if x.numel() == 0 or weight.numel() == 0:
         return formula(x, weight, bias, residual, activation)
     if _native.needs_grad(x, weight, bias, residual):
+        if n * x.element_size() >= 1 << 23:
+            raise ValueError(f"linear with gradients over {n} outputs: a row must be shorter "
+                             "than 8 MiB")
         return _Linear.apply(x, weight, bias, residual, activation)
     return _forward(x, weight, bias, residual, ACTIVATIONS[activation], False)[0]
 

@@ -19,8 +19,15 @@ from k8s_device_plugin_amd import ops
 
 REPO = Path(__file__).resolve().parent.parent
 U = 2.0 ** -24
+CSRC = REPO / "k8s_device_plugin_amd" / "csrc"
 GPU = pytest.param("cuda", marks=pytest.mark.gpu)
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def native():
+    if not (CSRC / "libvgpu_ops.so").exists():
+        subprocess.run(["make", "libvgpu_ops.so"], cwd=CSRC, check=True, capture_output=True)
 
 
 def half_step(dtype):
@@ -250,6 +257,9 @@ def test_linear_refusals(device):
             ops.linear(x.double(), w.double())
         with pytest.raises(ValueError, match="8 MiB"):
             ops.linear(torch.zeros(1, 1 << 21, device=device), torch.zeros(1, 1 << 21, device=device))
+        with pytest.raises(ValueError, match="8 MiB"):
+            ops.linear(torch.zeros(1, 4, device=device),
+                       torch.zeros(1 << 21, 4, device=device, requires_grad=True))
 
 
 # ---------------------------------------------------------------------------
@@ -747,6 +757,42 @@ def test_traced_and_transformed_calls_run_the_formula():
     traced = torch.jit.trace(lambda r: ops.linear(r, w), (x,))(x)
     for other in (mapped, traced):
         assert (y - other).abs().max() <= 66 * 2 * U * float((x.abs() @ w.abs().t()).max())
+
+
+def test_bad_calls_of_the_library_are_refused():
+    """The C entry points look at what they are given before they launch."""
+    import ctypes
+
+    from k8s_device_plugin_amd.ops import _native as n
+
+    lib = n.library()
+    at = torch.zeros(64, 64).data_ptr()
+
+    def linear(**how):
+        a = dict(x=at, w=at, y=at, m=4, n=4, k=4, xs0=4, xs1=1, ws0=4, ws1=1, dtype=0, act=0)
+        return lib.vgpu_ops_linear(ctypes.byref(n.LinearArgs(**{**a, **how})), None)
+
+    for how in (dict(m=0), dict(n=-1), dict(k=0), dict(dtype=3), dict(act=4), dict(xs0=-4),
+                dict(y=None), dict(w=None), dict(dy=at, act=1), dict(x=at + 4)):
+        assert linear(**how) < 0, how  # the last: a workspace is wanted
+
+    def norm(**how):
+        a = dict(x=at, y=at, ldx=8, ldy=8, rows=2, groups=1, d=8, eps=1e-5)
+        return lib.vgpu_ops_norm(ctypes.byref(n.NormArgs(**{**a, **how})), None)
+
+    for how in (dict(rows=0), dict(d=0), dict(d=32769), dict(groups=0), dict(dtype=7), dict(wtype=2),
+                dict(y=None), dict(dy=at, parts=0), dict(dy=at, parts=2, dweight=at)):
+        assert norm(**how) < 0, how
+
+    def distill(**how):
+        a = dict(x=at, index=at, rows_loss=at, state=at, origin=at, loss=at, counts=at, ldx=8, ldi=1,
+                 rows=2, v=8, top=1, index_bytes=8, chunks=1, reduction=2, temperature=1.0, scale=1.0)
+        return lib.vgpu_ops_distill(ctypes.byref(n.DistillArgs(**{**a, **how})), None)
+
+    for how in (dict(rows=0), dict(v=0), dict(top=0), dict(top=1025), dict(chunks=0), dict(dtype=9),
+                dict(index_bytes=2), dict(reduction=3), dict(temperature=0.0), dict(state=None),
+                dict(counts=None), dict(loss=None), dict(chunks=2), dict(dx=at), dict(grad=at)):
+        assert distill(**how) < 0, how
 
 
 @pytest.mark.gpu
