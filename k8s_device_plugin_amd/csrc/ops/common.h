@@ -111,7 +111,7 @@ __device__ inline float logistic(float z) {
   return __builtin_amdgcn_rcpf(1.f + __expf(-z));
 }
 
-/* y = act(z); the slope is dy/dz.  gelu is z Phi(z). */
+/* y = act(z); gelu is z Phi(z). */
 template <typename T, int ACT>
 __device__ inline float activate(float z) {
   float e;
@@ -137,18 +137,19 @@ __device__ inline void activate_all(f32x4 (&v)[N], int act) {
   else if (act == ACT_SILU) activate_each<T, ACT_SILU>(v);
 }
 
+/* g act'(z).  relu drops g where z is not above 0, an infinite one too. */
 template <typename T>
-__device__ inline float slope(float z, int act) {
-  if (act == ACT_RELU) return z > 0.f ? 1.f : 0.f;
+__device__ inline float slope(float g, float z, int act) {
+  if (act == ACT_RELU) return z <= 0.f ? 0.f : g;
   if (act == ACT_GELU) {
     float e, cdf = normal_cdf<T>(z, &e);
-    return cdf + z * 0.39894228040143268f * e;
+    return g * (cdf + z * 0.39894228040143268f * e);
   }
   if (act == ACT_SILU) {
     float s = logistic<T>(z);
-    return s * (1.f + z * (1.f - s));
+    return g * (s * (1.f + z * (1.f - s)));
   }
-  return 1.f;
+  return g;
 }
 
 /* The kernels that a product may run on: tiles of 256 x 256, 128 x 128,

@@ -43,7 +43,9 @@ __device__ inline f32x4 mma(const Frag<float> &a, const Frag<float> &b, f32x4 c,
 /* The same with the sum held in the accumulation registers for good.  Where
  * all 256 of them are sums the compiler would move some back and forth in
  * every step.  It cannot see what these write: the caller keeps other products
- * between two into the same sum, and waits (settle) before it reads one. */
+ * between two into the same sum, and waits (settle) before it reads one.  Nor
+ * does it put the two wait states between a vector instruction's write of a or b
+ * and these: fragments come from LDS reads alone. */
 __device__ inline void mma_pinned(const Frag<bf16> &a, const Frag<bf16> &b, f32x4 &c, int) {
   asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a.v), "v"(b.v));
 }
@@ -680,7 +682,7 @@ __global__ __launch_bounds__(256) void slope_rows(SlopeArgs p) {
     if (p.act != ACT_NONE) {
       load_vec<T>(z + r * p.ldz + col, n, u);
 #pragma unroll
-      for (int e = 0; e < V; e++) g[e] *= slope<T>(u[e], p.act);
+      for (int e = 0; e < V; e++) g[e] = slope<T>(g[e], u[e], p.act);
     }
 #pragma unroll
     for (int e = 0; e < V; e++) sum[e] += g[e];

@@ -124,7 +124,7 @@ def _forward(logits, index, teacher, temperature, reduction, scale, keep):
     # written; few long rows are better cut in pieces, and wait for backward
     dx = None
     if keep and reduction and chunks == 1:
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+        dx = logits.new_empty(logits.shape)
     part = (torch.empty(rows * chunks * 2, dtype=torch.float32, device=device)
             if chunks > 1 else None)
     rows_loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=device)
@@ -184,7 +184,7 @@ class _Distill(torch.autograd.Function):
                        scale, _native.plan("distill_chunks", rows, v, 1), True)
         a.written = dx is not None
         if dx is None:
-            dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            dx = logits.new_empty(logits.shape)
         a.dx, a.lddx, a.grad = dx.data_ptr(), v, grad.data_ptr()
         launch("distill", logits.device, a)
         return dx, None, None, None, None, None

@@ -91,12 +91,12 @@ def _forward(x, weight, bias, residual, act, keep):
     it, or, where y tells as much (relu without a residual), y itself."""
     n, k = weight.shape
     x2 = _matrix(x, k)
-    y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape[:-1] + (n,))
     z = None
     if keep and act and not (act == RELU and residual is None):
         # rounded like y: the slope is taken where a separate layer would
         # have stored its input
-        z = torch.empty(y.shape, dtype=x.dtype, device=x.device)
+        z = x.new_empty(y.shape)
     if bias is not None and n > 1 and bias.stride(0) != 1:
         bias = bias.contiguous()
     r2 = None if residual is None else rows_of(residual, n)
@@ -127,9 +127,9 @@ class _Linear(torch.autograd.Function):
             return (*found, dr, None)
         n, k = weight.shape
         x2, dy2 = _matrix(x, k), rows_of(dy, n)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        dw = torch.empty((n, k), dtype=x.dtype, device=x.device) if need_w else None
-        db = torch.empty(n, dtype=x.dtype, device=x.device) if need_b else None
+        dx = x.new_empty(x.shape) if need_x else None
+        dw = x.new_empty((n, k)) if need_w else None
+        db = x.new_empty(n) if need_b else None
         if need_x or need_w or need_b:
             _launch(LinearArgs(
                 x2.data_ptr(), weight.data_ptr(), None, None, dy2.data_ptr(), None, ptr(z),

@@ -72,7 +72,7 @@ def _forward(x, weight, bias, groups, eps, keep):
     width = x.shape[-1]
     x2 = rows_of(x, width)
     rows = x2.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     stats = (torch.empty((2, rows * groups), dtype=torch.float32, device=x.device)
              if keep else None)
     weight, bias = _vector(weight), _vector(bias)
@@ -105,9 +105,9 @@ class _LayerNorm(torch.autograd.Function):
         width = x.shape[-1]
         x2, dy2 = rows_of(x, width), rows_of(dy, width)
         rows, d = x2.shape[0], width // groups
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        dw = torch.empty(width, dtype=weight.dtype, device=x.device) if need_w else None
-        db = torch.empty(width, dtype=bias.dtype, device=x.device) if need_b else None
+        dx = x.new_empty(x.shape) if need_x else None
+        dw = weight.new_empty(width) if need_w else None
+        db = bias.new_empty(width) if need_b else None
         parts = _native.plan("norm_parts", rows, groups, d)
         part = (torch.empty(2 * parts * width, dtype=torch.float32, device=x.device)
                 if parts > 1 and (need_w or need_b) else None)

@@ -229,6 +229,24 @@ def test_linear_offsets_past_32_bits():
     within(y[:, -64:], x.double() @ far.t(), 8194 * U * (x.double().abs() @ far.t().abs()))
 
 
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_linear_relu_drops_what_is_not_finite_where_it_is_off(device, dtype, residual):
+    x = -torch.ones(3, 16, device=device, dtype=dtype)  # every sum is -16 ...
+    x[1] = 1                                            # ... 16 ...
+    x[2] = float("nan")                                 # ... or no number, which passes
+    w = torch.ones(24, 16, device=device, dtype=dtype)
+    b = torch.zeros(24, device=device, dtype=dtype, requires_grad=True)
+    r = torch.zeros(3, 24, device=device, dtype=dtype) if residual else None
+    dy = torch.ones(3, 24, device=device, dtype=dtype)
+    dy[0, 3], dy[0, 4], dy[1, 5] = float("inf"), float("nan"), float("inf")
+    db, = torch.autograd.grad(ops.linear(x, w, b, activation="relu", residual=r), b, dy)
+    want = torch.full((24,), 2.0, device=device, dtype=dtype)
+    want[5] = float("inf")
+    assert torch.equal(db, want)
+
+
 def test_linear_gradients_by_differences():
     gen = seeded()
     x, w, b, r = (normal(gen, *s).double().requires_grad_() for s in ((3, 5), (4, 5), (4,), (3, 4)))
