@@ -251,3 +251,15 @@ __device__ inline void join_columns(const float *part, int64_t parts, int64_t wi
 }
 
 #define OPS_LAUNCHED() ((int)hipGetLastError())
+
+/* A launch holds fewer than 2^32 threads along an axis: `blocks` of at most
+ * 1024 threads in rows of up to 2^20 along x and z, `y` along y.  flat_block() is
+ * a workgroup's number, which may pass the last. */
+constexpr int64_t GRID_ROW = 1 << 20;
+inline dim3 flat_grid(int64_t blocks, int64_t y = 1) {
+  return dim3((unsigned)(blocks < GRID_ROW ? blocks : GRID_ROW), (unsigned)y,
+              (unsigned)((blocks + GRID_ROW - 1) / GRID_ROW));
+}
+__device__ inline int64_t flat_block() {
+  return (int64_t)blockIdx.z * GRID_ROW + blockIdx.x;
+}

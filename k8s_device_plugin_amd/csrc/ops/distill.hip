@@ -98,8 +98,10 @@ __global__ __launch_bounds__(1024) void distill_slots(DistillArgs p) {
   float *sp = slots + (int64_t)wave * 2 * p.top;
   int *si = (int *)(sp + p.top);
   float inv_t = 1.f / p.temperature;
+  int64_t block = flat_block();
+  if (block * SLOT_ROWS >= p.rows) return;
   for (int q = wave; q < SLOT_ROWS; q += waves) {
-    int64_t row = (int64_t)blockIdx.x * SLOT_ROWS + q;
+    int64_t row = block * SLOT_ROWS + q;
     if (row >= p.rows) {
       if (lane == 0) targets[q] = 0;
       continue;
@@ -163,7 +165,7 @@ __global__ __launch_bounds__(1024) void distill_slots(DistillArgs p) {
   if (threadIdx.x || !p.counts) return;
   int n = 0;
   for (int q = 0; q < SLOT_ROWS; q++) n += targets[q];
-  p.counts[blockIdx.x] = (float)n;
+  p.counts[block] = (float)n;
 }
 
 /* Ends a row, one thread's work: its loss from the teacher's part and the
@@ -488,13 +490,14 @@ template <typename T>
 int run(const DistillArgs &p, hipStream_t s) {
   if (p.grad) {
     int64_t pieces = p.rows * p.chunks;
-    /* few workgroups where most often there is nothing to do */
-    int64_t most = p.written ? 4096 : (int64_t)1 << 30;
+    /* few workgroups where most often there is nothing to do; else as many as
+     * a launch holds */
+    int64_t most = p.written ? 4096 : (1 << 24) - 1;
     distill_backward<T><<<(unsigned)std::min(pieces, most), 256, 0, s>>>(p);
     return OPS_LAUNCHED();
   }
   int waves = std::min(16, 65536 / (p.top * 8)); /* as far as 64 KB of LDS go */
-  distill_slots<T><<<(unsigned)((p.rows + SLOT_ROWS - 1) / SLOT_ROWS), waves * 64,
+  distill_slots<T><<<flat_grid((p.rows + SLOT_ROWS - 1) / SLOT_ROWS), waves * 64,
                      waves * p.top * 8, s>>>(p);
   /* the fewest threads whose registers hold the row */
   dim3 grid = rows_grid(p.chunks, p.rows);

@@ -9,6 +9,14 @@ namespace {
 
 constexpr int64_t LONGEST = 1 << 23; /* bytes of a row: tiles use 32-bit offsets */
 
+int64_t tiles_of(int plan, int64_t m, int64_t n) {
+  static const int side[4][2] = {{256, 256}, {128, 128}, {64, 128}, {32, 128}};
+  return ((m + side[plan][0] - 1) / side[plan][0]) * ((n + side[plan][1] - 1) / side[plan][1]);
+}
+
+/* A launch holds fewer than 2^32 threads along an axis. */
+constexpr int64_t MOST_TILES = (1 << 24) - 1;
+
 /* What a product takes in us with tiles of one kind, k in `splits` parts: in
  * turns of as many workgroups as the card holds (256 of the largest tile, 512
  * of the others; a last turn of up to 256 has a CU each), each of so much a
@@ -20,12 +28,11 @@ double tile_time(int plan, int64_t splits, int64_t m, int64_t n, int64_t k, int 
   struct Cost {
     double stage, own; /* us */
   };
-  static const int side[4][2] = {{256, 256}, {128, 128}, {64, 128}, {32, 128}};
   static const Cost full[2][4] = {{{1.33, 7.9}, {0.86, 5.0}, {0.595, 3.7}, {0.417, 4.2}},
                                   {{7.37, 5.9}, {3.71, 3.3}, {1.975, 2.3}, {1.096, 2.4}}};
   static const Cost half[2][4] = {{{1.33, 7.9}, {0.56, 3.7}, {0.378, 3.1}, {0.321, 2.6}},
                                   {{7.37, 5.9}, {1.99, 3.1}, {1.110, 1.2}, {0.657, 0.0}}};
-  int64_t tiles = ((m + side[plan][0] - 1) / side[plan][0]) * ((n + side[plan][1] - 1) / side[plan][1]);
+  int64_t tiles = tiles_of(plan, m, n);
   int64_t stages = (k * size + STEPS * STEP_BYTES - 1) / (STEPS * STEP_BYTES);
   int64_t each = (stages + splits - 1) / splits, slots = plan == 0 ? 256 : 512;
   int64_t turns = tiles * splits / slots, rest = tiles * splits % slots;
@@ -45,7 +52,7 @@ double best_tiles(int64_t m, int64_t n, int64_t k, int size, int32_t *plan, int3
       /* partial sums of no more than 1.5 GB */
       if (s > 1 && ((double)m * n * s * 4 > 1.5e9 || k * size < s * STEPS * STEP_BYTES)) break;
       double time = tile_time(q, s, m, n, k, size);
-      if (time < best) {
+      if (time < best && (q == 0 || tiles_of(q, m, n) <= MOST_TILES)) {
         best = time;
         *plan = q;
         *splits = s;
@@ -173,6 +180,7 @@ struct Call {
     int64_t k = std::max(a.k, b.k);
     bool bare = !out.bias && !out.res && !out.z && out.act == ACT_NONE;
     Plan p = planned(m, n, k, size, a.kc, b.kc, bare);
+    if (p.plan == 0 && tiles_of(0, p.rows, n) > MOST_TILES) code = OPS_TOO_LONG;
     if (p.rows < m) {
       auto below = [&](const void *q, int64_t ld) {
         return q ? (void *)((uintptr_t)q + p.rows * ld * size) : nullptr;

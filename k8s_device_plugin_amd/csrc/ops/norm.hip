@@ -48,8 +48,8 @@ __global__ __launch_bounds__(block_of<TH>()) void norm_forward(NormArgs p) {
   constexpr int V = Vec<T>::N;
   __shared__ float lds[TH / 64];
   int lane = threadIdx.x % TH;
-  int64_t row = (int64_t)blockIdx.x * rows_at_once<TH>() + threadIdx.x / TH;
-  if (row >= p.rows) return; /* a whole wave, and only where TH is 64 */
+  int64_t row = flat_block() * rows_at_once<TH>() + threadIdx.x / TH;
+  if (row >= p.rows) return; /* a whole wave where TH is 64, else all of them */
   int64_t group = blockIdx.y, d = p.d;
   const T *x = (const T *)p.x + row * p.ldx + group * d;
   float v[VECS][V];
@@ -272,7 +272,7 @@ void launch(const NormArgs &p, hipStream_t s) {
         <<<dim3(p.parts, (unsigned)p.groups), block_of<TH>(), 0, s>>>(p);
   else
     norm_forward<T, W, TH, VECS>
-        <<<dim3((unsigned)((p.rows + R - 1) / R), (unsigned)p.groups), block_of<TH>(), 0, s>>>(p);
+        <<<flat_grid((p.rows + R - 1) / R, p.groups), block_of<TH>(), 0, s>>>(p);
 }
 
 /* The fewest threads whose registers hold the row, with 16 values each or (of

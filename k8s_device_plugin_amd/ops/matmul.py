@@ -75,7 +75,7 @@ def _launch(a, device):
     size = _native.entry("linear_work")(a)
     if size:
         if size < 0:
-            raise ValueError("linear: too many values to sum over" if size == -2
+            raise ValueError("linear: an axis is too long" if size == -2
                              else "linear: vgpu_ops_linear refused the arguments")
         work = torch.empty(size, dtype=torch.uint8, device=device)
         a.work, a.work_bytes = work.data_ptr(), size

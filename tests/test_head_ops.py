@@ -229,6 +229,17 @@ def test_linear_offsets_past_32_bits():
     within(y[:, -64:], x.double() @ far.t(), 8194 * U * (x.double().abs() @ far.t().abs()))
 
 
+@pytest.mark.gpu
+def test_linear_rows_past_one_axis_of_a_launch():
+    rows = (1 << 29) + 3
+    x = torch.randn(1 << 20, 8, device="cuda", dtype=torch.float16).repeat(513, 1)[:rows]
+    w = torch.randn(8, 8, device="cuda", dtype=torch.float16)
+    y = ops.linear(x, w)
+    for part in (slice(0, 5), slice(1 << 28, (1 << 28) + 5), slice(rows - 40, rows)):
+        within(y[part].double(), x[part].double() @ w.double().T,
+               least(torch.float16) + 2 * half_step(torch.float16) * (x[part].abs().double() @ w.abs().double().T))
+
+
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("device", ["cpu", GPU])
@@ -380,6 +391,21 @@ def test_norm_offsets_past_32_bits():
     y = ops.layer_norm(x)
     for rows in (slice(0, 4), slice(262140, 262148), slice(299996, 300000)):
         assert torch.equal(y[rows], ops.layer_norm(x[rows].clone()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [4, 8])
+def test_norm_rows_past_one_axis_of_a_launch(d):
+    rows = (1 << 26) + 77
+    x = torch.randn(rows, d, device="cuda", dtype=torch.float16)
+    x.requires_grad_()
+    y = ops.layer_norm(x)
+    dx, = torch.autograd.grad(y, x, x.detach())
+    for part in (slice(0, 5), slice((1 << 22) - 2, (1 << 22) + 2), slice(rows - 80, rows)):
+        few = x.detach()[part].clone().requires_grad_()
+        want = ops.layer_norm(few)
+        assert torch.equal(y.detach()[part], want.detach())
+        assert torch.equal(dx[part], torch.autograd.grad(want, few, few.detach())[0])
 
 
 def test_norm_gradients_by_differences():
@@ -613,6 +639,23 @@ def test_distill_offsets_past_32_bits():
     dx, = torch.autograd.grad(want.sum(), x64)
     within(loss.detach()[few], want.detach(), torch.full_like(want, U * (32 + v / 128 + 300)))
     within(grad[few], dx, U * 2000 * (dx.abs() + 1e-3))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_distill_rows_past_one_axis_of_a_launch(reduction):
+    rows, v = (1 << 26) + 77, 5
+    logits = torch.randn(rows, v, device="cuda", dtype=torch.float16).requires_grad_()
+    index = torch.randint(0, v, (rows, 1), device="cuda", dtype=torch.int32)
+    loss = ops.distill_loss(logits, index, reduction=reduction)
+    # an upstream gradient of other than 1 is written by the backward kernel
+    dx, = torch.autograd.grad(loss, logits, torch.full_like(loss, 2.0))
+    for part in (slice(0, 5), slice((1 << 24) - 3, (1 << 24) + 3), slice(rows - 80, rows)):
+        few = logits.detach()[part].clone().requires_grad_()
+        want = ops.distill_loss(few, index[part], reduction="none")
+        if reduction == "none":
+            assert torch.equal(loss.detach()[part], want.detach())
+        assert torch.equal(dx[part], torch.autograd.grad(want, few, torch.full_like(want, 2.0))[0])
 
 
 def test_distill_gradients_by_differences():
