@@ -105,6 +105,10 @@ def plan(name: str, *sizes) -> int:
     return entry(name)(*sizes)
 
 
+def autocast(device: torch.device) -> bool:
+    return device.type in ("cuda", "cpu") and torch.is_autocast_enabled(device.type)
+
+
 def needs_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 

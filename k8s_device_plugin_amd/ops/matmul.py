@@ -39,7 +39,7 @@ def linear(x, weight, bias=None, *, activation="none", residual=None):
         raise ValueError(f"bias {tuple(bias.shape)}, wanted ({n},)")
     if residual is not None and residual.shape != x.shape[:-1] + (n,):
         raise ValueError(f"residual {tuple(residual.shape)}, wanted {tuple(x.shape[:-1]) + (n,)}")
-    if torch.is_autocast_enabled(x.device.type):
+    if _native.autocast(x.device):
         dtype = torch.get_autocast_dtype(x.device.type)
         x, weight, bias, residual = (
             t if t is None or t.dtype == torch.float64 else t.to(dtype)

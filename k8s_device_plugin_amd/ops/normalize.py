@@ -34,7 +34,7 @@ def layer_norm(x, weight=None, bias=None, *, groups=1, eps=1e-5):
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and t.shape != (width,):
             raise ValueError(f"{name} {tuple(t.shape)}, wanted ({width},)")
-    if torch.is_autocast_enabled(x.device.type) and x.dtype != torch.float64:
+    if _native.autocast(x.device) and x.dtype != torch.float64:
         x, weight, bias = (t if t is None else t.float() for t in (x, weight, bias))
     kinds = {t.dtype for t in (weight, bias) if t is not None}
     if len(kinds) > 1 or not kinds <= {x.dtype, torch.float32}:

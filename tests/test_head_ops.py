@@ -811,6 +811,15 @@ def test_autocast_casts_as_torch_does():
 
 
 @pytest.mark.gpu
+def test_tensors_without_data():
+    x = torch.empty(3, 8, device="meta", requires_grad=True)
+    y = ops.linear(x, torch.empty(5, 8, device="meta"), activation="gelu")
+    assert y.shape == (3, 5) and y.device.type == "meta"
+    assert ops.layer_norm(x, groups=2).shape == (3, 8)
+    loss = ops.distill_loss(x, torch.empty(3, 2, dtype=torch.long, device="meta"))
+    assert torch.autograd.grad(loss, x)[0].shape == (3, 8)
+
+
 def test_traced_and_transformed_calls_run_the_formula():
     x, w = torch.randn(6, 64, device="cuda"), torch.randn(32, 64, device="cuda")
     y = ops.linear(x, w)
