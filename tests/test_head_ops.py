@@ -810,7 +810,6 @@ def test_autocast_casts_as_torch_does():
     assert w.grad.dtype == torch.float32
 
 
-@pytest.mark.gpu
 def test_tensors_without_data():
     x = torch.empty(3, 8, device="meta", requires_grad=True)
     y = ops.linear(x, torch.empty(5, 8, device="meta"), activation="gelu")
@@ -820,6 +819,7 @@ def test_tensors_without_data():
     assert torch.autograd.grad(loss, x)[0].shape == (3, 8)
 
 
+@pytest.mark.gpu
 def test_traced_and_transformed_calls_run_the_formula():
     x, w = torch.randn(6, 64, device="cuda"), torch.randn(32, 64, device="cuda")
     y = ops.linear(x, w)
