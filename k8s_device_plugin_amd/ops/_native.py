@@ -106,11 +106,16 @@ def plan(name: str, *sizes) -> int:
 
 
 def autocast(device: torch.device) -> bool:
-    return device.type in ("cuda", "cpu") and torch.is_autocast_enabled(device.type)
+    return (torch._C._is_any_autocast_enabled() and device.type in ("cuda", "cpu")
+            and torch.is_autocast_enabled(device.type))
 
 
 def needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
@@ -123,12 +128,13 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-def same_device(**tensors) -> None:
-    devices = {name: t.device for name, t in tensors.items() if t is not None}
-    one = next(iter(devices.values()))
-    if any(d != one for d in devices.values()):
-        raise ValueError("tensors on different devices: "
-                         + ", ".join(f"{n} on {d}" for n, d in devices.items()))
+def same_device(names: str, first, *others) -> None:
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError("tensors on different devices: " + ", ".join(
+                f"{n} on {t.device}" for n, t in zip(names.split(), (first, *others))
+                if t is not None))
 
 
 def gradients_of(plain, inputs, needed, grad):

@@ -67,7 +67,7 @@ def distill_loss(logits, index, teacher=None, *, temperature=1.0, reduction="mea
     top = index.shape[-1]
     if top > MOST_SLOTS:
         raise ValueError(f"{top} slots: at most {MOST_SLOTS}")
-    _native.same_device(logits=logits, index=index, teacher=teacher)
+    _native.same_device("logits index teacher", logits, index, teacher)
     if not _native.on_gpu(logits, index, teacher) or logits.numel() == 0 or top == 0:
         return _plain(logits, index, teacher, temperature, reduction, scale)
     for t in (logits, teacher):
@@ -122,39 +122,33 @@ def _forward(logits, index, teacher, temperature, reduction, scale, keep):
     chunks = _native.plan("distill_chunks", rows, v, 0)
     # one workgroup a row has it in registers when its gradient can be
     # written; few long rows are better cut in pieces, and wait for backward
-    dx = None
-    if keep and reduction and chunks == 1:
-        dx = logits.new_empty(logits.shape)
-    part = (torch.empty(rows * chunks * 2, dtype=torch.float32, device=device)
-            if chunks > 1 else None)
-    rows_loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=device)
-    loss = torch.empty((), dtype=torch.float32, device=device) if reduction else rows_loss
-    saved = torch.empty(rows * (4 + 2 * top if keep else 2) + (rows + 15) // 16,
+    dx = logits.new_empty(logits.shape) if keep and reduction and chunks == 1 else None
+    loss = torch.empty(() if reduction else logits.shape[:-1], dtype=torch.float32, device=device)
+    # behind what is kept: the rows' losses, where their sum is asked for, and
+    # the chunks' maxima and sums
+    kept = rows * (4 + 2 * top if keep else 2) + (rows + 15) // 16
+    saved = torch.empty(kept + (rows if reduction else 0) + (2 * rows * chunks if chunks > 1 else 0),
                         dtype=torch.float32, device=device)
-    a = _arguments(x, saved, rows, v, top, temperature, reduction, scale, chunks, keep)
-    a.index, a.ldi, a.index_bytes = i.data_ptr(), i.stride(0), i.element_size()
-    if t is not None:
-        a.teacher, a.ldt, a.ttype = t.data_ptr(), t.stride(0), DTYPES[t.dtype]
-    a.rows_loss, a.loss, a.part = rows_loss.data_ptr(), loss.data_ptr(), ptr(part)
-    if dx is not None:
-        a.dx, a.lddx = dx.data_ptr(), v
-    launch("distill", device, a)
+    at = saved.data_ptr() + 4 * kept
+    rows_loss = at if reduction else loss.data_ptr()
+    part = (at + (4 * rows if reduction else 0)) if chunks > 1 else None
+    launch("distill", device, DistillArgs(
+        x.data_ptr(), i.data_ptr(), ptr(t), ptr(dx), None, rows_loss,
+        *_rows(saved, rows, top, keep, loss.data_ptr()), part, x.stride(0), v, i.stride(0),
+        0 if t is None else t.stride(0), rows, v, DTYPES[x.dtype],
+        0 if t is None else DTYPES[t.dtype], i.element_size(), top, chunks, reduction, 0,
+        temperature, scale))
     return loss, saved, dx
 
 
-def _arguments(x, saved, rows, v, top, temperature, reduction, scale, chunks, keep):
-    a = DistillArgs(x=x.data_ptr(), ldx=x.stride(0), rows=rows, v=v, dtype=DTYPES[x.dtype], top=top,
-                    chunks=chunks, reduction=reduction, temperature=temperature, scale=scale,
-                    index_bytes=8)
-    row = 4 * rows
-    at = saved.data_ptr()
-    a.state, a.origin = at, at + row
-    at += 2 * row
-    if keep:
-        a.most, a.log_sum, a.slot_p, a.slot_i = at, at + row, at + 2 * row, at + (2 + top) * row
-        at += (2 + 2 * top) * row
-    a.counts = at
-    return a
+def _rows(saved, rows, top, keep, loss):
+    """Where the kernels find what is held of the rows; `state` to `slot_i`."""
+    at, row = saved.data_ptr(), 4 * rows
+    if not keep:
+        return at, at + row, None, None, None, loss, at + 2 * row, None
+    slots = at + 4 * row
+    end = slots + 2 * top * row
+    return at, at + row, at + 2 * row, at + 3 * row, slots, loss, end, slots + top * row
 
 
 class _Distill(torch.autograd.Function):
@@ -180,11 +174,12 @@ class _Distill(torch.autograd.Function):
         rows, v = x.shape
         grad = grad.contiguous()
         temperature, reduction, scale = ctx.how
-        a = _arguments(x, saved, rows, v, index.shape[-1], temperature, REDUCTIONS[reduction],
-                       scale, _native.plan("distill_chunks", rows, v, 1), True)
-        a.written = dx is not None
-        if dx is None:
+        top, written = index.shape[-1], dx is not None
+        if not written:
             dx = logits.new_empty(logits.shape)
-        a.dx, a.lddx, a.grad = dx.data_ptr(), v, grad.data_ptr()
-        launch("distill", logits.device, a)
+        launch("distill", logits.device, DistillArgs(
+            x.data_ptr(), None, None, dx.data_ptr(), grad.data_ptr(), None,
+            *_rows(saved, rows, top, True, None), None, x.stride(0), v, 0, 0, rows, v,
+            DTYPES[x.dtype], 0, 8, top, _native.plan("distill_chunks", rows, v, 1),
+            REDUCTIONS[reduction], written, temperature, scale))
         return dx, None, None, None, None, None

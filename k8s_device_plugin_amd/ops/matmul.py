@@ -47,7 +47,7 @@ def linear(x, weight, bias=None, *, activation="none", residual=None):
     for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
         if t is not None and t.dtype != x.dtype:
             raise TypeError(f"{name} is {t.dtype}, x {x.dtype}")
-    _native.same_device(x=x, weight=weight, bias=bias, residual=residual)
+    _native.same_device("x weight bias residual", x, weight, bias, residual)
     if not _native.on_gpu(x, weight, bias, residual):
         return formula(x, weight, bias, residual, activation)
     if x.dtype not in DTYPES:
@@ -91,12 +91,13 @@ def _forward(x, weight, bias, residual, act, keep):
     it, or, where y tells as much (relu without a residual), y itself."""
     n, k = weight.shape
     x2 = _matrix(x, k)
-    y = x.new_empty(x.shape[:-1] + (n,))
+    shape = (x2.shape[0], n) if x.dim() == 2 else x.shape[:-1] + (n,)
+    y = x.new_empty(shape)
     z = None
     if keep and act and not (act == RELU and residual is None):
         # rounded like y: the slope is taken where a separate layer would
         # have stored its input
-        z = x.new_empty(y.shape)
+        z = x.new_empty(shape)
     if bias is not None and n > 1 and bias.stride(0) != 1:
         bias = bias.contiguous()
     r2 = None if residual is None else rows_of(residual, n)

@@ -36,10 +36,11 @@ def layer_norm(x, weight=None, bias=None, *, groups=1, eps=1e-5):
             raise ValueError(f"{name} {tuple(t.shape)}, wanted ({width},)")
     if _native.autocast(x.device) and x.dtype != torch.float64:
         x, weight, bias = (t if t is None else t.float() for t in (x, weight, bias))
-    kinds = {t.dtype for t in (weight, bias) if t is not None}
-    if len(kinds) > 1 or not kinds <= {x.dtype, torch.float32}:
+    kind = _kind(x, weight, bias)
+    if kind not in (x.dtype, torch.float32) or (bias is not None and bias.dtype != kind):
+        kinds = {t.dtype for t in (weight, bias) if t is not None}
         raise TypeError(f"weight and bias are {kinds}: wanted both {x.dtype} or both float32")
-    _native.same_device(x=x, weight=weight, bias=bias)
+    _native.same_device("x weight bias", x, weight, bias)
     if not _native.on_gpu(x, weight, bias):
         return _plain(x, weight, bias, groups, eps)
     if x.dtype not in DTYPES:
@@ -65,7 +66,11 @@ def _plain(x, weight, bias, groups, eps):
 
 
 def _vector(t):
-    return t if t is None or t.numel() == 1 or t.stride(0) == 1 else t.contiguous()
+    return t if t is None or t.stride(0) == 1 or t.numel() == 1 else t.contiguous()
+
+
+def _kind(x, weight, bias):
+    return weight.dtype if weight is not None else x.dtype if bias is None else bias.dtype
 
 
 def _forward(x, weight, bias, groups, eps, keep):
@@ -76,7 +81,7 @@ def _forward(x, weight, bias, groups, eps, keep):
     stats = (torch.empty((2, rows * groups), dtype=torch.float32, device=x.device)
              if keep else None)
     weight, bias = _vector(weight), _vector(bias)
-    kind = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
+    kind = _kind(x, weight, bias)
     at = ptr(stats)
     launch("norm", x.device, NormArgs(
         x2.data_ptr(), ptr(weight), ptr(bias), None, y.data_ptr(), None, None, None,
@@ -111,7 +116,7 @@ class _LayerNorm(torch.autograd.Function):
         parts = _native.plan("norm_parts", rows, groups, d)
         part = (torch.empty(2 * parts * width, dtype=torch.float32, device=x.device)
                 if parts > 1 and (need_w or need_b) else None)
-        kind = next((t.dtype for t in (weight, bias) if t is not None), x.dtype)
+        kind = _kind(x, weight, bias)
         weight = _vector(weight)
         launch("norm", x.device, NormArgs(
             x2.data_ptr(), ptr(weight), None, dy2.data_ptr(), None, ptr(dx), ptr(dw), ptr(db),

@@ -810,6 +810,21 @@ def test_autocast_casts_as_torch_does():
     assert w.grad.dtype == torch.float32
 
 
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_results_may_be_changed_in_place(device):
+    x, w = normal(seeded(), 2, 3, 8, device=device), normal(seeded(1), 6, 8, device=device)
+    for act, residual in (("none", False), ("gelu", True)):
+        r = torch.ones(2, 3, 6, device=device) if residual else None
+        lead, flat = x.clone().requires_grad_(), x.flatten(0, 1).requires_grad_()
+        y = ops.linear(lead, w, activation=act, residual=r).mul_(2)
+        z = ops.linear(flat, w, activation=act, residual=None if r is None else r.flatten(0, 1)) * 2
+        assert torch.equal(y.flatten(0, 1), z)
+        y.sum().backward(), z.sum().backward()
+        assert torch.equal(lead.grad.flatten(0, 1), flat.grad)
+    lead = x.clone().requires_grad_()
+    ops.layer_norm(lead).mul_(2).sum().backward()
+
+
 def test_tensors_without_data():
     x = torch.empty(3, 8, device="meta", requires_grad=True)
     y = ops.linear(x, torch.empty(5, 8, device="meta"), activation="gelu")
