@@ -11,7 +11,9 @@ A from-scratch AMD MI355X (gfx950 / CDNA4) re-design of the capabilities of
 - ``monitor``    : node sidecar exporting Prometheus metrics from the
                    per-container shared-memory regions and writing back
                    priority/blocking feedback.
-- ``ops``        : ctypes bindings for the native enforcement library
+- ``ops``        : CU masks, the operators that the zoo's models end in
+                   (``libvgpu_ops.so``, gfx950 kernels) and
+                   ctypes bindings for the native enforcement library
                    ``libvgpu-hip.so`` (LD_PRELOAD HIP interceptor, C).
 - ``parallel``   : xGMI / NUMA topology discovery from KFD for
                    topology-aware placement.

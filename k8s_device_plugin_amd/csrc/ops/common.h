@@ -217,8 +217,9 @@ struct NormArgs {
 };
 
 /* Distillation from a teacher's top logits.  rows_loss, state, origin, most
- * and log_sum hold one value a row, slot_p and slot_i `top` values a row, part 2 x chunks a row;
- * counts holds, for each 16 rows, how many of them have a target. */
+ * and log_sum hold one value a row, slot_p and slot_i `top` values a row, part
+ * 2 x chunks a row; counts holds, for each 16 rows, how many of them have a
+ * target. */
 struct DistillArgs {
   const void *x, *index, *teacher;
   void *dx;

