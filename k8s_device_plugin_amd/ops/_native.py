@@ -11,6 +11,7 @@ from functools import lru_cache
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 PACKAGE = Path(__file__).resolve().parent.parent
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -59,12 +60,17 @@ def library() -> ctypes.CDLL:
 
 def on_gpu(*tensors) -> bool:
     """Whether the kernels run: ordinary tensors on a GPU, and nothing that
-    traces or transforms the call.  Otherwise the plain formula runs."""
+    traces or transforms the call.  Otherwise the plain formula runs: so too
+    for tensors whose sign is still to be turned, as conj()'s imaginary part,
+    and inside forward-mode differentiation."""
+    if torch.compiler.is_compiling():
+        return False
     for t in tensors:
-        if t is not None and (type(t) not in _PLAIN_TENSORS or not t.is_cuda):
+        if t is not None and (type(t) not in _PLAIN_TENSORS or not t.is_cuda or t.is_neg()):
             return False
-    return not (torch.compiler.is_compiling() or torch._C._get_tracing_state() is not None
-                or torch._C._are_functorch_transforms_active())
+    return not (torch._C._get_tracing_state() is not None
+                or torch._C._are_functorch_transforms_active()
+                or forward_ad._current_level >= 0)
 
 
 _entries = {}   # name -> bound function

@@ -174,7 +174,7 @@ class _Distill(torch.autograd.Function):
             return (*found, None, None, None, None, None)
         x = rows_of(logits, logits.shape[-1])
         rows, v = x.shape
-        grad = grad.contiguous()
+        grad = grad.resolve_neg().contiguous()
         temperature, reduction, scale = ctx.how
         top, written = index.shape[-1], dx is not None
         if not written:

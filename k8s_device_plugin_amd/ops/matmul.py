@@ -127,7 +127,7 @@ class _Linear(torch.autograd.Function):
                 (need_x, need_w, need_b), dy)
             return (*found, dr, None)
         n, k = weight.shape
-        x2, dy2 = _matrix(x, k), rows_of(dy, n)
+        x2, dy2 = _matrix(x, k), rows_of(dy.resolve_neg(), n)
         dx = x.new_empty(x.shape) if need_x else None
         dw = x.new_empty((n, k)) if need_w else None
         db = x.new_empty(n) if need_b else None

@@ -108,7 +108,7 @@ class _LayerNorm(torch.autograd.Function):
                 lambda x, w, b: _plain(x, w, b, groups, ctx.eps), (x, weight, bias),
                 (need_x, need_w, need_b), dy), None, None)
         width = x.shape[-1]
-        x2, dy2 = rows_of(x, width), rows_of(dy, width)
+        x2, dy2 = rows_of(x, width), rows_of(dy.resolve_neg(), width)
         rows, d = x2.shape[0], width // groups
         dx = x.new_empty(x.shape) if need_x else None
         dw = weight.new_empty(width) if need_w else None

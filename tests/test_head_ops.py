@@ -834,6 +834,84 @@ def test_tensors_without_data():
     assert torch.autograd.grad(loss, x)[0].shape == (3, 8)
 
 
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_sign_that_is_still_to_be_turned(device):
+    turned = torch.randn(4, 8, 2, device=device).view(4, 16)
+    turned = torch.view_as_complex(turned.view(4, 8, 2)).conj().imag
+    assert turned.is_neg()
+    plain = turned.resolve_neg()
+    w = torch.randn(6, 8, device=device)
+    index = torch.zeros(4, 1, dtype=torch.long, device=device)
+    bound = 64 * U  # a sum of 8 terms of ordinary size, either way
+    for f in (lambda t: ops.linear(t, w), ops.layer_norm,
+              lambda t: ops.distill_loss(t, index, reduction="none")):
+        assert (f(turned) - f(plain)).abs().max() <= bound
+    for f in (lambda t: ops.linear(t, w), ops.layer_norm):
+        x = plain.clone().requires_grad_()
+        y = f(x)
+        up = torch.view_as_complex(torch.randn(*y.shape, 2, device=device)).conj().imag
+        a, = torch.autograd.grad(y, x, up, retain_graph=True)
+        b, = torch.autograd.grad(y, x, up.resolve_neg())
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_forward_mode_runs_the_formula(device):
+    x, v = (torch.randn(3, 8, device=device) for _ in range(2))
+    w = torch.randn(6, 8, device=device)
+    index = torch.zeros(3, 1, dtype=torch.long, device=device)
+    for f in (lambda t: ops.linear(t, w, activation="silu"), ops.layer_norm,
+              lambda t: ops.distill_loss(t, index)):
+        with torch.autograd.forward_ad.dual_level():
+            y = f(torch.autograd.forward_ad.make_dual(x, v))
+            got = torch.autograd.forward_ad.unpack_dual(y).tangent
+        assert got is not None
+        leaf = x.clone().requires_grad_()
+        z = f(leaf)
+        up = torch.randn_like(z)
+        back, = torch.autograd.grad(z, leaf, up)
+        # both are up^T J v: sums of fewer than 32 terms of ordinary size
+        assert abs((got * up).sum() - (back * v).sum()) <= 1e-3
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_compiled_calls_run_the_formula(device):
+    x, w = torch.randn(6, 8, device=device), torch.randn(5, 8, device=device)
+    index = torch.zeros(6, 1, dtype=torch.long, device=device)
+
+    def f(x):
+        return ops.linear(x, w, activation="gelu"), ops.layer_norm(x), ops.distill_loss(x, index)
+
+    for got, want in zip(torch.compile(f, backend="eager", fullgraph=True)(x), f(x)):
+        assert (got - want).abs().max() <= 64 * U
+
+
+CAPTURED_FIRST = """
+import torch
+from k8s_device_plugin_amd import ops
+x, w = torch.randn(5, 64, device="cuda"), torch.randn(40, 64, device="cuda")
+index = torch.zeros(5, 1, dtype=torch.long, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = ops.layer_norm(ops.linear(x, w))
+    loss = ops.distill_loss(y, index)
+for _ in range(3):
+    x.normal_()
+    graph.replay()
+    want = ops.layer_norm(ops.linear(x, w))
+    assert torch.equal(y, want) and torch.equal(loss, ops.distill_loss(want, index))
+    torch.cuda.synchronize()
+print("same")
+"""
+
+
+@pytest.mark.gpu
+def test_first_call_of_a_process_may_be_captured():
+    out = subprocess.run([sys.executable, "-c", CAPTURED_FIRST], cwd=REPO, capture_output=True,
+                         text=True, timeout=100)
+    assert out.returncode == 0 and "same" in out.stdout, out.stderr[-2000:]
+
+
 @pytest.mark.gpu
 def test_traced_and_transformed_calls_run_the_formula():
     x, w = torch.randn(6, 64, device="cuda"), torch.randn(32, 64, device="cuda")
