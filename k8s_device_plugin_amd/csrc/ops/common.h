@@ -177,8 +177,9 @@ struct GemmArgs {
   int32_t plan, splits;
 };
 
-/* dz = dy act'(z) into rows of lddz elements with zeros behind n, and, in
- * part [parts, n], sums of dz's columns over runs of rows. */
+/* dz = dy act'(z) into rows of lddz elements with zeros behind n, and dbias,
+ * the sums of dz's columns, by way of sums over runs of rows in part [parts, n]
+ * where there is more than one run. */
 struct SlopeArgs {
   const void *dy, *z;
   void *dz, *dbias;

@@ -699,7 +699,7 @@ __global__ __launch_bounds__(256) void slope_rows(SlopeArgs p) {
     for (int e = 0; e < V; e++) sum[e] += g[e];
     if (dz && col < p.lddz) store_vec<T>(dz + r * p.lddz + col, (int)min((int64_t)V, p.lddz - col), g);
   }
-  if (!p.part) return;
+  if (!p.dbias) return;
   if (wave)
 #pragma unroll
     for (int e = 0; e < V; e++) lds[wave - 1][lane][e] = sum[e];
@@ -708,6 +708,10 @@ __global__ __launch_bounds__(256) void slope_rows(SlopeArgs p) {
 #pragma unroll
   for (int e = 0; e < V; e++)
     for (int w = 0; w < 3; w++) sum[e] += lds[w][lane][e];
+  if (p.parts == 1) {
+    store_vec<T>((T *)p.dbias + col, n, sum);
+    return;
+  }
   float *part = p.part + blockIdx.y * p.n + col;
 #pragma unroll
   for (int e = 0; e < V; e++)
@@ -723,7 +727,7 @@ template <typename T>
 int run_slope(const SlopeArgs &p, hipStream_t s) {
   int64_t vecs = (std::max(p.n, p.dz ? p.lddz : p.n) + Vec<T>::N - 1) / Vec<T>::N;
   slope_rows<T><<<dim3((unsigned)((vecs + 63) / 64), (unsigned)p.parts), 256, 0, s>>>(p);
-  if (p.part) slope_join<T><<<(unsigned)((p.n + 63) / 64), 1024, 0, s>>>(p);
+  if (p.dbias && p.parts > 1) slope_join<T><<<(unsigned)((p.n + 63) / 64), 1024, 0, s>>>(p);
   return OPS_LAUNCHED();
 }
 

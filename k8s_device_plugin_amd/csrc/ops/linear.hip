@@ -228,11 +228,12 @@ struct Call {
       s.dy = p.dy, s.z = p.z, s.lddy = p.lddy, s.ldz = p.n, s.m = p.m, s.n = p.n;
       s.dtype = dtype, s.act = p.act, s.lddz = padded(p.n), s.dbias = p.db;
       /* runs of rows for the columns' sums: about four workgroups a CU, and at
-       * least 8 rows each */
+       * least 8 rows each; up to 16 rows need no second launch */
       int64_t blocks = (s.lddz * size + 1023) / 1024;
       s.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>((p.m + 7) / 8, 1024 / blocks));
+      if (p.m <= 16) s.parts = 1;
       if (copy) s.dz = take(p.m * s.lddz * size);
-      if (p.db) s.part = (float *)take(s.parts * p.n * 4);
+      if (p.db && s.parts > 1) s.part = (float *)take(s.parts * p.n * 4);
       if (copy) dz = {s.dz, p.m, s.lddz, s.lddz, 1};
       launch([&] { return launch_slope(s, stream); });
     }
