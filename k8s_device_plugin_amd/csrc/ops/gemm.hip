@@ -142,13 +142,23 @@ struct Tile {
       off[i] = (r + i * ROWS) * (uint32_t)(ld * sizeof(T)) + (c ^ spread(r + i * ROWS)) * 16;
   }
 
-  /* One of a stage's loads.  What lies past the operand's end comes as zeros:
-   * with k strided that is all past the end of k, with k contiguous chunks
-   * past it are asked for there.  Rows past m or n only feed results that are
+  /* One of a stage's loads.  What lies past the operand's end comes as zeros,
+   * dword by dword: with k strided that is all past the end of k, with k
+   * contiguous chunks past it are asked for there.  Rows past m or n only feed results that are
    * not stored. */
   template <int I>
   __device__ void load(u32x4 from, int k_left, uint32_t lds) const {
     load16_to_lds<I * THREADS * 16>(from, !KC || kpos < k_left ? off[I] : OUT_OF_RANGE, lds);
+  }
+
+  /* Where k, which is contiguous, ends inside a chunk: zeros behind, instead
+   * of what follows the row in memory.  `left` of the stage's k are there. */
+  static __device__ void trim(char *lds, int left) {
+    for (int r = threadIdx.x; r < R; r += THREADS) {
+      T *q = (T *)(lds + r * STAGE + (left / E ^ spread(r)) * 16);
+#pragma unroll 1
+      for (int e = left % E; e < E; e++) q[e] = T(0);
+    }
   }
 
   /* The fragment of rows row0 .. row0+15 at one of the stage's steps. */
@@ -385,6 +395,15 @@ __global__ __launch_bounds__(WR *WC * 64, TM == 256 ? 1 : 2) void gemm_tile(Gemm
       __builtin_amdgcn_sched_barrier(0);
     });
   };
+  /* the stage in which k ends inside a chunk */
+  int ragged = p.k % TA::E ? stages_all - 1 : -1;
+  auto trim = [&](int s, char *at) {
+    if (s != ragged) return;
+    int left = (int)(p.k - (int64_t)s * BK);
+    if (AKC) TA::trim(at, left);
+    if (BKC) TB::trim(at + TA::BYTES, left);
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
   int buffer = 0;
   /* the stage whose first step is in `now`; leaves the next one's there */
   auto stage = [&](int s, Step &now, Step &then) {
@@ -393,6 +412,7 @@ __global__ __launch_bounds__(WR *WC * 64, TM == 256 ? 1 : 2) void gemm_tile(Gemm
     Source q = source(s + BUFFERS);
     step(now, then, lds + at * BYTES, 1, nullptr, 0);
     land_and_meet<(BUFFERS - 2) * LOADS>();
+    if constexpr (AKC || BKC) trim(s + 1, lds + buffer * BYTES);
     step(then, now, lds + buffer * BYTES, 0, &q, at);
   };
 
@@ -402,6 +422,7 @@ __global__ __launch_bounds__(WR *WC * 64, TM == 256 ? 1 : 2) void gemm_tile(Gemm
     each<LOADS>([&](auto f) { load(f, q, i); });
   }
   land_and_meet<(BUFFERS - 1) * LOADS>();
+  if constexpr (AKC || BKC) trim(s0, lds);
 #pragma unroll
   for (int f = 0; f < FRAGS; f++) read(f, even, lds, 0);
   if constexpr (PINNED) settle(acc);
@@ -518,7 +539,7 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
     u32x4 a, b[LOADS];
   };
   auto fetch = [&](Step &q, int64_t s) {
-    bool in = s < s1 && (s * 4 + g) * V < p.k; /* k ends on a whole chunk of a */
+    bool in = s < s1 && (s * 4 + g) * V < p.k;
     uint32_t at = (uint32_t)(s * 64);
     q.a = load16(ra, in ? a_off + at : OUT_OF_RANGE);
     int64_t skip = BKC ? 0 : s * 4 * V * p.ldb * (int64_t)sizeof(T);
@@ -529,12 +550,22 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
   };
 
   f32x4 acc[FN] = {};
-  auto multiply = [&](const Step &q) {
+  int ragged = (int)(p.k % V); /* values of a chunk in which k ends */
+  int64_t last = p.k / V;
+  auto multiply = [&](const Step &q, int64_t s) {
     Frag<T> fa, fb[FN];
     fa.v = __builtin_bit_cast(vec, q.a);
-    if constexpr (BKC) {
-      fb[0].v = __builtin_bit_cast(vec, q.b[0]);
-    } else {
+    if constexpr (BKC) fb[0].v = __builtin_bit_cast(vec, q.b[0]);
+    if (ragged && s == last / 4) { /* zeros behind it, not what follows the row */
+      bool here = g == (int)(last % 4);
+#pragma unroll
+      for (int e = 1; e < V; e++)
+        if (here && e >= ragged) {
+          fa.v[e] = T(0);
+          if (BKC) fb[0].v[e] = T(0);
+        }
+    }
+    if constexpr (!BKC) {
       vec r[V];
 #pragma unroll
       for (int t = 0; t < V; t++) r[t] = __builtin_bit_cast(vec, q.b[t]);
@@ -554,7 +585,7 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
     for (int c = 0; c < C; c++) fetch(then[c], s + WAVES * C + c);
     __builtin_amdgcn_sched_barrier(0); /* the loads go out before the products */
 #pragma unroll
-    for (int c = 0; c < C; c++) multiply(now[c]);
+    for (int c = 0; c < C; c++) multiply(now[c], s + c);
     __builtin_amdgcn_sched_barrier(0);
   };
   int64_t s = s0 + wave * C;

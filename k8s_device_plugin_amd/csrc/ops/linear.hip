@@ -149,35 +149,33 @@ struct Call {
   }
   int64_t padded(int64_t n) const { return (n * size + 15) / 16 * 16 / size; }
 
-  /* Loads are 16 bytes wide, so rows that do not start on 16 bytes, or whose k
-   * ends inside 16, are laid out anew with zeros behind; so is a matrix that
-   * is contiguous along neither axis, or not along k where any_axis is false. */
+  static int64_t dwords(int64_t bytes) { return (bytes + 3) / 4 * 4; }
+
+  /* Loads take dwords, and are cut off at the extent dword by dword, so rows
+   * that do not start on 4 bytes are laid out anew; so is a matrix that is
+   * contiguous along neither axis, or not along k where any_axis is false. */
   Operand prepare(Matrix t, bool any_axis) {
-    bool aligned = (uintptr_t)t.p % 16 == 0;
-    if (t.rows == 1 && t.s1 == 1) t.s0 = t.k;
-    if (aligned && t.s1 == 1 && t.k * size % 16 == 0 && t.s0 * size % 16 == 0 &&
-        t.s0 * size < LONGEST)
-      return {t.p, t.s0, ((t.rows - 1) * t.s0 + t.k) * size, t.k, true};
-    if (aligned && any_axis && t.s0 == 1 && t.s1 >= t.rows && t.s1 * size % 16 == 0 &&
-        t.s1 * size < LONGEST)
-      /* the last row's last load is whole: its 16 bytes are one line's */
-      return {t.p, t.s1, (((t.k - 1) * t.s1 + t.rows) * size + 15) / 16 * 16, t.k, false};
-    bool along = any_axis && t.s0 == 1 && t.s1 != 1 && padded(t.rows) * size < LONGEST;
+    bool aligned = (uintptr_t)t.p % 4 == 0;
+    if (t.rows == 1 && t.s1 == 1) t.s0 = dwords(t.k * size) / size;
+    if (aligned && t.s1 == 1 && t.s0 * size % 4 == 0 && t.s0 * size <= LONGEST)
+      return {t.p, t.s0, dwords(((t.rows - 1) * t.s0 + t.k) * size), t.k, true};
+    if (aligned && any_axis && t.s0 == 1 && t.s1 >= t.rows && t.s1 * size % 4 == 0 &&
+        t.s1 * size <= LONGEST)
+      return {t.p, t.s1, dwords(((t.k - 1) * t.s1 + t.rows) * size), t.k, false};
+    bool along = any_axis && t.s0 == 1 && t.s1 != 1 && padded(t.rows) * size <= LONGEST;
     int64_t rows = along ? t.k : t.rows, cols = along ? t.rows : t.k, ld = padded(cols);
-    if (ld * size >= LONGEST) code = OPS_TOO_LONG;
+    if (ld * size > LONGEST) code = OPS_TOO_LONG;
     void *to = take(rows * ld * size);
     launch([&] {
       return launch_repack(t.p, along ? t.s1 : t.s0, along ? t.s0 : t.s1, rows, cols, to, ld, size,
                            stream);
     });
-    return {to, ld, rows * ld * size, along ? t.k : ld, !along};
+    return {to, ld, rows * ld * size, t.k, !along};
   }
 
   /* out [m,n] = a b^T; `out` says where to and with what epilogue. */
   void product(const Operand &a, const Operand &b, int64_t m, int64_t n, GemmArgs out) {
-    /* a k that one side pads with zeros ends beyond the other's extent, which
-     * reads as zeros there too */
-    int64_t k = std::max(a.k, b.k);
+    int64_t k = a.k;
     bool bare = !out.bias && !out.res && !out.z && out.act == ACT_NONE;
     Plan p = planned(m, n, k, size, a.kc, b.kc, bare);
     if (p.plan == 0 && tiles_of(0, p.rows, n) > MOST_TILES) code = OPS_TOO_LONG;
@@ -221,8 +219,7 @@ struct Call {
   void backward(const LinearArgs &p) {
     Matrix dz = {p.dy, p.m, p.n, p.lddy, 1};
     /* rows of dy that the loads do not allow are copied along with the slope */
-    bool copy = (p.dx || p.dw) && (p.act != ACT_NONE || p.n * size % 16 || p.lddy * size % 16 ||
-                                   (uintptr_t)p.dy % 16);
+    bool copy = (p.dx || p.dw) && (p.act != ACT_NONE || p.lddy * size % 4 || (uintptr_t)p.dy % 4);
     if (p.db || copy) {
       SlopeArgs s = {};
       s.dy = p.dy, s.z = p.z, s.lddy = p.lddy, s.ldz = p.n, s.m = p.m, s.n = p.n;
@@ -234,7 +231,7 @@ struct Call {
       if (p.m <= 16) s.parts = 1;
       if (copy) s.dz = take(p.m * s.lddz * size);
       if (p.db && s.parts > 1) s.part = (float *)take(s.parts * p.n * 4);
-      if (copy) dz = {s.dz, p.m, s.lddz, s.lddz, 1};
+      if (copy) dz = {s.dz, p.m, p.n, s.lddz, 1};
       launch([&] { return launch_slope(s, stream); });
     }
     if (p.dx) {

@@ -936,7 +936,7 @@ def test_bad_calls_of_the_library_are_refused():
         return lib.vgpu_ops_linear(ctypes.byref(n.LinearArgs(**{**a, **how})), None)
 
     for how in (dict(m=0), dict(n=-1), dict(k=0), dict(dtype=3), dict(act=4), dict(xs0=-4),
-                dict(y=None), dict(w=None), dict(dy=at, act=1), dict(x=at + 4)):
+                dict(y=None), dict(w=None), dict(dy=at, act=1), dict(xs1=2)):
         assert linear(**how) < 0, how  # the last: a workspace is wanted
 
     def norm(**how):
