@@ -503,10 +503,11 @@ __global__ __launch_bounds__(256) void gemm_join(GemmArgs p) {
  * k strided: the strip is 16 lanes by 16 bytes of n, a step 4 V rows of k;
  * lane i holds V neighbouring columns, of which the j-th go to the j-th
  * product, so 16-bit values are only turned inside a lane.
+ * LOOSE: rows of 16-bit values that start on 2 bytes, by loads that may.
  *
  * Bound by reading b.  1 x 4096 -> 4096 bf16: 8.9 us with b out of the cache;
  * 2 x 25088 -> 4096 fp32: 93 us, 4.4 TB/s, and with k strided 76 us, 5.4 TB/s. */
-template <typename T, bool BKC>
+template <typename T, bool BKC, bool LOOSE>
 __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
   constexpr int V = Vec<T>::N, WAVES = 8;
   constexpr int FN = BKC ? 1 : V;    /* products a step */
@@ -542,6 +543,12 @@ __global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
     bool in = s < s1 && (s * 4 + g) * V < p.k;
     uint32_t at = (uint32_t)(s * 64);
     q.a = load16(ra, in ? a_off + at : OUT_OF_RANGE);
+    if constexpr (LOOSE) {
+      int64_t k = (s * 4 + g) * V;
+      int n = in && n0 + i < p.n ? (int)min((int64_t)V, p.k - k) : 0;
+      q.b[0] = __builtin_bit_cast(u32x4, load_raw<T>((const T *)b + i * p.ldb + k, n));
+      return;
+    }
     int64_t skip = BKC ? 0 : s * 4 * V * p.ldb * (int64_t)sizeof(T);
     u32x4 rb = window(b + skip, b_left - skip);
 #pragma unroll
@@ -650,11 +657,11 @@ __global__ __launch_bounds__(256) void gemm_outer(GemmArgs p) {
   }
 }
 
-template <typename T, bool BKC>
+template <typename T, bool BKC, bool LOOSE>
 void launch_rows(const GemmArgs &p, hipStream_t stream) {
   constexpr int STRIP = BKC ? 16 : 16 * Vec<T>::N;
   dim3 grid((unsigned)((p.n + STRIP - 1) / STRIP), (unsigned)p.splits);
-  gemm_rows<T, BKC><<<grid, 512, 0, stream>>>(p);
+  gemm_rows<T, BKC, LOOSE><<<grid, 512, 0, stream>>>(p);
 }
 
 template <typename T, bool AKC, bool BKC>
@@ -673,6 +680,15 @@ void launch_tile(const GemmArgs &p, hipStream_t stream) {
 }
 
 template <typename T>
+int join(const GemmArgs &p, hipStream_t stream) {
+  if (p.splits > 1) {
+    int64_t items = p.m * ((p.n + 3) / 4);
+    gemm_join<T><<<(unsigned)((items + 255) / 256), 256, 0, stream>>>(p);
+  }
+  return OPS_LAUNCHED();
+}
+
+template <typename T>
 int run(const GemmArgs &p, hipStream_t stream) {
   if (p.plan == PLAN_OUTER) {
     dim3 grid((unsigned)((p.n + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N)),
@@ -680,17 +696,20 @@ int run(const GemmArgs &p, hipStream_t stream) {
     gemm_outer<T><<<grid, 256, 0, stream>>>(p);
     return OPS_LAUNCHED();
   }
-  if (p.plan == PLAN_ROWS && p.b_kc) launch_rows<T, true>(p, stream);
-  else if (p.plan == PLAN_ROWS) launch_rows<T, false>(p, stream);
+  if (p.plan == PLAN_ROWS && p.b_kc) {
+    if constexpr (sizeof(T) == 2)
+      if ((uintptr_t)p.b % 4 || p.ldb % 2) {
+        launch_rows<T, true, true>(p, stream);
+        return join<T>(p, stream);
+      }
+    launch_rows<T, true, false>(p, stream);
+  }
+  else if (p.plan == PLAN_ROWS) launch_rows<T, false, false>(p, stream);
   else if (p.a_kc && p.b_kc) launch_tile<T, true, true>(p, stream);
   else if (p.a_kc) launch_tile<T, true, false>(p, stream);
   else if (p.b_kc) launch_tile<T, false, true>(p, stream);
   else launch_tile<T, false, false>(p, stream);
-  if (p.splits > 1) {
-    int64_t items = p.m * ((p.n + 3) / 4);
-    gemm_join<T><<<(unsigned)((items + 255) / 256), 256, 0, stream>>>(p);
-  }
-  return OPS_LAUNCHED();
+  return join<T>(p, stream);
 }
 
 /* The bits of [rows, cols] of any strides to rows of `ld` elements, zeros
@@ -701,6 +720,21 @@ __global__ __launch_bounds__(256) void repack(const T *src, int64_t rs, int64_t 
   for (int64_t r = blockIdx.y; r < rows; r += gridDim.y)
     for (int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x; c < ld; c += (int64_t)gridDim.x * 256)
       dst[r * ld + c] = c < cols ? src[r * rs + c * cs] : T(0);
+}
+
+/* The same of rows that are contiguous, in loads of 16 bytes that start on any
+ * element: a thread a chunk, 2^shift chunks of a row beside each other in a
+ * workgroup.  Bound by memory: 8001 x 20001 16-bit values 102 us, 6.3 TB/s. */
+template <typename T>
+__global__ __launch_bounds__(256) void repack_rows(const T *src, int64_t rs, int64_t rows,
+                                                   int64_t cols, T *dst, int64_t ld, int shift) {
+  constexpr int V = Vec<T>::N;
+  int64_t c = (((int64_t)blockIdx.x << shift) + (threadIdx.x & ((1 << shift) - 1))) * V;
+  int64_t at_once = 256 >> shift;
+  if (c >= ld) return;
+  int n = (int)min((int64_t)V, cols - c);
+  for (int64_t r = blockIdx.y * at_once + (threadIdx.x >> shift); r < rows; r += gridDim.y * at_once)
+    *(typename Vec<T>::type *)(dst + r * ld + c) = load_raw<T>(src + r * rs + c, n);
 }
 
 /* dz = dy act'(z) and the columns' sums in one pass over dy and z, which bounds
@@ -778,6 +812,19 @@ int launch_gemm(const GemmArgs &p, hipStream_t s) {
 
 int launch_repack(const void *src, int64_t rs, int64_t cs, int64_t rows, int64_t cols, void *dst,
                   int64_t ld, int size, hipStream_t s) {
+  if (cs == 1) {
+    int64_t chunks = ld * size / 16;
+    int shift = 0;
+    while (shift < 8 && (int64_t)1 << shift < chunks) shift++;
+    int64_t blocks = (rows + (256 >> shift) - 1) / (256 >> shift);
+    dim3 grid((unsigned)((chunks + ((int64_t)1 << shift) - 1) >> shift),
+              (unsigned)std::min<int64_t>(blocks, 16384));
+    if (size == 4)
+      repack_rows<<<grid, 256, 0, s>>>((const uint32_t *)src, rs, rows, cols, (uint32_t *)dst, ld, shift);
+    else
+      repack_rows<<<grid, 256, 0, s>>>((const uint16_t *)src, rs, rows, cols, (uint16_t *)dst, ld, shift);
+    return OPS_LAUNCHED();
+  }
   dim3 grid((unsigned)std::min<int64_t>((ld + 255) / 256, 1024),
             (unsigned)std::min<int64_t>(rows, 16384));
   if (size == 4)

@@ -69,7 +69,7 @@ struct Plan {
   int64_t rows;
 };
 
-Plan choose(int64_t m, int64_t n, int64_t k, int size, bool a_kc, bool b_kc, bool bare) {
+Plan choose(int64_t m, int64_t n, int64_t k, int size, bool a_kc, bool b_kc, bool bare, bool odd) {
   Plan p = {0, 1, m};
   if (k <= OUTER_K && !a_kc && !b_kc && bare && m <= 65535 * 4 * OUTER_ROWS) {
     p.plan = PLAN_OUTER;
@@ -81,8 +81,10 @@ Plan choose(int64_t m, int64_t n, int64_t k, int size, bool a_kc, bool b_kc, boo
    * out of the cache: 1 x 4096 x 4096 bf16 12.3 and 15.8; 1 x 50000 -> 4096
    * bf16 71 and 81; 16 of them 115 and 85; 1 x 4096 -> 50000 bf16 90 and 82.
    * With k strided in b, 8 rows fp32: 14336 -> 4096 48 and 53, 4096 -> 50000
-   * 166 and 158. */
-  bool rows = b_kc ? n * k * size <= 1 << 26 || (m <= 4 && k * size >= 1 << 14) : n < 1 << 15;
+   * 166 and 158.  16-bit rows that start on 2 bytes only the former reads where
+   * they lie; for the tiles they would be laid out anew: 8 x 20001 -> 8001 127 us
+   * and 193. */
+  bool rows = odd || (b_kc ? n * k * size <= 1 << 26 || (m <= 4 && k * size >= 1 << 14) : n < 1 << 15);
   if (a_kc && m <= 16 && rows) {
     p.plan = PLAN_ROWS;
     int64_t steps = (k * size + STEP_BYTES - 1) / STEP_BYTES;
@@ -103,17 +105,17 @@ Plan choose(int64_t m, int64_t n, int64_t k, int size, bool a_kc, bool b_kc, boo
 }
 
 /* choose() takes a microsecond or two; a program asks for few sizes. */
-Plan planned(int64_t m, int64_t n, int64_t k, int size, bool a_kc, bool b_kc, bool bare) {
+Plan planned(int64_t m, int64_t n, int64_t k, int size, bool a_kc, bool b_kc, bool bare, bool odd) {
   struct Entry {
     int64_t m, n, k;
     int form;
     Plan plan;
   };
   static thread_local Entry known[64];
-  int form = 16 | size << 5 | a_kc | b_kc << 1 | bare << 2;
+  int form = 16 | size << 5 | a_kc | b_kc << 1 | bare << 2 | odd << 3;
   Entry &e = known[(uint64_t)(m * 1000003 + n * 10007 + k * 101 + form) % 64];
   if (e.m != m || e.n != n || e.k != k || e.form != form)
-    e = {m, n, k, form, choose(m, n, k, size, a_kc, b_kc, bare)};
+    e = {m, n, k, form, choose(m, n, k, size, a_kc, b_kc, bare, odd)};
   return e.plan;
 }
 
@@ -125,7 +127,7 @@ struct Matrix { /* [rows, k]; strides in elements */
 struct Operand { /* as the kernels read it */
   const void *p;
   int64_t ld, extent, k;
-  bool kc;
+  bool kc, odd = false; /* rows start on 2 bytes */
 };
 
 /* One call: run for good, or (without a workspace) only to see how much of it
@@ -153,12 +155,14 @@ struct Call {
 
   /* Loads take dwords, and are cut off at the extent dword by dword, so rows
    * that do not start on 4 bytes are laid out anew; so is a matrix that is
-   * contiguous along neither axis, or not along k where any_axis is false. */
-  Operand prepare(Matrix t, bool any_axis) {
+   * contiguous along neither axis, or not along k where any_axis is false.
+   * The kernel for few rows reads b's wherever they start. */
+  Operand prepare(Matrix t, bool any_axis, bool anywhere = false) {
     bool aligned = (uintptr_t)t.p % 4 == 0;
     if (t.rows == 1 && t.s1 == 1) t.s0 = dwords(t.k * size) / size;
-    if (aligned && t.s1 == 1 && t.s0 * size % 4 == 0 && t.s0 * size <= LONGEST)
-      return {t.p, t.s0, dwords(((t.rows - 1) * t.s0 + t.k) * size), t.k, true};
+    bool odd = !aligned || t.s0 * size % 4;
+    if (t.s1 == 1 && (anywhere || !odd) && t.s0 * size <= LONGEST)
+      return {t.p, t.s0, dwords(((t.rows - 1) * t.s0 + t.k) * size), t.k, true, odd};
     if (aligned && any_axis && t.s0 == 1 && t.s1 >= t.rows && t.s1 * size % 4 == 0 &&
         t.s1 * size <= LONGEST)
       return {t.p, t.s1, dwords(((t.k - 1) * t.s1 + t.rows) * size), t.k, false};
@@ -177,7 +181,7 @@ struct Call {
   void product(const Operand &a, const Operand &b, int64_t m, int64_t n, GemmArgs out) {
     int64_t k = a.k;
     bool bare = !out.bias && !out.res && !out.z && out.act == ACT_NONE;
-    Plan p = planned(m, n, k, size, a.kc, b.kc, bare);
+    Plan p = planned(m, n, k, size, a.kc, b.kc, bare, b.odd);
     if (p.plan == 0 && tiles_of(0, p.rows, n) > MOST_TILES) code = OPS_TOO_LONG;
     if (p.rows < m) {
       auto below = [&](const void *q, int64_t ld) {
@@ -205,8 +209,8 @@ struct Call {
   }
   void product(const Matrix &a, const Matrix &b, const GemmArgs &out) {
     /* few rows are read with k contiguous, but for short sums */
-    Operand p = prepare(a, a.rows > 16 || a.k <= OUTER_K), q = prepare(b, true);
-    product(p, q, a.rows, b.rows, out);
+    Operand p = prepare(a, a.rows > 16 || a.k <= OUTER_K);
+    product(p, prepare(b, true, a.rows <= 16 && p.kc), a.rows, b.rows, out);
   }
 
   void forward(const LinearArgs &p) {

@@ -229,6 +229,37 @@ def test_linear_offsets_past_32_bits():
     within(y[:, -64:], x.double() @ far.t(), 8194 * U * (x.double().abs() @ far.t().abs()))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m", [1, 7, 16, 40, 300, 2100])
+@pytest.mark.parametrize("pad", [1, 2, 3, 8])
+@pytest.mark.gpu
+def test_linear_reads_nothing_behind_its_rows(dtype, m, pad):
+    """NaN lies behind every row and behind the last one, along either axis."""
+    gen, device, h = seeded(m), "cuda", half_step(dtype)
+    n = 44
+
+    def inside(rows, cols, more=0):
+        whole = torch.full((rows + more, cols + pad), float("nan"), device=device, dtype=dtype)
+        whole[:rows, :cols] = normal(gen, rows, cols, dtype=dtype, device=device)
+        return whole[:rows, :cols]
+
+    for k in (1, 31, 130, 1277):
+        x, dy = inside(m, k), inside(m, n)
+        for w in (inside(n, k), inside(k, n, more=3).t()):
+            leaf = [t.detach().requires_grad_() for t in (x, w)]
+            y = ops.linear(*leaf)
+            same = [t.detach().contiguous().requires_grad_() for t in (x, w)]
+            z = ops.linear(*same)
+            got = [y, *torch.autograd.grad(y, leaf, dy)]
+            want = [z, *torch.autograd.grad(z, same, dy.contiguous())]
+            for g, t, terms, (a, b) in zip(got, want, (k, n, m), ((x, w.t()), (dy, w), (dy.t(), x))):
+                # two results e (1 + h) + s, where s is a sum's error in 32 bits:
+                # they differ by 2 s + 2 h |e|, and |e| <= (|t| + s) / (1 - h)
+                s = (terms + 2) * U * (a.abs().float() @ b.abs().float()).double()
+                within(g.double(), t.double(), 2 * least(dtype) + 2 * s
+                       + 2 * h * (t.double().abs() + s) / (1 - h))
+
+
 @pytest.mark.gpu
 def test_linear_rows_past_one_axis_of_a_launch():
     rows = (1 << 29) + 3
