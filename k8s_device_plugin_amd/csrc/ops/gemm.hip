@@ -508,13 +508,16 @@ __global__ __launch_bounds__(256) void gemm_join(GemmArgs p) {
  * Bound by reading b.  1 x 4096 -> 4096 bf16: 8.9 us with b out of the cache;
  * 2 x 25088 -> 4096 fp32: 93 us, 4.4 TB/s, and with k strided 76 us, 5.4 TB/s. */
 template <typename T, bool BKC, bool LOOSE>
-__global__ __launch_bounds__(512) void gemm_rows(GemmArgs p) {
+__global__ __launch_bounds__(512, BKC ? 4 : 2) void gemm_rows(GemmArgs p) {
   constexpr int V = Vec<T>::N, WAVES = 8;
   constexpr int FN = BKC ? 1 : V;    /* products a step */
   constexpr int STRIP = 16 * FN;     /* columns of y */
   constexpr int LOADS = BKC ? 1 : V; /* of b a step */
-  /* steps a wave has in flight, twice: 8 KB of b */
-  constexpr int C = 8 / LOADS;
+  /* Steps a wave has in flight, twice: with k contiguous 6, whose registers
+   * leave room for a second workgroup on the CU.  us for 6, and for 8 with one
+   * workgroup: 1 x 5155 -> 4311 bf16 33 and 43, 1 x 501 -> 20000 24 and 34, 1 x
+   * 4096 -> 4096 10.9 and 10.6. */
+  constexpr int C = BKC ? 6 : 8 / LOADS;
   typedef typename Vec<T>::type vec;
   __shared__ f32x4 lds[WAVES][16][STRIP / 4];
 
