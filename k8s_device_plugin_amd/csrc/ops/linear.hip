@@ -78,7 +78,7 @@ Plan choose(int64_t m, int64_t n, int64_t k, int size, bool a_kc, bool b_kc, boo
   /* Up to 16 rows stream b past the matrix cores while it is small, and beyond
    * that where a row of it is long enough for its workgroup and a's few rows
    * cost nothing beside it; tiles take the others.  us, rows and tiles, weights
-   * out of the cache: 1 x 4096 x 4096 bf16 12.3 and 15.8; 1 x 50000 -> 4096
+   * out of the cache: 1 x 4096 -> 4096 bf16 10.8 and 15.8; 1 x 50000 -> 4096
    * bf16 71 and 81; 16 of them 115 and 85; 1 x 4096 -> 50000 bf16 90 and 82.
    * With k strided in b, 8 rows fp32: 14336 -> 4096 48 and 53, 4096 -> 50000
    * 166 and 158.  16-bit rows that start on 2 bytes only the former reads where
