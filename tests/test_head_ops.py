@@ -261,6 +261,28 @@ def test_linear_reads_nothing_behind_its_rows(dtype, m, pad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m, n, k", [(4096, 4096, 517), (4099, 1030, 3001), (513, 4096, 67)])
+def test_linear_large_tiles_read_nothing_behind_their_rows(dtype, m, n, k):
+    gen = seeded(k)
+
+    def inside(rows, cols):
+        whole = torch.full((rows + 1, cols + 3), float("nan"), device="cuda", dtype=dtype)
+        whole[:rows, :cols] = normal(gen, rows, cols, dtype=dtype, device="cuda")
+        return whole[:rows, :cols]
+
+    x = inside(m, k)
+    for w in (inside(n, k), inside(k, n).t()):
+        y = ops.linear(x, w)
+        # columns of 64 bits at a few places, all rows; and no NaN anywhere
+        assert y.isfinite().all()
+        at = torch.tensor([0, 1, 127, 128, n // 2, n - 2, n - 1], device="cuda")
+        want = x.double() @ w[at].double().t().contiguous()
+        s = (k + 2) * U * (x.abs().double() @ w[at].abs().double().t().contiguous())
+        within(y[:, at], want, s)
+
+
+@pytest.mark.gpu
 def test_linear_rows_past_one_axis_of_a_launch():
     rows = (1 << 29) + 3
     x = torch.randn(1 << 20, 8, device="cuda", dtype=torch.float16).repeat(513, 1)[:rows]
