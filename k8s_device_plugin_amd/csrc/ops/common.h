@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 typedef __bf16 bf16;
 typedef _Float16 fp16;
@@ -30,6 +31,15 @@ template <typename T>
 __device__ inline float to_f(T v) { return (float)v; }
 template <typename T>
 __device__ inline T from_f(float v) { return (T)v; }
+
+/* A finite v as the nearest finite value of T's range: for what is stored to
+ * take a slope at, which has a limit there but is NaN at an infinity. */
+template <typename T>
+__device__ inline float in_range(float v) {
+  if constexpr (sizeof(T) == 4) return v;
+  constexpr float MOST = std::is_same_v<T, fp16> ? 65504.f : 0x1.fep127f;
+  return fabsf(v) < INFINITY ? fminf(fmaxf(v, -MOST), MOST) : v;
+}
 
 /* n <= Vec<T>::N values at p, in one access where all N are there.  Global
  * accesses of 16 bytes need no alignment beyond the element's, so rows of an
@@ -170,7 +180,8 @@ struct GemmArgs {
   int64_t ldr;
   void *y;
   int64_t ldy;
-  void *z; /* the value before the activation, where backward needs it */
+  void *z; /* the value before the activation, where backward needs it; finite where
+              the sum is */
   int64_t ldz;
   float *work; /* splits x m x n partial sums */
   int32_t dtype, a_kc, b_kc, act;

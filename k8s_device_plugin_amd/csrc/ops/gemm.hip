@@ -225,7 +225,7 @@ struct Epilogue {
     if (p.z)
 #pragma unroll
       for (int q = 0; q < COUNT; q++)
-        *(Four<T> *)((T *)p.z + (m + q * step) * p.ldz + col) = narrow(v[q]);
+        *(Four<T> *)((T *)p.z + (m + q * step) * p.ldz + col) = narrow(kept(v[q]));
     activate_all<T>(v, p.act);
     if (p.res)
 #pragma unroll
@@ -252,7 +252,7 @@ struct Epilogue {
       }
       f32x4 u[1] = {{v[e], 0.f, 0.f, 0.f}};
       if (p.bias) u[0][0] += to_f<T>(((const T *)p.bias)[col + e]);
-      if (p.z) ((T *)p.z)[m * p.ldz + col + e] = from_f<T>(u[0][0]);
+      if (p.z) ((T *)p.z)[m * p.ldz + col + e] = from_f<T>(in_range<T>(u[0][0]));
       activate_all<T>(u, p.act);
       if (p.res) u[0][0] += to_f<T>(((const T *)p.res)[m * p.ldr + col + e]);
       ((T *)p.y)[m * p.ldy + col + e] = from_f<T>(u[0][0]);
@@ -261,6 +261,9 @@ struct Epilogue {
 
   static __device__ f32x4 wide(Four<T> t) {
     return f32x4{to_f<T>(t[0]), to_f<T>(t[1]), to_f<T>(t[2]), to_f<T>(t[3])};
+  }
+  static __device__ f32x4 kept(f32x4 v) {
+    return f32x4{in_range<T>(v[0]), in_range<T>(v[1]), in_range<T>(v[2]), in_range<T>(v[3])};
   }
   static __device__ Four<T> narrow(f32x4 v) {
     return Four<T>{from_f<T>(v[0]), from_f<T>(v[1]), from_f<T>(v[2]), from_f<T>(v[3])};

@@ -56,3 +56,43 @@ def test_distill_all_named_classes_masked_in_the_student(device, dtype, reductio
         ops.distill_loss(leaf, index, teacher, temperature=t, reduction=reduction), leaf,
         torch.full_like(loss, 0.5))
     within(half, *distill_gradient(logits, index, teacher, t, each / 2))
+
+
+@pytest.mark.parametrize("device,dtype", PAIRS)
+@pytest.mark.parametrize("act", ["gelu", "silu", "relu"])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("m,n", [(3, 24), (40, 520), (300, 520)])
+def test_linear_value_before_the_activation_past_the_types_range(device, dtype, act, residual, m, n):
+    """Sums of +-1.4e6, which fp16 cannot hold: the slope is 1 or 0 there, as
+    it is in fp32, and the gradients are finite."""
+    k = 16
+    sign = torch.ones(n)
+    sign[1::2] = -1
+    x = torch.full((m, k), 300.0, device=device, dtype=dtype).requires_grad_()
+    w = (300 * sign)[:, None].expand(n, k).to(device=device, dtype=dtype).contiguous().requires_grad_()
+    b = torch.zeros(n, device=device, dtype=dtype, requires_grad=True)
+    r = torch.zeros(m, n, device=device, dtype=dtype) if residual else None
+    y = ops.linear(x, w, b, activation=act, residual=r)
+    assert (y[:, ::2] == torch.full((), 300.0 * 300 * k, dtype=torch.float64).to(dtype).to(device)).all()
+    assert (y[:, 1::2] == 0).all()
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.full_like(y, 0.125))
+    # sums of multiples of 1/8 below 2^21: exact, and stored with one rounding
+    on = (sign > 0).double().to(device)
+    assert torch.equal(dx, (0.125 * 300 * on.sum()).expand(m, k).to(dtype))
+    assert torch.equal(dw, (0.125 * 300 * m * on)[:, None].expand(n, k).to(dtype))
+    assert torch.equal(db, (0.125 * m * on).to(dtype))
+
+
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+@pytest.mark.gpu
+def test_linear_value_before_the_activation_past_bfloat16s_range(act):
+    """2^126 x 3.97 and a bias: finite in fp32, rounded past bf16's greatest."""
+    big = 1.9921875 * 2.0 ** 63
+    x = torch.full((5, 1), big, device="cuda", dtype=torch.bfloat16)
+    w = torch.tensor([[big], [-big]] * 12, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    b = torch.tensor([2.3e36, -2.3e36] * 12, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = ops.linear(x, w, b, activation=act)
+    assert (y[:, ::2] == INF).all() and (y[:, 1::2] == 0).all()
+    dw, db = torch.autograd.grad(y, (w, b), torch.ones_like(y))
+    on = torch.tensor([1.0, 0.0] * 12, device="cuda", dtype=torch.float64)
+    assert torch.equal(dw[:, 0], (5 * big * on).bfloat16()) and torch.equal(db, (5 * on).bfloat16())
