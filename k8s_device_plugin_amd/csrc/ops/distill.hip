@@ -115,7 +115,7 @@ __global__ __launch_bounds__(1024) void distill_slots(DistillArgs p) {
     bool bad = false, some = false;
     for (int k = lane; k < p.top; k += 64) {
       int64_t i = index_at(p, row, k);
-      float t = p.teacher ? any_f(p.teacher, row * p.ldt + k, p.ttype) * inv_t : 0.f;
+      float t = p.teacher ? any_f(p.teacher, row * p.ldt + k, p.ttype) : 0.f;
       bool here = i >= 0 && t != -INFINITY;
       bad |= i >= p.v;
       some |= here;
@@ -128,8 +128,9 @@ __global__ __launch_bounds__(1024) void distill_slots(DistillArgs p) {
     bad = __any(bad);
     some = __any(some);
     float state = bad ? BAD_INDEX : some ? TARGET : NO_TARGET;
+    /* divided by T behind the difference: logits of any size stay in range */
     float mass = 0.f;
-    for (int k = lane; k < p.top; k += 64) mass += expf(sp[k] - high);
+    for (int k = lane; k < p.top; k += 64) mass += expf((sp[k] - high) * inv_t);
     mass = wave_sum(mass);
     float log_mass = logf(mass), loss = 0.f, origin = -INFINITY;
     for (int k = lane; k < p.top; k += 64)
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(1024) void distill_slots(DistillArgs p) {
     for (int o = 32; o; o >>= 1) origin = fmaxf(origin, __shfl_xor(origin, o, 64));
     if (origin == -INFINITY) origin = 0.f;
     for (int k = lane; k < p.top; k += 64) {
-      float log_p = sp[k] - high - log_mass, m = expf(sp[k] - high) / mass;
+      float t = (sp[k] - high) * inv_t, log_p = t - log_mass, m = expf(t) / mass;
       if (some && si[k] >= 0 && m != 0.f) loss += m * (log_p - (to_f<T>(x[si[k]]) - origin) * inv_t);
       sp[k] = m;
     }

@@ -90,9 +90,11 @@ def _plain(logits, index, teacher, temperature, reduction, scale):
     here = (index >= 0) & (teacher != -torch.inf)
     bad = (index >= logits.shape[-1]).any(-1)
     some = here.any(-1) | bad
-    t = torch.where(here, teacher.to(kind) / temperature, -torch.inf)
+    t = teacher.to(torch.promote_types(teacher.dtype, kind)).masked_fill(~here, -torch.inf)
     t = torch.where(here.any(-1, keepdim=True), t, 0.0)
-    log_p = torch.log_softmax(t, -1)
+    if index.shape[-1]:  # so that no finite logit leaves its range
+        t = (t - t.amax(-1, keepdim=True)) / temperature
+    log_p = torch.log_softmax(t, -1).to(kind)
     x = torch.where(some.unsqueeze(-1), logits.to(kind), 0.0)
     most = x.detach().amax(-1, keepdim=True)  # so that no finite logit leaves its range
     x = (x - torch.where(most.isfinite(), most, 0.0)) / temperature

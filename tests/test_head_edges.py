@@ -96,3 +96,30 @@ def test_linear_value_before_the_activation_past_bfloat16s_range(act):
     dw, db = torch.autograd.grad(y, (w, b), torch.ones_like(y))
     on = torch.tensor([1.0, 0.0] * 12, device="cuda", dtype=torch.float64)
     assert torch.equal(dw[:, 0], (5 * big * on).bfloat16()) and torch.equal(db, (5 * on).bfloat16())
+
+
+@pytest.mark.parametrize("device,dtype", PAIRS)
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("t", [0.25, 0.5, 1.0, 3.0])
+def test_distill_teacher_at_the_lowest_value(device, dtype, reduction, t):
+    """Slots at the type's lowest value have no mass beside an ordinary one,
+    and weigh alike where there is no other: dividing by T empties no row."""
+    logits, index, teacher = distill_inputs(6, 60, 5, dtype, device)
+    same = teacher.clone()
+    low = torch.finfo(dtype).min
+    teacher[1], same[1] = low, 0.0
+    teacher[2, :2], teacher[2, 2:] = low, -INF
+    same[2, :2], same[2, 2:] = 0.0, -INF
+    teacher[3, 1:], same[3, 1:] = low, -INF
+    teacher[4], same[4] = -low, 0.0
+    teacher[5, 0] = -INF
+    same[5, 0] = -INF
+
+    def both(teacher):
+        leaf = logits.clone().requires_grad_()
+        loss = ops.distill_loss(leaf, index, teacher, temperature=t, reduction=reduction)
+        return loss.detach(), torch.autograd.grad(loss, leaf, torch.ones_like(loss))[0]
+
+    check_distill(logits, index, same, t, reduction)
+    for a, b in zip(both(teacher), both(same)):
+        assert torch.equal(a, b)
