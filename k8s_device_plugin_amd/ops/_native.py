@@ -145,8 +145,11 @@ def same_device(names: str, first, *others) -> None:
 
 def gradients_of(plain, inputs, needed, grad):
     """The gradients with a graph of their own, for a second derivative: the
-    plain formula is run again and differentiated."""
+    plain formula is run again and differentiated.  It is run on aliases, so
+    that each gradient stops at its own input where inputs depend on each other
+    or are the same tensor: autograd goes on from there by itself."""
     with torch.enable_grad():
+        inputs = [None if t is None else t.view_as(t) for t in inputs]
         wanted = [t for t, need in zip(inputs, needed) if need]
         found = iter(torch.autograd.grad(plain(*inputs), wanted, grad, create_graph=True))
         return [next(found) if need else None for need in needed]

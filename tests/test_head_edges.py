@@ -123,3 +123,66 @@ def test_distill_teacher_at_the_lowest_value(device, dtype, reduction, t):
     check_distill(logits, index, same, t, reduction)
     for a, b in zip(both(teacher), both(same)):
         assert torch.equal(a, b)
+
+
+def tied(kind, device, dtype=torch.float32):
+    """Calls whose inputs depend on each other, as (f of the operator and its
+    leaves, the leaves)."""
+    gen = seeded(4)
+    e = normal(gen, 7, 5, device=device).to(dtype).requires_grad_()
+    b = normal(gen, 7, device=device).to(dtype).requires_grad_()
+    if kind == "same":
+        return lambda op: op(e, e, b), [e, b]
+    if kind == "embedding":
+        return lambda op: op(torch.tanh(e[:3]), e, b), [e, b]
+    if kind == "bias":
+        return lambda op: op(e[:4], e, e.sum(1) * b), [e, b]
+
+    def norm(op):
+        w = e[0] * 2
+        return op(torch.sin(e[:3] * w), w, e[1])
+    return norm, [e]
+
+
+def derivatives(call, op, leaves):
+    """First gradients with a graph, and the second ones of their squares."""
+    y = call(op)
+    up = torch.linspace(-1, 2, y.numel(), device=y.device, dtype=y.dtype).view(y.shape)
+    first = torch.autograd.grad(y, leaves, up, create_graph=True)
+    return [*(g.detach() for g in first),
+            *torch.autograd.grad(sum((g * g).sum() for g in first), leaves, materialize_grads=True)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["same", "embedding", "bias", "norm"])
+@pytest.mark.parametrize("act", ["none", "gelu"])
+def test_gradients_with_a_graph_where_inputs_depend_on_each_other(kind, act):
+    f = {"none": lambda z: z, "gelu": F.gelu}[act]
+    if kind == "norm":
+        ours = lambda *t: ops.layer_norm(*t)  # noqa: E731
+        plain = lambda x, w, b: F.layer_norm(x, (5,), w, b)  # noqa: E731
+    else:
+        ours = lambda *t: ops.linear(*t, activation=act)  # noqa: E731
+        plain = lambda *t: f(F.linear(*t))  # noqa: E731
+    call, leaves = tied(kind, "cuda")
+    got = derivatives(call, ours, leaves)
+    call, leaves = tied(kind, "cpu", torch.float64)
+    for a, b in zip(got, derivatives(call, plain, leaves)):
+        # sums of fewer than 2000 products of ordinary size, twice differentiated
+        assert (a.double().cpu() - b).norm() <= 2000 * U * b.norm()
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_gradients_of_stop_at_each_input(device):
+    from k8s_device_plugin_amd.ops import _native
+
+    leaf = normal(seeded(), 6, 5, device=device).requires_grad_()
+    x = torch.tanh(leaf[:3])
+    for inputs in ((x, leaf), (leaf, leaf)):
+        grad = torch.ones(inputs[0].shape[0], 6, device=device)
+        got = _native.gradients_of(F.linear, inputs, (True, True), grad)
+        apart = [t.detach().requires_grad_() for t in inputs]
+        for a, b in zip(got, torch.autograd.grad(F.linear(*apart), apart, grad)):
+            assert torch.equal(a, b) and a.requires_grad
+        none, w = _native.gradients_of(F.linear, inputs, (False, True), grad)
+        assert none is None and torch.equal(w, got[1])
