@@ -62,8 +62,9 @@ def on_gpu(*tensors) -> bool:
     """Whether the kernels run: ordinary tensors on a GPU, and nothing that
     traces or transforms the call.  Otherwise the plain formula runs: so too
     for tensors whose sign is still to be turned, as conj()'s imaginary part,
-    and inside forward-mode differentiation."""
-    if torch.compiler.is_compiling():
+    inside forward-mode differentiation, and under a dispatch mode, which
+    records, counts or replaces torch's operations and would miss the call."""
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack():
         return False
     for t in tensors:
         if t is not None and (type(t) not in _PLAIN_TENSORS or not t.is_cuda or t.is_neg()):
@@ -143,13 +144,20 @@ def same_device(names: str, first, *others) -> None:
                 if t is not None))
 
 
+def formula_backward() -> bool:
+    """Whether a backward pass is the formula's: to be differentiated again, or
+    seen by a dispatch mode."""
+    return torch.is_grad_enabled() or torch._C._len_torch_dispatch_stack() > 0
+
+
 def gradients_of(plain, inputs, needed, grad):
-    """The gradients with a graph of their own, for a second derivative: the
-    plain formula is run again and differentiated.  It is run on aliases, so
+    """The gradients, with a graph of their own where that is wanted: the plain
+    formula is run again and differentiated.  It is run on aliases, so
     that each gradient stops at its own input where inputs depend on each other
     or are the same tensor: autograd goes on from there by itself."""
+    again = torch.is_grad_enabled()
     with torch.enable_grad():
         inputs = [None if t is None else t.view_as(t) for t in inputs]
         wanted = [t for t, need in zip(inputs, needed) if need]
-        found = iter(torch.autograd.grad(plain(*inputs), wanted, grad, create_graph=True))
+        found = iter(torch.autograd.grad(plain(*inputs), wanted, grad, create_graph=again))
         return [next(found) if need else None for need in needed]

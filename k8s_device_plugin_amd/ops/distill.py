@@ -170,7 +170,7 @@ class _Distill(torch.autograd.Function):
         # handed out once: what a caller does to it must not reach a second
         # backward pass, which writes its own
         dx, ctx.dx = ctx.dx, None
-        if torch.is_grad_enabled():
+        if _native.formula_backward():
             found = _native.gradients_of(lambda x: _plain(x, index, teacher, *ctx.how), (logits,),
                                          (True,), grad)
             return (*found, None, None, None, None, None)

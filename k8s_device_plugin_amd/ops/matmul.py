@@ -121,7 +121,7 @@ class _Linear(torch.autograd.Function):
         x, weight, bias, z = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         dr = dy if need_r else None
-        if torch.is_grad_enabled():
+        if _native.formula_backward():
             found = _native.gradients_of(
                 lambda x, w, b: formula(x, w, b, None, ctx.activation), (x, weight, bias),
                 (need_x, need_w, need_b), dy)

@@ -103,7 +103,7 @@ class _LayerNorm(torch.autograd.Function):
         x, weight, bias, stats = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         groups = ctx.groups
-        if torch.is_grad_enabled():
+        if _native.formula_backward():
             return (*_native.gradients_of(
                 lambda x, w, b: _plain(x, w, b, groups, ctx.eps), (x, weight, bias),
                 (need_x, need_w, need_b), dy), None, None)

@@ -186,3 +186,38 @@ def test_gradients_of_stop_at_each_input(device):
             assert torch.equal(a, b) and a.requires_grad
         none, w = _native.gradients_of(F.linear, inputs, (False, True), grad)
         assert none is None and torch.equal(w, got[1])
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_calls_under_a_dispatch_mode_run_the_formula(device):
+    """What records or counts torch's operations sees the whole call."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+
+    gen = seeded()
+    x, w = normal(gen, 6, 8, device=device), normal(gen, 5, 8, device=device)
+    index = torch.zeros(6, 1, dtype=torch.long, device=device)
+
+    def f(x, w):
+        y = ops.linear(x, w, activation="gelu")
+        return y, ops.layer_norm(x), ops.distill_loss(y, index)
+
+    def gradients(x, w):
+        x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+        y, h, loss = f(x, w)
+        return torch.autograd.grad((y.sum(), (h * h * h).sum(), loss), (x, w))
+
+    a, b = normal(gen, 6, 8, device=device), normal(gen, 5, 8, device=device)
+    for g in (f, gradients):
+        traced = make_fx(g)(x, w)
+        for got, want in zip(traced(a, b), g(a, b)):
+            assert (got - want).abs().max() <= 256 * U * (1 + want.abs().max())
+    with FlopCounterMode(display=False) as counter:
+        ops.linear(x, w)
+    assert counter.get_total_flops() == 2 * 6 * 8 * 5
+    # a backward pass alone, whose graph was made outside: the formula is run again
+    leaf = x.clone().requires_grad_()
+    y = ops.linear(leaf, w)
+    with FlopCounterMode(display=False) as counter:
+        got, = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    assert counter.get_total_flops() >= 2 * 6 * 8 * 5 and not got.requires_grad
