@@ -521,6 +521,17 @@ int run(const DistillArgs &p, hipStream_t s) {
 
 extern "C" {
 
+/* The number of the capture that a stream takes part in, 0 for none. */
+uint64_t vgpu_ops_capture(void *stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess) {
+    (void)hipGetLastError(); /* not the next launch's */
+    return 0;
+  }
+  return status == hipStreamCaptureStatusActive ? id : 0;
+}
+
 /* Into how many pieces a row is cut.  Forward: one where the rows alone fill
  * the card, else pieces of no less than 4096 classes.  Backward: pieces that
  * workgroups take in turn. */

@@ -6,7 +6,7 @@ path: a missing library is an error, never a silent fallback.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_float, c_int32, c_int64, c_void_p
+from ctypes import POINTER, c_float, c_int32, c_int64, c_uint64, c_void_p
 from functools import lru_cache
 from pathlib import Path
 
@@ -54,6 +54,8 @@ def library() -> ctypes.CDLL:
     lib.vgpu_ops_linear_work.argtypes = [POINTER(LinearArgs)]
     lib.vgpu_ops_linear_work.restype = c_int64
     lib.vgpu_ops_norm_parts.argtypes = [c_int64, c_int64, c_int64]
+    lib.vgpu_ops_capture.argtypes = [c_void_p]
+    lib.vgpu_ops_capture.restype = c_uint64
     lib.vgpu_ops_distill_chunks.argtypes = [c_int64, c_int64, c_int32]
     return lib
 
@@ -104,6 +106,13 @@ def launch(name: str, device: torch.device, *args) -> None:
     if rc:
         raise RuntimeError(f"vgpu_ops_{name}: " + ("refused the arguments" if rc < 0
                                                    else f"HIP error {rc}"))
+
+
+def capture(device: torch.device) -> int:
+    """The number of the capture that the device's current stream takes part
+    in, 0 for none (as of the default stream, which cannot)."""
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    return entry("capture")(stream) if stream else 0
 
 
 @lru_cache(maxsize=4096)

@@ -39,7 +39,8 @@ def distill_loss(logits, index, teacher=None, *, temperature=1.0, reduction="mea
 
     Where a gradient is wanted of a loss that is one number, it is written
     along with the loss, for an upstream gradient of 1, and held until
-    backward.  Another upstream gradient costs a second writing: a factor that
+    backward (not where only one of the two passes is captured into a graph, or
+    each into its own).  Another upstream gradient costs a second writing: a factor that
     is known before, as 1/n for n accumulated steps, belongs in ``scale``.
 
     On the CPU, and while a call is traced or transformed, the formula is run
@@ -161,6 +162,7 @@ class _Distill(torch.autograd.Function):
         ctx.how = temperature, reduction, scale
         loss, saved, ctx.dx = _forward(logits, index, teacher, temperature, REDUCTIONS[reduction],
                                        scale, True)
+        ctx.capture = None if ctx.dx is None else _native.capture(logits.device)
         ctx.save_for_backward(logits, index, teacher, saved)
         return loss
 
@@ -170,6 +172,10 @@ class _Distill(torch.autograd.Function):
         # handed out once: what a caller does to it must not reach a second
         # backward pass, which writes its own
         dx, ctx.dx = ctx.dx, None
+        # nor must it reach a replay of this pass alone, which has to write its
+        # gradient each time
+        if dx is not None and _native.capture(logits.device) != ctx.capture:
+            dx = None
         if _native.formula_backward():
             found = _native.gradients_of(lambda x: _plain(x, index, teacher, *ctx.how), (logits,),
                                          (True,), grad)

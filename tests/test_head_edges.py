@@ -221,3 +221,42 @@ def test_calls_under_a_dispatch_mode_run_the_formula(device):
     with FlopCounterMode(display=False) as counter:
         got, = torch.autograd.grad(y, leaf, torch.ones_like(y))
     assert counter.get_total_flops() >= 2 * 6 * 8 * 5 and not got.requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("how", ["eager", "another graph"])
+@pytest.mark.parametrize("rows,v", [(20, 1000), (600, 9001)])
+def test_distill_backward_captured_without_its_forward(dtype, how, rows, v):
+    """A captured backward pass writes its gradient on every replay, whatever
+    the upstream gradient was before and whatever was done to the last one."""
+    logits, index, teacher = distill_inputs(rows, v, 3, dtype, "cuda")
+    leaf = logits.requires_grad_()
+    up = torch.ones((), device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    first, graph = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+
+    def loss_of():
+        return ops.distill_loss(leaf, index, teacher, temperature=2.0)
+
+    with torch.cuda.stream(side):
+        want, = torch.autograd.grad(loss_of(), leaf)
+        twice, = torch.autograd.grad(loss_of(), leaf, 2 * up)
+        torch.cuda.synchronize()
+        if how == "eager":
+            loss = loss_of()
+        else:
+            with torch.cuda.graph(first, stream=side):
+                loss = loss_of()
+            first.replay()
+        with torch.cuda.graph(graph, stream=side):
+            grad, = torch.autograd.grad(loss, leaf, up, retain_graph=True)
+        for scale, expected in ((1, want), (2, twice), (1, want), (1, want), (2, twice)):
+            up.fill_(scale)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(grad, expected)
+            grad.mul_(7)  # the caller's, as a clipped gradient is
+            torch.randn(1 << 20, device="cuda").sum()
+    torch.cuda.current_stream().wait_stream(side)
