@@ -156,17 +156,21 @@ struct Call {
   /* Loads take dwords, and are cut off at the extent dword by dword, so rows
    * that do not start on 4 bytes are laid out anew; so is a matrix that is
    * contiguous along neither axis, or not along k where any_axis is false.
-   * The kernel for few rows reads b's wherever they start. */
+   * Where k is too long for a row (a weight's gradient over many tokens), the
+   * other axis is taken in any case.  The kernel for few rows reads b's wherever
+   * they start. */
   Operand prepare(Matrix t, bool any_axis, bool anywhere = false) {
+    bool fits = padded(t.k) * size <= LONGEST;
+    if (!fits) any_axis = true;
     bool aligned = (uintptr_t)t.p % 4 == 0;
-    if (t.rows == 1 && t.s1 == 1) t.s0 = dwords(t.k * size) / size;
+    if (t.rows == 1 && t.s1 == 1) t.s0 = fits ? dwords(t.k * size) / size : 1;
     bool odd = !aligned || t.s0 * size % 4;
-    if (t.s1 == 1 && (anywhere || !odd) && t.s0 * size <= LONGEST)
+    if (t.s1 == 1 && (anywhere || !odd) && t.s0 * size <= LONGEST && fits)
       return {t.p, t.s0, dwords(((t.rows - 1) * t.s0 + t.k) * size), t.k, true, odd};
     if (aligned && any_axis && t.s0 == 1 && t.s1 >= t.rows && t.s1 * size % 4 == 0 &&
         t.s1 * size <= LONGEST)
       return {t.p, t.s1, dwords(((t.k - 1) * t.s1 + t.rows) * size), t.k, false};
-    bool along = any_axis && t.s0 == 1 && t.s1 != 1 && padded(t.rows) * size <= LONGEST;
+    bool along = any_axis && (!fits || (t.s0 == 1 && t.s1 != 1)) && padded(t.rows) * size <= LONGEST;
     int64_t rows = along ? t.k : t.rows, cols = along ? t.rows : t.k, ld = padded(cols);
     if (ld * size > LONGEST) code = OPS_TOO_LONG;
     void *to = take(rows * ld * size);

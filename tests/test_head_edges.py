@@ -260,3 +260,52 @@ def test_distill_backward_captured_without_its_forward(dtype, how, rows, v):
             grad.mul_(7)  # the caller's, as a clipped gradient is
             torch.randn(1 << 20, device="cuda").sum()
     torch.cuda.current_stream().wait_stream(side)
+
+
+MANY = (1 << 21) + 1  # rows of fp32: one more than 8 MiB of them
+
+
+def linear_work(m, n, k, dtype=0, **how):
+    import ctypes
+
+    from k8s_device_plugin_amd.ops import _native
+
+    a = dict(x=4096, w=4096, dy=4096, dx=4096, dw=4096, db=4096, m=m, n=n, k=k, xs0=k, xs1=1, ws0=k,
+             ws1=1, lddy=n, dtype=dtype)
+    return _native.library().vgpu_ops_linear_work(ctypes.byref(_native.LinearArgs(**{**a, **how})))
+
+
+@pytest.mark.parametrize("dtype,m", [(0, MANY), (1, 2 * MANY), (2, 2 * MANY)])
+@pytest.mark.parametrize("n,k", [(1, 64), (2, 64), (16, 64), (17, 64), (257, 64), (300, 64), (1030, 64),
+                                 (64, 1), (64, 5), (1, 1), (33, 2)])
+def test_linear_backward_of_many_rows_has_a_plan(dtype, m, n, k):
+    assert linear_work(m, n, k, dtype) >= 0
+    assert linear_work(m, n, k, dtype, xs0=1, xs1=m) >= 0       # tokens contiguous
+    assert linear_work(m, n, k, dtype, xs0=1, xs1=m + 3) >= 0
+    assert linear_work(m, n, k, dtype, xs0=0) >= 0              # one row for all
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,m", [(torch.float32, MANY), (torch.bfloat16, 2 * MANY)])
+@pytest.mark.parametrize("n,k,columns", [(1, 64, False), (16, 64, False), (257, 64, False),
+                                         (64, 64, True), (64, 1, False), (40, 3, True)])
+def test_linear_backward_of_many_rows(dtype, m, n, k, columns):
+    """Small whole numbers: their sums are exact in any order."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    whole = lambda *s: torch.randint(-1, 2, s, generator=gen, device="cuda", dtype=torch.int8).to(dtype)  # noqa: E731
+    x = whole(k, m).t() if columns else whole(m, k)
+    x.requires_grad_()
+    w, b = whole(n, k).requires_grad_(), whole(n).requires_grad_()
+    y = ops.linear(x, w, b)
+    g = whole(m, n)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), g)
+    sums, column = torch.zeros(n, k, dtype=torch.float64, device="cuda"), 0
+    for part in range(0, m, 1 << 18):
+        at = slice(part, min(m, part + (1 << 18)))
+        sums += g[at].double().t() @ x.detach()[at].double()
+        column = column + g[at].double().sum(0)
+    assert torch.equal(dw, sums.to(dtype)) and torch.equal(db, column.to(dtype))
+    for at in (slice(0, 70), slice(m // 2, m // 2 + 70), slice(m - 70, m)):
+        assert torch.equal(dx[at], (g[at].double() @ w.detach().double()).to(dtype))
+        assert torch.equal(y.detach()[at], (x.detach()[at].double() @ w.detach().double().t()
+                                            + b.detach().double()).to(dtype))
