@@ -16,6 +16,7 @@ int64_t tiles_of(int plan, int64_t m, int64_t n) {
 
 /* A launch holds fewer than 2^32 threads along an axis. */
 constexpr int64_t MOST_TILES = (1 << 24) - 1;
+constexpr int64_t MOST_STRIPS = (1 << 23) - 1; /* of 512 threads */
 
 /* What a product takes in us with tiles of one kind, k in `splits` parts: in
  * turns of as many workgroups as the card holds (256 of the largest tile, 512
@@ -158,7 +159,7 @@ struct Call {
    * contiguous along neither axis, or not along k where any_axis is false.
    * Where k is too long for a row (a weight's gradient over many tokens), the
    * other axis is taken in any case.  The kernel for few rows reads b's wherever
-   * they start. */
+   * they start, where a launch of it holds them. */
   Operand prepare(Matrix t, bool any_axis, bool anywhere = false) {
     bool fits = padded(t.k) * size <= LONGEST;
     if (!fits) any_axis = true;
@@ -214,7 +215,8 @@ struct Call {
   void product(const Matrix &a, const Matrix &b, const GemmArgs &out) {
     /* few rows are read with k contiguous, but for short sums */
     Operand p = prepare(a, a.rows > 16 || a.k <= OUTER_K);
-    product(p, prepare(b, true, a.rows <= 16 && p.kc), a.rows, b.rows, out);
+    bool anywhere = a.rows <= 16 && p.kc && b.rows <= MOST_STRIPS * 16;
+    product(p, prepare(b, true, anywhere), a.rows, b.rows, out);
   }
 
   void forward(const LinearArgs &p) {

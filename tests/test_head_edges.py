@@ -309,3 +309,15 @@ def test_linear_backward_of_many_rows(dtype, m, n, k, columns):
         assert torch.equal(dx[at], (g[at].double() @ w.detach().double()).to(dtype))
         assert torch.equal(y.detach()[at], (x.detach()[at].double() @ w.detach().double().t()
                                             + b.detach().double()).to(dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 3])
+def test_linear_outputs_past_one_axis_of_a_launch(m):
+    """16-bit weights whose rows start on 2 bytes, and more strips of outputs
+    than a launch for few rows holds."""
+    n = (1 << 27) + 21
+    w = torch.randint(-8, 9, (n, 1), device="cuda", dtype=torch.int8).to(torch.float16)
+    x = torch.arange(1, m + 1, device="cuda", dtype=torch.float16)[:, None]
+    y = ops.linear(x, w)
+    assert torch.equal(y, x * w.t())
