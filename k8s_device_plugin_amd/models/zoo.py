@@ -16,7 +16,8 @@ ResNet-V2 = pre-activation bottlenecks (BN-ReLU-conv), matching the
 
 The models' heads (projection, the norm of DeepLab's pooled branch, the
 training loss) run through ``ops.linear``, ``ops.layer_norm`` and
-``ops.distill_loss``: gfx950 kernels on a GPU, torch's formula on the CPU.
+``ops.distill_loss`` on a GPU.  Their layers are torch's own modules, which are
+called as they are on the CPU, and wherever something hangs on them.
 """
 from __future__ import annotations
 
@@ -28,26 +29,58 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .. import ops
-from ..ops.matmul import formula
+from ..ops import _native
 
 
-class HeadLinear(nn.Linear):
-    """nn.Linear with its activation in the product's epilogue (ops.linear).
-    Parameters and state are nn.Linear's."""
+def untouched(module, kind) -> bool:
+    """Whether calling the module runs ``kind``'s own forward and nothing else:
+    not another layer in its place, and no hook, pruning, parametrization or
+    forward of its own, all of which want the call itself."""
+    return (type(module) is kind and "forward" not in module.__dict__
+            and module._compiled_call_impl is None
+            and not (module._forward_hooks or module._forward_pre_hooks
+                     or module._backward_hooks or module._backward_pre_hooks
+                     or nn.modules.module._has_any_global_hook()))
 
-    def __init__(self, in_features, out_features, bias=True, activation="none"):
-        super().__init__(in_features, out_features, bias)
-        self.activation = activation
+
+def by_kernel(x, *parameters) -> bool:
+    """Whether an operator's kernel runs on x with these parameters; what the
+    operators would refuse is left to torch."""
+    there = [t for t in parameters if t is not None]
+    return (_native.on_gpu(x, *there) and x.dtype in _native.DTYPES
+            and (_native.autocast(x.device) or all(t.dtype == x.dtype for t in there))
+            and all(t.dtype in _native.DTYPES and t.device == x.device
+                    and max(t.shape) * t.element_size() < 1 << 23 for t in there))
+
+
+def project(layer, x):
+    """layer(x), through ops.linear where the layer is torch's own."""
+    if untouched(layer, nn.Linear) and by_kernel(x, layer.weight, layer.bias):
+        return ops.linear(x, layer.weight, layer.bias)
+    return layer(x)
+
+
+class Classifier(nn.Sequential):
+    """nn.Sequential that runs a linear layer and a relu behind it as one
+    kernel (ops.linear) where both are torch's own."""
 
     def forward(self, x):
-        # scripts, and 64 bits on a GPU, take torch's own
         if torch.jit.is_scripting():
-            y = F.linear(x, self.weight, self.bias)
-            return F.relu(y) if self.activation == "relu" else y
+            for layer in self:
+                x = layer(x)
+            return x
         else:
-            if x.dtype == torch.float64:
-                return formula(x, self.weight, self.bias, None, self.activation)
-            return ops.linear(x, self.weight, self.bias, activation=self.activation)
+            layers = list(self)
+            while layers:
+                layer = layers.pop(0)
+                if untouched(layer, nn.Linear) and by_kernel(x, layer.weight, layer.bias):
+                    relu = bool(layers) and untouched(layers[0], nn.ReLU)
+                    x = ops.linear(x, layer.weight, layer.bias, activation="relu" if relu else "none")
+                    if relu:
+                        layers.pop(0)
+                else:
+                    x = layer(x)
+            return x
 
 
 # ---------------------------------------------------------------------------
@@ -93,14 +126,17 @@ class ResNetV2(nn.Module):
                 in_ch = w * PreActBottleneck.expansion
         self.blocks = nn.Sequential(*blocks)
         self.bn_final = nn.BatchNorm2d(in_ch)
-        self.fc = HeadLinear(in_ch, num_classes)
+        self.fc = nn.Linear(in_ch, num_classes)
 
     def forward(self, x):
         x = self.pool(self.stem(x))
         x = self.blocks(x)
         x = F.relu(self.bn_final(x))
         x = F.adaptive_avg_pool2d(x, 1).flatten(1)
-        return self.fc(x)
+        if torch.jit.is_scripting():
+            return self.fc(x)
+        else:
+            return project(self.fc, x)
 
 
 def resnet_v2_50():
@@ -129,11 +165,10 @@ class VGG16(nn.Module):
                 layers += [nn.Conv2d(in_ch, v, 3, padding=1), nn.ReLU(inplace=True)]
                 in_ch = v
         self.features = nn.Sequential(*layers)
-        self.classifier = nn.Sequential(
-            # Identity where the relu stood: layers keep their numbers
-            HeadLinear(512 * 7 * 7, 4096, activation="relu"), nn.Identity(), nn.Dropout(0.5),
-            HeadLinear(4096, 4096, activation="relu"), nn.Identity(), nn.Dropout(0.5),
-            HeadLinear(4096, num_classes),
+        self.classifier = Classifier(
+            nn.Linear(512 * 7 * 7, 4096), nn.ReLU(inplace=True), nn.Dropout(0.5),
+            nn.Linear(4096, 4096), nn.ReLU(inplace=True), nn.Dropout(0.5),
+            nn.Linear(4096, num_classes),
         )
 
     def forward(self, x):
@@ -169,16 +204,28 @@ class ASPP(nn.Module):
 
     def pooled(self, x):
         """self.gp(x).  On a 1x1 map the convolution is a matrix product and
-        the group norm a layer norm of each group's channels."""
+        the group norm a layer norm of each group's channels; a layer that is
+        not torch's own is called as it is."""
         if torch.jit.is_scripting():
             return self.gp(x)
         else:
-            if x.dtype == torch.float64:
+            if not untouched(self.gp, nn.Sequential) or len(self.gp) != 4:
                 return self.gp(x)
             pool, conv, norm, act = self.gp
-            p = ops.linear(pool(x).flatten(1), conv.weight.flatten(1))
-            p = ops.layer_norm(p, norm.weight, norm.bias, groups=norm.num_groups, eps=norm.eps)
-            return act(p)[:, :, None, None]
+            p = pool(x)
+            if (untouched(conv, nn.Conv2d) and conv.kernel_size == (1, 1) and conv.padding == (0, 0)
+                    and conv.groups == 1 and by_kernel(p, conv.weight, conv.bias)
+                    and p.shape[2:] == (1, 1)):
+                p = ops.linear(p.flatten(1), conv.weight.flatten(1), conv.bias)[:, :, None, None]
+            else:
+                p = conv(p)
+            if (untouched(norm, nn.GroupNorm) and by_kernel(p, norm.weight, norm.bias)
+                    and p.shape[2:] == (1, 1)):
+                p = ops.layer_norm(p.flatten(1), norm.weight, norm.bias, groups=norm.num_groups,
+                                   eps=norm.eps)[:, :, None, None]
+            else:
+                p = norm(p)
+            return act(p)
 
     def forward(self, x):
         size = x.shape[-2:]
@@ -223,11 +270,14 @@ class LSTMNet(nn.Module):
         super().__init__()
         self.lstm = nn.LSTM(input_size, hidden, num_layers=layers,
                             batch_first=True)
-        self.fc = HeadLinear(hidden, num_classes)
+        self.fc = nn.Linear(hidden, num_classes)
 
     def forward(self, x):
         out, _ = self.lstm(x)
-        return self.fc(out[:, -1])
+        if torch.jit.is_scripting():
+            return self.fc(out[:, -1])
+        else:
+            return project(self.fc, out[:, -1])
 
 
 # ---------------------------------------------------------------------------
