@@ -346,13 +346,19 @@ def distilled_batch(case: BenchCase, teacher: nn.Module, batch, top: int):
 
 
 def loss_of(case: BenchCase, out, y):
-    """Cross entropy with labels, or the distance to a teacher's top logits."""
-    if case.seg:
-        return F.cross_entropy(out.float(), y)
-    index, teacher = y if isinstance(y, tuple) else (y.unsqueeze(1), None)
-    if out.dtype == torch.float64:
-        out = out.float()
-    return ops.distill_loss(out, index, teacher)
+    """Cross entropy with labels, or the distance to a teacher's top logits.
+
+    A label for each row of a GPU's logits is ops.distill_loss's one slot: there
+    a row with a negative label counts as one without, and a label past the
+    classes makes the loss NaN.  Maps, probabilities of classes and whatever
+    has no kernel are F.cross_entropy's.
+    """
+    if isinstance(y, tuple):
+        return ops.distill_loss(out.float() if out.dtype == torch.float64 else out, *y)
+    if (not case.seg and out.dim() == 2 and y.dim() == 1 and out.dtype in _native.DTYPES
+            and y.dtype in (torch.int32, torch.int64) and _native.on_gpu(out, y)):
+        return ops.distill_loss(out, y.unsqueeze(1))
+    return F.cross_entropy(out.float(), y)
 
 
 def step(case: BenchCase, model: nn.Module, batch, optimizer=None) -> None:

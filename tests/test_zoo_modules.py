@@ -3,6 +3,7 @@ put in their place or made of them works as it does on any other."""
 import pytest
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
 from k8s_device_plugin_amd.models import zoo
 from test_zoo_heads import GPU, close
@@ -149,3 +150,25 @@ def test_heads_leave_to_torch_what_the_operators_refuse():
     assert zoo.project(wide, torch.randn(2, 1 << 21, device="cuda")).shape == (2, 2)
     with torch.autocast("cuda", dtype=torch.bfloat16):
         assert zoo.project(fc.float(), torch.randn(2, 8, device="cuda")).dtype == torch.bfloat16
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_loss_takes_every_target_of_cross_entropy(device):
+    case = zoo.CASES["resnet50_train"]
+    gen = torch.Generator().manual_seed(0)
+    out = torch.randn(6, 9, generator=gen).to(device)
+    maps = torch.randn(6, 9, 4, generator=gen).to(device)
+    label = torch.randint(0, 9, (6,), generator=gen).to(device)
+    ignored = label.clone()
+    ignored[2] = -100
+    for logits, y in ((out, torch.softmax(out + 1, 1)), (maps, label[:, None].expand(6, 4)),
+                      (maps, torch.softmax(maps + 1, 1)), (out[0], label[0]),
+                      (out.double(), label), (out, label), (out, ignored)):
+        a, b = (logits.clone().requires_grad_() for _ in range(2))
+        ours, theirs = zoo.loss_of(case, a, y), F.cross_entropy(b.float(), y)
+        assert close(ours.detach(), theirs.detach())
+        ours.backward(), theirs.backward()
+        assert close(a.grad, b.grad)
+    if device == "cpu":
+        with pytest.raises(IndexError):
+            zoo.loss_of(case, out, label + 9)
