@@ -207,7 +207,7 @@ int launch_repack(const void *src, int64_t rs, int64_t cs, int64_t rows, int64_t
 /* y = act(x W^T + bias) + res, x [m,k] and W [n,k] of any strides (in
  * elements), y and z [m,n] contiguous.  With dy, the backward pass instead: z
  * is then what the slope is taken at, and dx [m,k], dw [n,k], db [n] what is
- * written of the gradients, contiguous. */
+ * written of the gradients, contiguous; x is wanted for dw alone, W for dx. */
 struct LinearArgs {
   const void *x, *w, *bias, *res, *dy;
   void *y, *z, *dx, *dw, *db, *work;

@@ -265,7 +265,8 @@ struct Call {
 bool sound(const LinearArgs &p) {
   return p.m > 0 && p.n > 0 && p.k > 0 && p.dtype >= DT_F32 && p.dtype <= DT_FP16 &&
          p.act >= ACT_NONE && p.act <= ACT_SILU && p.xs0 >= 0 && p.xs1 >= 0 && p.ws0 >= 0 &&
-         p.ws1 >= 0 && p.x && p.w && (p.dy ? p.act == ACT_NONE || p.z : p.y != nullptr);
+         p.ws1 >= 0 && (p.x || (p.dy && !p.dw)) && (p.w || (p.dy && !p.dx)) &&
+         (p.dy ? p.act == ACT_NONE || p.z : p.y != nullptr);
 }
 
 }  // namespace

@@ -108,33 +108,64 @@ def _forward(x, weight, bias, residual, act, keep):
     return y, (y if z is None else z) if act else None
 
 
+def _formula_gradients(dy, x, weight, z, needed):
+    """Those of an activation whose slope is 0 or 1, by torch's operations.  x
+    and weight are there where a gradient takes them."""
+    dz = dy if z is None else torch.where(z <= 0, 0.0, dy)
+    flat = dz.reshape(-1, dz.shape[-1])
+    return (dz @ weight if needed[0] else None,
+            flat.t() @ x.reshape(-1, x.shape[-1]) if needed[1] else None,
+            flat.sum(0) if needed[2] else None)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
         y, z = _forward(x, weight, bias, residual, ACTIVATIONS[activation], True)
-        ctx.activation = activation
-        ctx.save_for_backward(x, weight, bias, None if z is None else z.view_as(y))
+        # what no gradient takes may be changed before the backward pass, as
+        # with torch's own; the derivative of a bent slope takes x and weight
+        bent = activation not in ("none", "relu")
+        need_x, need_w = ctx.needs_input_grad[:2]
+        ctx.activation, ctx.k = activation, x.shape[-1]
+        ctx.bias = (bias, bias._version) if bent and bias is not None else None
+        ctx.save_for_backward(x if need_w or bent else None, weight if need_x or bent else None,
+                              None if z is None else z.view_as(y))
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, weight, bias, z = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dr = dy if need_r else None
+        x, weight, z = ctx.saved_tensors
+        needed = ctx.needs_input_grad[:3]
+        dr = dy if ctx.needs_input_grad[3] else None
         if _native.formula_backward():
-            found = _native.gradients_of(
-                lambda x, w, b: formula(x, w, b, None, ctx.activation), (x, weight, bias),
-                (need_x, need_w, need_b), dy)
-            return (*found, dr, None)
-        n, k = weight.shape
-        x2, dy2 = _matrix(x, k), rows_of(dy.resolve_neg(), n)
-        dx = x.new_empty(x.shape) if need_x else None
-        dw = x.new_empty((n, k)) if need_w else None
-        db = x.new_empty(n) if need_b else None
-        if need_x or need_w or need_b:
+            return (*_formula_gradients(ctx, x, weight, z, needed, dy), dr, None)
+        n, k = dy.shape[-1], ctx.k
+        dy2 = rows_of(dy.resolve_neg(), n)
+        dx = dy.new_empty(dy.shape[:-1] + (k,)) if needed[0] else None
+        dw = dy.new_empty((n, k)) if needed[1] else None
+        db = dy.new_empty(n) if needed[2] else None
+        if any(needed):
+            x2 = _matrix(x, k) if needed[1] else None
             _launch(LinearArgs(
-                x2.data_ptr(), weight.data_ptr(), None, None, dy2.data_ptr(), None, ptr(z),
-                ptr(dx), ptr(dw), ptr(db), None, x2.shape[0], n, k, *x2.stride(),
-                *weight.stride(), 0, dy2.stride(0), 0, DTYPES[x.dtype],
-                ACTIVATIONS[ctx.activation]), x.device)
+                ptr(x2), ptr(weight) if needed[0] else None, None, None, dy2.data_ptr(), None, ptr(z),
+                ptr(dx), ptr(dw), ptr(db), None, dy2.shape[0], n, k,
+                *((0, 0) if x2 is None else x2.stride()),
+                *(weight.stride() if needed[0] else (0, 0)), 0, dy2.stride(0), 0, DTYPES[dy.dtype],
+                ACTIVATIONS[ctx.activation]), dy.device)
         return dx, dw, db, dr, None
+
+
+def _formula_gradients(ctx, x, weight, z, needed, dy):
+    """The same by torch's operations."""
+    if ctx.activation in ("none", "relu"):
+        dz = dy if z is None else torch.where(z <= 0, 0.0, dy)
+        rows = dz.reshape(-1, dz.shape[-1])
+        return ((rows @ weight).reshape(dy.shape[:-1] + (ctx.k,)) if needed[0] else None,
+                rows.t() @ _matrix(x, ctx.k) if needed[1] else None,
+                rows.sum(0) if needed[2] else None)
+    bias, version = ctx.bias or (None, 0)
+    if bias is not None and bias._version != version:
+        raise RuntimeError("linear: the bias has been changed in place; the formula's gradient of "
+                           f"{ctx.activation} needs it as it was")
+    return _native.gradients_of(lambda x, w, b: formula(x, w, b, None, ctx.activation),
+                                (x, weight, bias), needed, dy)

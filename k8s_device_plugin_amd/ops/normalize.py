@@ -94,29 +94,29 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps):
         y, stats = _forward(x, weight, bias, groups, eps, True)
-        ctx.groups, ctx.eps = groups, eps
-        ctx.save_for_backward(x, weight, bias, stats)
+        ctx.groups, ctx.eps, ctx.kind = groups, eps, _kind(x, weight, bias)
+        ctx.save_for_backward(x, weight, stats)  # no gradient takes the bias
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
+        x, weight, stats = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        groups = ctx.groups
+        groups, kind = ctx.groups, ctx.kind
+        width = x.shape[-1]
         if _native.formula_backward():
+            bias = x.new_zeros(width, dtype=kind).requires_grad_() if need_b else None
             return (*_native.gradients_of(
                 lambda x, w, b: _plain(x, w, b, groups, ctx.eps), (x, weight, bias),
                 (need_x, need_w, need_b), dy), None, None)
-        width = x.shape[-1]
         x2, dy2 = rows_of(x, width), rows_of(dy.resolve_neg(), width)
         rows, d = x2.shape[0], width // groups
         dx = x.new_empty(x.shape) if need_x else None
-        dw = weight.new_empty(width) if need_w else None
-        db = bias.new_empty(width) if need_b else None
+        dw = x.new_empty(width, dtype=kind) if need_w else None
+        db = x.new_empty(width, dtype=kind) if need_b else None
         parts = _native.plan("norm_parts", rows, groups, d)
         part = (torch.empty(2 * parts * width, dtype=torch.float32, device=x.device)
                 if parts > 1 and (need_w or need_b) else None)
-        kind = _kind(x, weight, bias)
         weight = _vector(weight)
         launch("norm", x.device, NormArgs(
             x2.data_ptr(), ptr(weight), None, dy2.data_ptr(), None, ptr(dx), ptr(dw), ptr(db),

@@ -321,3 +321,80 @@ def test_linear_outputs_past_one_axis_of_a_launch(m):
     x = torch.arange(1, m + 1, device="cuda", dtype=torch.float16)[:, None]
     y = ops.linear(x, w)
     assert torch.equal(y, x * w.t())
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+def test_linear_inputs_that_no_gradient_takes_may_be_changed(device, act):
+    gen = seeded()
+    x, w, b = (normal(gen, *s, device=device) for s in ((3, 8), (5, 8), (5,)))
+    g = normal(gen, 3, 5, device=device)
+
+    def gradients(learnt, change):
+        t = {"x": x.clone(), "w": w.clone(), "b": b.clone()}
+        leaves = [t[n].requires_grad_() for n in learnt]
+        t["x"] = t["x"] * 1
+        y = ops.linear(t["x"], t["w"], t["b"], activation=act)
+        with torch.no_grad():
+            for n in change:
+                t[n].mul_(3)
+        return torch.autograd.grad(y, leaves, g)
+
+    bent = act in ("gelu", "silu")
+    for learnt, change in (("wb", "b" if bent else "wb"), ("x", "b" if bent else "xb"), ("xwb", "b"),
+                           ("b", "b" if bent else "xwb")):
+        for a, c in zip(gradients(learnt, change), gradients(learnt, "")):
+            assert torch.equal(a, c), (learnt, change)
+    if not bent:
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            gradients("xw", "w")
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_norm_bias_may_be_changed(device):
+    x, b = normal(seeded(), 3, 8, device=device).requires_grad_(), torch.zeros(8, device=device)
+    b.requires_grad_()
+    y = ops.layer_norm(x, None, b)
+    z = ops.layer_norm(x, None, b)
+    with torch.no_grad():
+        b.add_(1)
+    for a, c in zip(torch.autograd.grad(y.sin().sum(), (x, b), create_graph=True),
+                    torch.autograd.grad(z.sin().sum(), (x, b))):
+        assert (a - c).abs().max() <= 400 * U
+
+
+@pytest.mark.gpu
+def test_linear_second_derivative_needs_the_bias_of_a_bent_slope():
+    x, w = (normal(seeded(), *s, device="cuda").requires_grad_() for s in ((3, 8), (5, 8)))
+    b = torch.zeros(5, device="cuda")
+    y = ops.linear(x, w, b, activation="gelu")
+    b.add_(1)
+    torch.autograd.grad(y.sum(), x, retain_graph=True)
+    with pytest.raises(RuntimeError, match="bias has been changed"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+@pytest.mark.parametrize("act", ["none", "relu", "silu"])
+@pytest.mark.parametrize("learnt", [(0,), (1,), (2,), (0, 1), (0, 2), (1, 2), (0, 1, 2)])
+def test_linear_derivatives_of_some_inputs(device, act, learnt):
+    """First and second derivatives, with the other inputs frozen."""
+    gen = seeded(9)
+    f = {"none": lambda z: z, "relu": F.relu, "silu": F.silu}[act]
+    tensors = [normal(gen, *s) for s in ((2, 3, 8), (5, 8), (5,))]
+    tensors[0][0, 0] = 0  # rows whose sum is the bias alone
+
+    def both(op, device, dtype):
+        t = [a.to(device=device, dtype=dtype, copy=True) for a in tensors]
+        leaves = [t[i].requires_grad_() for i in learnt]
+        y = op(*t)
+        up = torch.linspace(-1, 2, y.numel(), device=device, dtype=dtype).view(y.shape).requires_grad_()
+        first = torch.autograd.grad(y, leaves, up, create_graph=True)
+        plain = torch.autograd.grad(y, leaves, up, retain_graph=True)
+        second = torch.autograd.grad(sum((g * g).sum() for g in first), [*leaves, up],
+                                     materialize_grads=True)
+        return [g.detach() for g in (*first, *plain, *second)]
+
+    got = both(lambda *t: ops.linear(*t, activation=act), device, torch.float32)
+    for a, b in zip(got, both(lambda *t: f(F.linear(*t)), "cpu", torch.float64)):
+        assert a.shape == b.shape and (a.double().cpu() - b).norm() <= 2000 * U * b.norm()
