@@ -88,8 +88,9 @@ constexpr float NO_TARGET = 0.f, TARGET = 1.f, BAD_INDEX = 2.f;
 constexpr int SLOT_ROWS = 16; /* rows a workgroup of distill_slots */
 
 /* What the teacher says of a row, a wave each: the slots' masses, and
- * sum_k p_k (log p_k - (x[i_k] - o)/T) with o the greatest of the slots' logits,
- * to which the loss adds the log of the softmax's sum above o/T.  Where all of
+ * sum_k p_k (T log p_k - (x[i_k] - o)) with o the greatest of the slots' logits,
+ * to which the loss adds T times the log of the softmax's sum, above o; it is that
+ * sum times T, and finite where x/T need not be.  Where all of
  * the slots' logits are -inf, o is 0: the sum is then +inf, and not NaN.  A class that is
  * named twice is folded into its first slot, so that no two slots write to one
  * place of the gradient.  4096 rows of 64 slots: 18 us, most of it waiting for
@@ -140,7 +141,8 @@ __global__ __launch_bounds__(1024) void distill_slots(DistillArgs p) {
     if (origin == -INFINITY) origin = 0.f;
     for (int k = lane; k < p.top; k += 64) {
       float t = (sp[k] - high) * inv_t, log_p = t - log_mass, m = expf(t) / mass;
-      if (some && si[k] >= 0 && m != 0.f) loss += m * (log_p - (to_f<T>(x[si[k]]) - origin) * inv_t);
+      if (some && si[k] >= 0 && m != 0.f)
+        loss += m * (p.temperature * log_p - (to_f<T>(x[si[k]]) - origin));
       sp[k] = m;
     }
     loss = wave_sum(loss);
@@ -181,9 +183,8 @@ template <typename T>
 __device__ inline float finish(const DistillArgs &p, int64_t row, Run all) {
   float log_sum = logf(all.s), state = p.state[row];
   if (state == BAD_INDEX) log_sum = NAN;
-  float above = (all.m - p.origin[row]) / p.temperature + log_sum;
-  p.rows_loss[row] =
-      state == NO_TARGET ? 0.f : (p.rows_loss[row] + above) * p.temperature * p.temperature;
+  float above = (all.m - p.origin[row]) + p.temperature * log_sum;
+  p.rows_loss[row] = state == NO_TARGET ? 0.f : (p.rows_loss[row] + above) * p.temperature;
   if (p.most) {
     p.most[row] = all.m;
     p.log_sum[row] = log_sum;

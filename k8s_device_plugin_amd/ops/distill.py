@@ -98,10 +98,11 @@ def _plain(logits, index, teacher, temperature, reduction, scale):
     log_p = torch.log_softmax(t, -1).to(kind)
     x = torch.where(some.unsqueeze(-1), logits.to(kind), 0.0)
     most = x.detach().amax(-1, keepdim=True)  # so that no finite logit leaves its range
-    x = (x - torch.where(most.isfinite(), most, 0.0)) / temperature
-    log_q = torch.log_softmax(x, -1).gather(-1, index.long().clamp(0, logits.shape[-1] - 1))
-    p = torch.where(here, log_p.exp(), 0.0)
-    rows = torch.where(p != 0, p * (log_p - log_q), 0.0).sum(-1) * temperature ** 2
+    x = x - torch.where(most.isfinite(), most, 0.0)
+    lse = torch.logsumexp(x / temperature, -1, keepdim=True)
+    t_log_q = x.gather(-1, index.long().clamp(0, logits.shape[-1] - 1)) - temperature * lse
+    tp = torch.where(here, log_p.exp(), 0.0) * temperature
+    rows = torch.where(tp != 0, tp * (temperature * log_p - t_log_q), 0.0).sum(-1)
     rows = torch.where(some, rows, 0.0) * torch.where(bad, torch.nan, 1.0)
     if reduction == "none":
         return rows

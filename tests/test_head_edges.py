@@ -398,3 +398,28 @@ def test_linear_derivatives_of_some_inputs(device, act, learnt):
     got = both(lambda *t: ops.linear(*t, activation=act), device, torch.float32)
     for a, b in zip(got, both(lambda *t: f(F.linear(*t)), "cpu", torch.float64)):
         assert a.shape == b.shape and (a.double().cpu() - b).norm() <= 2000 * U * b.norm()
+
+
+@pytest.mark.parametrize("device,dtype", PAIRS)
+@pytest.mark.parametrize("t", [0.25, 0.5, 1.0])
+@pytest.mark.parametrize("top,v", [(1, 50), (3, 50), (1, 9000)])
+def test_distill_named_class_at_the_students_lowest_value(device, dtype, t, top, v):
+    """Where the loss is below fp32's greatest it is that, though x / T is not."""
+    logits, index, teacher = distill_inputs(3, v, top, dtype, device, seed=v)
+    low = torch.finfo(dtype).min
+    logits[1, index[1]] = low
+    logits[2, index[2, 0]] = low
+    leaf = logits.clone().requires_grad_()
+    loss = ops.distill_loss(leaf, index, teacher, temperature=t, reduction="none")
+    s = logits.double() / t
+    q = torch.log_softmax(s, 1).gather(1, index)
+    p = torch.softmax(teacher.double() / t, 1)
+    want = t * t * (p * (p.log() - q)).sum(1)
+    # masses off by p_off of themselves, products and sums by a few u
+    far = (teacher.double() / t).abs().amax(1)
+    off = U * (8 * far + 64 + v / 128 + top) * (t * t * (p * (p.log().abs() + q.abs())).sum(1) + 1)
+    within(loss.detach(), want, off)
+    grad, = torch.autograd.grad(loss, leaf, torch.ones_like(loss))
+    exact, slack = distill_gradient(logits.masked_fill(logits == low, -INF), index, teacher, t, 1.0)
+    # 16-bit logits: the hardware's power of two gives 0 for a result below 2^-126
+    within(grad[1:], exact[1:], slack[1:] + (0 if dtype == torch.float32 else t * 2.0 ** -126))
