@@ -45,7 +45,8 @@ __device__ inline f32x4 mma(const Frag<float> &a, const Frag<float> &b, f32x4 c,
  * every step.  It cannot see what these write: the caller keeps other products
  * between two into the same sum, and waits (settle) before it reads one.  Nor
  * does it put the two wait states between a vector instruction's write of a or b
- * and these: fragments come from LDS reads alone. */
+ * and these: fragments come from LDS reads alone.  A test reads the compiled
+ * code for both. */
 __device__ inline void mma_pinned(const Frag<bf16> &a, const Frag<bf16> &b, f32x4 &c, int) {
   asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a.v), "v"(b.v));
 }
@@ -90,8 +91,9 @@ __device__ inline u32x4 load16(u32x4 from, uint32_t offset) {
 /* 16 bytes a lane straight to LDS, at `to` + SKIP + 16 lane.  Written out
  * because the compiler, which cannot tell this buffer from the ones being read,
  * would wait for it before the next read of LDS; land_and_meet() does the
- * waiting.  It has no result.  m0 is no register that the compiler keeps values
- * in: it writes it anew before each instruction of its own that reads it. */
+ * waiting.  It has no result.  m0 is reserved, no register that the compiler keeps
+ * values in (it warns where a clobber names it): it writes it anew before each
+ * instruction of its own that reads it. */
 template <int SKIP>
 __device__ inline void load16_to_lds(u32x4 from, uint32_t offset, uint32_t to) {
   asm volatile(
