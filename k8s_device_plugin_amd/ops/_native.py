@@ -12,6 +12,7 @@ from pathlib import Path
 
 import torch
 from torch.autograd import forward_ad
+from torch.utils._device import DeviceContext
 
 PACKAGE = Path(__file__).resolve().parent.parent
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -64,9 +65,10 @@ def on_gpu(*tensors) -> bool:
     """Whether the kernels run: ordinary tensors on a GPU, and nothing that
     traces or transforms the call.  Otherwise the plain formula runs: so too
     for tensors whose sign is still to be turned, as conj()'s imaginary part,
-    inside forward-mode differentiation, and under a dispatch mode, which
-    records, counts or replaces torch's operations and would miss the call."""
-    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack():
+    inside forward-mode differentiation, and under a mode that records, counts
+    or replaces torch's operations and would miss the call."""
+    if (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack()
+            or (torch._C._len_torch_function_stack() and _watched())):
         return False
     for t in tensors:
         if t is not None and (type(t) not in _PLAIN_TENSORS or not t.is_cuda or t.is_neg()):
@@ -74,6 +76,12 @@ def on_gpu(*tensors) -> bool:
     return not (torch._C._get_tracing_state() is not None
                 or torch._C._are_functorch_transforms_active()
                 or forward_ad._current_level >= 0)
+
+
+def _watched() -> bool:
+    """Whether a function mode looks on, other than the default device's."""
+    return any(type(mode) is not DeviceContext
+               for mode in torch.overrides._get_current_function_mode_stack())
 
 
 _entries = {}   # name -> bound function

@@ -423,3 +423,25 @@ def test_distill_named_class_at_the_students_lowest_value(device, dtype, t, top,
     exact, slack = distill_gradient(logits.masked_fill(logits == low, -INF), index, teacher, t, 1.0)
     # 16-bit logits: the hardware's power of two gives 0 for a result below 2^-126
     within(grad[1:], exact[1:], slack[1:] + (0 if dtype == torch.float32 else t * 2.0 ** -126))
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_calls_under_a_function_mode_run_the_formula(device):
+    from torch.overrides import TorchFunctionMode
+
+    class Names(TorchFunctionMode):
+        def __torch_function__(self, f, types, args=(), kwargs=None):
+            seen.append(getattr(f, "__name__", str(f)))
+            return f(*args, **(kwargs or {}))
+
+    gen, seen = seeded(), []
+    x, w = normal(gen, 6, 700, device=device), normal(gen, 5, 700, device=device)
+    index = torch.zeros(6, 1, dtype=torch.long, device=device)
+    for call, name in ((lambda: ops.linear(x, w), "linear"), (lambda: ops.layer_norm(x), "layer_norm"),
+                       (lambda: ops.distill_loss(x, index), "gather")):
+        with Names():
+            call()
+        assert name in seen
+        want = call()
+        with torch.device(device):  # a default device is a mode too, which looks on at nothing
+            assert torch.equal(call(), want)
