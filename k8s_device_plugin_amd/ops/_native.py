@@ -172,6 +172,8 @@ def gradients_of(plain, inputs, needed, grad):
     formula is run again and differentiated.  It is run on aliases, so
     that each gradient stops at its own input where inputs depend on each other
     or are the same tensor: autograd goes on from there by itself."""
+    if not any(needed):
+        return [None] * len(inputs)
     again = torch.is_grad_enabled()
     with torch.enable_grad():
         inputs = [None if t is None else t.view_as(t) for t in inputs]

@@ -445,3 +445,36 @@ def test_calls_under_a_function_mode_run_the_formula(device):
         want = call()
         with torch.device(device):  # a default device is a mode too, which looks on at nothing
             assert torch.equal(call(), want)
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+def test_linear_with_a_gradient_in_the_residual_alone(device, act):
+    gen = seeded()
+    x, w = normal(gen, 3, 8, device=device), normal(gen, 5, 8, device=device)
+    r = normal(gen, 3, 5, device=device).requires_grad_()
+    y = ops.linear(x, w, activation=act, residual=r)
+    up = normal(gen, 3, 5, device=device).requires_grad_()
+    for graph in (False, True):
+        got, = torch.autograd.grad(y, r, up, retain_graph=True, create_graph=graph)
+        assert torch.equal(got, up)
+
+
+@pytest.mark.parametrize("device", ["cpu", GPU])
+def test_backward_alone_under_a_dispatch_mode(device):
+    from torch.utils.flop_counter import FlopCounterMode
+
+    gen = seeded()
+    x, w, b = (normal(gen, *s, device=device).requires_grad_() for s in ((6, 12), (12,), (12,)))
+    index = torch.arange(6, device=device)[:, None]
+    for y in (ops.layer_norm(x, w, b, groups=3), ops.layer_norm(x, None, b), ops.layer_norm(x),
+              ops.distill_loss(x, index), ops.distill_loss(x, index, reduction="none", temperature=2.0)):
+        leaves = [t for t in (x, w, b) if t is x or (y.dim() == 2 and torch.autograd.grad(
+            y.sum(), t, retain_graph=True, allow_unused=True)[0] is not None)]
+        up = normal(gen, *(y.shape or (1,)), device=device).reshape(y.shape)
+        want = torch.autograd.grad(y, leaves, up, retain_graph=True)
+        with FlopCounterMode(display=False):
+            got = torch.autograd.grad(y, leaves, up)
+        for a, c in zip(got, want):
+            # two evaluations of sums of fewer than 32 terms of ordinary size
+            assert a.dtype == c.dtype and not a.requires_grad and (a - c).abs().max() <= 400 * U
