@@ -510,8 +510,9 @@ __global__ __launch_bounds__(256) void gemm_join(GemmArgs p) {
  * product, so 16-bit values are only turned inside a lane.
  * LOOSE: rows of 16-bit values that start on 2 bytes, by loads that may.
  *
- * Bound by reading b.  1 x 4096 -> 4096 bf16: 9.4 us; 1 x 25088 -> 4096 fp32: 77
- * us, 5.3 TB/s, and with k strided (the gradient of 2 rows) 76 us, 5.4 TB/s. */
+ * Bound by reading b.  1 x 4096 -> 4096 bf16: 9.3 us; 1 x 25088 -> 4096 fp32: 77
+ * us, 5.3 TB/s, and 2 rows of it in a training step 95 us, 4.3 TB/s; with k strided
+ * (their gradient) 76 us, 5.4 TB/s. */
 template <typename T, bool BKC, bool LOOSE>
 __global__ __launch_bounds__(512, BKC ? 4 : 2) void gemm_rows(GemmArgs p) {
   constexpr int V = Vec<T>::N, WAVES = 8;
